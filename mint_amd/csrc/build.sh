@@ -9,7 +9,9 @@ cd "$(dirname "$0")"
 OUT=../lib
 mkdir -p "$OUT" "$OUT/obj"
 HIPCC=${HIPCC:-/opt/rocm/bin/hipcc}
-FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -fvisibility=hidden -fvisibility-inlines-hidden -Wno-unused-result $FACT_EXTRA_FLAGS"
+# packed fp32 instructions off: some forms that -O3 makes of ordinary float code have given wrong results on this hardware
+# now and then (the host pass warns that it does not know the feature)
+FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -fvisibility=hidden -fvisibility-inlines-hidden -Wno-unused-result -Xclang -target-feature -Xclang -packed-fp32-ops $FACT_EXTRA_FLAGS"
 # the flag set is part of the object cache key: a default build after a variant build (FACT_EXTRA_FLAGS=-D...) must not
 # link the variant's objects into the shipped library, nor the other way round
 if [ "$(cat "$OUT/obj/.flags" 2>/dev/null)" != "$FLAGS" ]; then

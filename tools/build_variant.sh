@@ -10,7 +10,7 @@ name=$1; unit=$2; shift 2
 mkdir -p $R/tools/bin /tmp/fact_variant
 [ -f $R/mint_amd/lib/obj/gemm.o ] || $R/mint_amd/csrc/build.sh
 # (the variant is a test / bench build: engine.hip / probe.hip with the debug surface, mint_amd/csrc/build.sh)
-hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -fvisibility=hidden -fvisibility-inlines-hidden -Wno-unused-result -DFACT_DEBUG_ABI "$@" -c $R/mint_amd/csrc/$unit.hip -o /tmp/fact_variant/$unit.$name.o
+hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -fvisibility=hidden -fvisibility-inlines-hidden -Wno-unused-result -Xclang -target-feature -Xclang -packed-fp32-ops -DFACT_DEBUG_ABI "$@" -c $R/mint_amd/csrc/$unit.hip -o /tmp/fact_variant/$unit.$name.o
 objs=""
 for f in gemm gemm_big rowops attention engine_dbg probe_dbg; do
   if [ ${f%_dbg} = $unit ]; then objs="$objs /tmp/fact_variant/$unit.$name.o"; else objs="$objs $R/mint_amd/lib/obj/$f.o"; fi
