@@ -206,6 +206,83 @@ int fact_set_grad_callback(FactHandle* h, fact_grad_cb cb, void* user, void* com
  *                        add a communication stream (data parallelism) set 0 to stay within the hardware queues */
 int fact_set_option(FactHandle* h, const char* key, int value);
 
+/* ---- attention operators with relative positions --------------------------------------------------------------------
+ * Handle-free operators on caller tensors (bf16 unless stated); the engine runs the same kernels for a stack whose
+ * FactAttnCfg asks for them (fact_create_ex).  No allocation, no host synchronisation and no memset nodes: every call can be
+ * captured into a HIP graph.  Row-major tensors [batch][token][head][dh] given by a pointer and three element strides
+ * (batch, token, head); the dh values of a head are contiguous; pointers are 16-byte aligned, strides multiples of 8.  Input
+ * strides may be 0 (a broadcast input); outputs must not overlap each other or an input unless stated. */
+
+/* Attention with an optional sliding window, sinks and a learned relative position bias by buckets.
+ *   position of query row i of sequence b   p = (q_start ? q_start[b] : 0) + i
+ *   key j is visible from p iff             j < len_b (len_b = kv_len ? clamp(kv_len[b], 0, nk) : nk),
+ *                                           window_right < 0 or j <= p + window_right,
+ *                                           window_left  < 0 or j >= p - window_left or j < sinks
+ *   s_ij = scale * q_i . k_j + (rel_table ? rel_table[m(j - p)][h] : 0),  m(d) = rel_map[clamp(d, -D, D) + D]
+ *   out_i = softmax over the visible keys of s_i, times v; a row that sees no key (or only keys whose bias is -inf) gives 0
+ * H query heads, head h reads key / value head h / (H / Hkv).  dh 32, 64, 80, 96 or 128.  Keys and values at j >= len_b are
+ * not read.  Scores, softmax statistics and all sums are fp32; the probabilities enter the second product as bf16.
+ * Every sum (over heads that share keys, over the splits of a long key range, over the positions behind a bucket) has a fixed
+ * order: results do not change from run to run. */
+typedef struct FactAttention {
+  const void *q, *k, *v;   /* [B][nq][H][dh], [B][nk][Hkv][dh] twice */
+  void* out;               /* [B][nq][H][dh] */
+  void* out_lo;            /* may be NULL: bf16 rounding residual of `out` (layout of out).  With it the forward's product with v
+                            * carries the probabilities to 16 bits and the backward's row sums dO . O take out + out_lo: what
+                            * the fp32 gradient of the table needs */
+  float* lse;              /* [B][H][nq] base-2 log-sum-exp of the scaled scores (+inf: row without keys); forward: may be NULL */
+  const void* dout;        /* backward: gradient of out */
+  void *dq, *dk, *dv;      /* backward: written */
+  float* drel;             /* backward with rel_table: fp32 gradient [rel_buckets][H] */
+  const float* rel_table;  /* [rel_buckets][H] fp32, or NULL */
+  const int32_t* rel_map;  /* [2 * rel_max_distance + 1] bucket of each clipped distance (values are clamped to the table) */
+  const int32_t* kv_len;   /* device [B], or NULL */
+  const int32_t* q_start;  /* device [B], or NULL */
+  int64_t q_stride[3], k_stride[3], v_stride[3], out_stride[3], dout_stride[3], dq_stride[3], dk_stride[3], dv_stride[3];
+  int B, H, Hkv, nq, nk, dh;
+  int window_left, window_right, sinks;
+  int rel_buckets, rel_max_distance; /* 1..256 buckets, D 1..1024 */
+  int drel_accumulate;               /* 1: drel += gradient, 0: drel = gradient */
+  float scale;                       /* > 0, at least 2^-24 */
+} FactAttention;
+/* Device bytes of the workspace of a call (16-byte aligned; contents need no initialisation and carry nothing between
+ * calls; two calls that may run at the same time need one each). */
+int fact_attention_workspace(const FactAttention* a, int backward, size_t* bytes);
+int fact_attention(const FactAttention* a, void* workspace, size_t workspace_bytes, void* stream);
+/* Needs q, k, v, out, lse (and out_lo if the forward wrote it) of the forward call and the same shapes and options. */
+int fact_attention_backward(const FactAttention* a, void* workspace, size_t workspace_bytes, void* stream);
+/* Host utility: the logarithmic bucket map of 2 * max_distance + 1 clipped distances d = key - query, -max_distance first.
+ * One side has n buckets (num_buckets / 2 when bidirectional - keys after the query take the upper half - else num_buckets;
+ * without bidirectional keys after the query share bucket 0): n / 2 buckets of one distance each, then
+ * n/2 + floor(log(|d| / (n/2)) / log(max_distance / (n/2)) * (n - n/2)), at most n - 1, computed in integers. */
+int fact_relative_buckets(int num_buckets, int max_distance, int bidirectional, int32_t* map);
+
+
+/* RMS norm of every query and key head with a learned gain, then rotation by position, in one pass:
+ *   y = x * rsqrt(mean(x^2) + eps) * gamma;  pairs of the first rotary_dim values turned by pos * base^(-2 i / rotary_dim)
+ * Pair i is (i, i + rotary_dim / 2), or (2 i, 2 i + 1) with interleaved.  dtype 0 = bf16, 1 = fp32 (all tensors but the
+ * fp32 gains and the int32 positions).  dh a multiple of 8 up to 128, rotary_dim a multiple of 8 up to dh (0: no rotation).
+ * Outputs may be the inputs themselves (same pointer and strides). */
+typedef struct FactQkNorm {
+  const void *q, *k;            /* [B][n][H][dh], [B][n][Hkv][dh]: the projections (both directions) */
+  void *q_out, *k_out;          /* forward */
+  const void *dq_out, *dk_out;  /* backward: gradients of q_out, k_out */
+  void *dq, *dk;                /* backward: gradients of q, k (may be dq_out, dk_out) */
+  const float *q_gamma, *k_gamma; /* [dh] fp32, or NULL for 1 */
+  float *dq_gamma, *dk_gamma;     /* backward: [dh] fp32, either may be NULL */
+  const int32_t* positions;       /* device, [B][n] through position_stride, or NULL: position0 + token index */
+  int64_t q_stride[3], k_stride[3], q_out_stride[3], k_out_stride[3], dq_out_stride[3], dk_out_stride[3], dq_stride[3],
+      dk_stride[3], position_stride[2];
+  double base;                    /* > 0 */
+  int B, n, H, Hkv, dh, rotary_dim, interleaved, dtype;
+  int position0;
+  int dgamma_accumulate;          /* 1: dgamma += gradient, 0: dgamma = gradient */
+  float eps;
+} FactQkNorm;
+int fact_qk_norm_workspace(const FactQkNorm* a, int backward, size_t* bytes);
+int fact_qk_norm(const FactQkNorm* a, void* workspace, size_t workspace_bytes, void* stream);
+int fact_qk_norm_backward(const FactQkNorm* a, void* workspace, size_t workspace_bytes, void* stream);
+
 #if defined(__GNUC__) || defined(__clang__)
 #pragma GCC visibility pop
 #endif

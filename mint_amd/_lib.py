@@ -46,6 +46,25 @@ class FactArenas(C.Structure):
                 ("adam_v", C.c_void_p)]
 
 
+class FactAttention(C.Structure):
+    _fields_ = ([(n, C.c_void_p) for n in ("q", "k", "v", "out", "out_lo", "lse", "dout", "dq", "dk", "dv", "drel", "rel_table",
+                                           "rel_map", "kv_len", "q_start")]
+                + [(n + "_stride", C.c_int64 * 3) for n in ("q", "k", "v", "out", "dout", "dq", "dk", "dv")]
+                + [(n, C.c_int) for n in ("B", "H", "Hkv", "nq", "nk", "dh", "window_left", "window_right", "sinks",
+                                          "rel_buckets", "rel_max_distance", "drel_accumulate")]
+                + [("scale", C.c_float)])
+
+
+class FactQkNorm(C.Structure):
+    _fields_ = ([(n, C.c_void_p) for n in ("q", "k", "q_out", "k_out", "dq_out", "dk_out", "dq", "dk", "q_gamma", "k_gamma",
+                                           "dq_gamma", "dk_gamma", "positions")]
+                + [(n + "_stride", C.c_int64 * 3) for n in ("q", "k", "q_out", "k_out", "dq_out", "dk_out", "dq", "dk")]
+                + [("position_stride", C.c_int64 * 2), ("base", C.c_double)]
+                + [(n, C.c_int) for n in ("B", "n", "H", "Hkv", "dh", "rotary_dim", "interleaved", "dtype", "position0",
+                                          "dgamma_accumulate")]
+                + [("eps", C.c_float)])
+
+
 # fact_grad_cb: void (*)(void* user, int bucket, size_t offset_floats, size_t count_floats)
 GRAD_CB = C.CFUNCTYPE(None, C.c_void_p, C.c_int, C.c_size_t, C.c_size_t)
 
@@ -71,6 +90,13 @@ SIGNATURES = {
     "fact_adam_cancel": (_i, [_vp]),
     "fact_num_buckets": (_i, [_vp, C.POINTER(_i)]),
     "fact_loss": (_i, [_vp, _vp, _i, _i, _i, _i, _vp, _vp]),
+    "fact_attention_workspace": (_i, [C.POINTER(FactAttention), _i, C.POINTER(_sz)]),
+    "fact_attention": (_i, [C.POINTER(FactAttention), _vp, _sz, _vp]),
+    "fact_attention_backward": (_i, [C.POINTER(FactAttention), _vp, _sz, _vp]),
+    "fact_relative_buckets": (_i, [_i, _i, _i, C.POINTER(C.c_int32)]),
+    "fact_qk_norm_workspace": (_i, [C.POINTER(FactQkNorm), _i, C.POINTER(_sz)]),
+    "fact_qk_norm": (_i, [C.POINTER(FactQkNorm), _vp, _sz, _vp]),
+    "fact_qk_norm_backward": (_i, [C.POINTER(FactQkNorm), _vp, _sz, _vp]),
     "fact_kprof": (_i, [_vp, _i]),
     "fact_kprof_dump": (_i, [_vp, C.c_char_p]),
     "fact_kprof_read": (_i, [_vp, _i, C.POINTER(_i), C.POINTER(C.c_char_p), C.POINTER(C.c_double),

@@ -1,0 +1,274 @@
+"""Attention operators with relative positions on the HIP engine (include/fact_hip.h FactAttention, FactQkNorm).
+
+    qk_norm_rope / qk_norm_rope_backward   RMS norm of each query and key head with a learned gain, then rotation by position
+    attention / attention_backward         sliding window, sinks, learned relative position bias by buckets
+    relative_buckets                       the logarithmic bucket map of the clipped distances
+
+Tensors are [batch, token, head, dh] CUDA tensors of any strides whose last dimension is contiguous (views of one packed
+projection are read in place; what the kernels cannot address is copied first).  Calls run on the current stream of the
+tensors' device, never synchronise, and take their scratch memory from torch's allocator per call, so they can be captured into
+graphs and run on several streams at once.  There is no autograd: as in the engine, the backward is a call of its own.
+Models use the same kernels through the transformer options of their config (mint_amd/protos.py).
+"""
+import collections
+import ctypes as C
+
+import torch
+
+from mint_amd import _lib as L
+
+AttentionSaved = collections.namedtuple("AttentionSaved", ["lse", "out_lo"])
+AttentionSaved.__doc__ = """What attention(training=True) leaves for the backward: the base-2 log-sum-exp of every row, fp32
+[batch, heads, queries], and - with a relative bias - the rounding residual of the output (its row sums enter the fp32 gradient
+of the table)."""
+
+DTYPES = {torch.bfloat16: 0, torch.float32: 1}
+
+
+def relative_buckets(num_buckets, max_distance, bidirectional=True, device=None):
+    """int32 [2 * max_distance + 1]: bucket of each distance key - query clipped to +-max_distance.  Half of a side's buckets
+    hold one distance each, the rest grow by equal ratios up to max_distance; with `bidirectional` keys after the query have the
+    upper half of the buckets, without it they share bucket 0."""
+    got = (C.c_int32 * (2 * max(0, int(max_distance)) + 1))()
+    L.check(L.lib().fact_relative_buckets(int(num_buckets), int(max_distance), 1 if bidirectional else 0, got))
+    return torch.tensor(list(got), dtype=torch.int32, device=device)
+
+
+def _need(cond, msg, *args):
+    if not cond:
+        raise ValueError(msg % args)
+
+
+def _heads(t, name, dtype, device=None):
+    """A [batch, token, head, dh] tensor that the kernels can read in place, or a contiguous copy of it."""
+    _need(torch.is_tensor(t) and t.dim() == 4, "%s must be a [batch, token, head, dh] tensor", name)
+    _need(t.is_cuda, "%s must be a CUDA tensor: there is no CPU path", name)
+    _need(device is None or t.device == device, "%s is on %s, expected %s", name, t.device, device)
+    if dtype is not None:
+        _need(t.dtype == dtype, "%s must be %s, not %s", name, dtype, t.dtype)
+    return t if _addressable(t) else t.clone(memory_format=torch.contiguous_format)
+
+
+def _addressable(t):
+    s = t.stride()
+    return s[3] == 1 and not (s[0] | s[1] | s[2]) & 7 and not t.data_ptr() & 15
+
+
+def _dest(t, name, shape, dtype, device):
+    """A caller's output tensor (written in place: it has to be addressable), or a new one."""
+    if t is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    _need(torch.is_tensor(t) and t.shape == torch.Size(shape) and t.dtype == dtype and t.device == device,
+          "%s must be a %s tensor of shape %s on %s", name, dtype, tuple(shape), device)
+    _need(_addressable(t), "%s must have a contiguous last dimension, 16-byte alignment and strides that are multiples of 8", name)
+    _need(all(t.stride(i) for i in range(3) if t.shape[i] > 1), "%s must not be a broadcast tensor", name)
+    return t
+
+
+def _vector(t, name, shape, dtype, device):
+    if t is None:
+        return None
+    _need(torch.is_tensor(t) and t.dtype == dtype and t.device == device and t.shape == torch.Size(shape),
+          "%s must be a %s tensor of shape %s on %s", name, dtype, tuple(shape), device)
+    return t if t.is_contiguous() and not t.data_ptr() & 15 else t.clone(memory_format=torch.contiguous_format)
+
+
+def _p(t):
+    return None if t is None else t.data_ptr()
+
+
+def _set(a, name, t):
+    setattr(a, name, t.data_ptr())
+    s = t.stride()
+    getattr(a, name + "_stride")[:] = (s[0], s[1], s[2])
+
+
+class _On:
+    """The device of a call's tensors made current, if it is not."""
+
+    def __init__(self, device):
+        self.device = device
+
+    def __enter__(self):
+        self.before = torch.cuda.current_device()
+        if self.before != self.device.index:
+            torch.cuda.set_device(self.device)
+        return C.c_void_p(torch.cuda.current_stream(self.device).cuda_stream)
+
+    def __exit__(self, *exc):
+        if self.before != self.device.index:
+            torch.cuda.set_device(self.before)
+
+
+def _workspace(fn, a, backward, device):
+    n = C.c_size_t(0)
+    L.check(fn(C.byref(a), backward, C.byref(n)))
+    return (torch.empty(n.value, dtype=torch.uint8, device=device) if n.value else None), n.value
+
+
+# ---- attention ------------------------------------------------------------------------------------------------------
+def _attention_args(q, k, v, scale, window, sinks, rel_table, rel_map, kv_len, q_start):
+    q = _heads(q, "q", torch.bfloat16)
+    dev = q.device
+    k, v = _heads(k, "k", torch.bfloat16, dev), _heads(v, "v", torch.bfloat16, dev)
+    B, nq, H, dh = q.shape
+    _need(k.shape == v.shape and k.shape[0] == B and k.shape[3] == dh, "k and v must be [%d, tokens, heads, %d], got %s and %s",
+          B, dh, tuple(k.shape), tuple(v.shape))
+    nk, Hkv = k.shape[1], k.shape[2]
+    _need(Hkv > 0 and H % Hkv == 0, "the %d query heads must be a multiple of the %d key heads", H, Hkv)
+    window = (-1, -1) if window is None else window
+    _need(len(window) == 2, "window must be (left, right)")
+    a = L.FactAttention(B=B, H=H, Hkv=Hkv, nq=nq, nk=nk, dh=dh, window_left=int(window[0]), window_right=int(window[1]),
+                        sinks=int(sinks), scale=float(dh ** -0.5 if scale is None else scale))
+    _need((rel_table is None) == (rel_map is None), "rel_table and rel_map belong together")
+    if rel_table is not None:
+        _need(torch.is_tensor(rel_table) and rel_table.dim() == 2 and rel_table.shape[1] == H,
+              "rel_table must be [buckets, %d]", H)
+        _need(torch.is_tensor(rel_map) and rel_map.dim() == 1 and rel_map.numel() >= 3 and rel_map.numel() % 2 == 1,
+              "rel_map must hold the bucket of 2 * max_distance + 1 distances")
+        rel_table = _vector(rel_table, "rel_table", rel_table.shape, torch.float32, dev)
+        rel_map = _vector(rel_map, "rel_map", rel_map.shape, torch.int32, dev)
+        a.rel_table, a.rel_map = rel_table.data_ptr(), rel_map.data_ptr()
+        a.rel_buckets, a.rel_max_distance = rel_table.shape[0], rel_map.numel() // 2
+    kv_len = _vector(kv_len, "kv_len", (B,), torch.int32, dev)
+    q_start = _vector(q_start, "q_start", (B,), torch.int32, dev)
+    a.kv_len, a.q_start = _p(kv_len), _p(q_start)
+    _set(a, "q", q)
+    _set(a, "k", k)
+    _set(a, "v", v)
+    return a, (q, k, v, rel_table, rel_map, kv_len, q_start)  # (the copies live until the launch is enqueued)
+
+
+def attention(q, k, v, scale=None, window=None, sinks=0, rel_table=None, rel_map=None, kv_len=None, q_start=None,
+              training=False, out=None):
+    """Attention of q [B, nq, H, dh] over k, v [B, nk, Hkv, dh], bf16; head h reads key head h // (H // Hkv).
+
+    Query row i of sequence b stands at position q_start[b] + i (0 + i without q_start) and sees the keys j with j < kv_len[b],
+    j <= position + window[1] and (j >= position - window[0] or j < sinks); a negative window side is open.  rel_table
+    [buckets, H] fp32 adds rel_table[rel_map[clip(j - position)]][h] to scale * q . k.  A row that sees no key gives zeros.
+    Keys and values at and after kv_len are never read.  Returns out [B, nq, H, dh], with `training` (out, AttentionSaved)."""
+    a, held = _attention_args(q, k, v, scale, window, sinks, rel_table, rel_map, kv_len, q_start)
+    dev = held[0].device
+    shape = (a.B, a.nq, a.H, a.dh)
+    out = _dest(out, "out", shape, torch.bfloat16, dev)
+    saved = None
+    if 0 in shape:
+        return (out, AttentionSaved(out.new_empty((a.B, a.H, a.nq), dtype=torch.float32), None)) if training else out
+    if a.nk == 0:
+        out.zero_()
+        lse = torch.full((a.B, a.H, a.nq), float("inf"), device=dev) if training else None
+        return (out, AttentionSaved(lse, None)) if training else out
+    _set(a, "out", out)
+    if training:
+        lse = torch.empty((a.B, a.H, a.nq), dtype=torch.float32, device=dev)
+        lo = torch.empty_strided(out.shape, out.stride(), dtype=out.dtype, device=dev) if rel_table is not None else None
+        saved = AttentionSaved(lse, lo)
+        a.lse, a.out_lo = lse.data_ptr(), _p(lo)
+    with _On(dev) as stream:
+        ws, n = _workspace(L.lib().fact_attention_workspace, a, 0, dev)
+        L.check(L.lib().fact_attention(C.byref(a), _p(ws), n, stream))
+    return (out, saved) if training else out
+
+
+def attention_backward(dout, q, k, v, out, saved, scale=None, window=None, sinks=0, rel_table=None, rel_map=None, kv_len=None,
+                       q_start=None, dq=None, dk=None, dv=None):
+    """Gradients of attention(..., training=True) for dout [B, nq, H, dh]: (dq, dk, dv), with a relative bias also the fp32
+    gradient of rel_table.  `out` and `saved` are what the forward returned; dq, dk, dv may be given (views of one packed
+    gradient, for instance)."""
+    a, held = _attention_args(q, k, v, scale, window, sinks, rel_table, rel_map, kv_len, q_start)
+    dev = held[0].device
+    shape = torch.Size((a.B, a.nq, a.H, a.dh))
+    dout, out = _heads(dout, "dout", torch.bfloat16, dev), _heads(out, "out", torch.bfloat16, dev)
+    _need(dout.shape == shape and out.shape == shape, "dout and out must be %s", tuple(shape))
+    _need(isinstance(saved, AttentionSaved), "saved must be what attention(training=True) returned")
+    dq = _dest(dq, "dq", q.shape, torch.bfloat16, dev)
+    dk = _dest(dk, "dk", k.shape, torch.bfloat16, dev)
+    dv = _dest(dv, "dv", v.shape, torch.bfloat16, dev)
+    drel = None
+    if rel_table is not None:
+        drel = torch.empty((a.rel_buckets, a.H), dtype=torch.float32, device=dev)
+    if 0 in shape or a.nk == 0:
+        for t in (dq, dk, dv, drel):
+            if t is not None:
+                t.zero_()
+        return (dq, dk, dv) if drel is None else (dq, dk, dv, drel)
+    lse = _vector(saved.lse, "saved.lse", (a.B, a.H, a.nq), torch.float32, dev)
+    lo = saved.out_lo
+    if lo is not None:
+        _need(lo.shape == shape and lo.dtype == torch.bfloat16 and lo.device == dev, "saved.out_lo must be %s", tuple(shape))
+        if lo.stride() != out.stride() or lo.data_ptr() & 15:  # (the two are read with one set of strides)
+            out, lo = out.contiguous(), lo.contiguous()
+    for name, t in (("out", out), ("dout", dout), ("dq", dq), ("dk", dk), ("dv", dv)):
+        _set(a, name, t)
+    a.lse, a.out_lo, a.drel = lse.data_ptr(), _p(lo), _p(drel)
+    with _On(dev) as stream:
+        ws, n = _workspace(L.lib().fact_attention_workspace, a, 1, dev)
+        L.check(L.lib().fact_attention_backward(C.byref(a), _p(ws), n, stream))
+    return (dq, dk, dv) if drel is None else (dq, dk, dv, drel)
+
+
+# ---- norm of queries and keys with rotation ---------------------------------------------------------------------------
+def _norm_args(q, k, q_gamma, k_gamma, eps, rotary_dim, base, interleaved, positions, position0):
+    q = _heads(q, "q", None)
+    _need(q.dtype in DTYPES, "q must be bfloat16 or float32, not %s", q.dtype)
+    dev = q.device
+    k = _heads(k, "k", q.dtype, dev)
+    B, n, H, dh = q.shape
+    _need(k.shape[0] == B and k.shape[1] == n and k.shape[3] == dh, "k must be [%d, %d, heads, %d], got %s", B, n, dh,
+          tuple(k.shape))
+    q_gamma = _vector(q_gamma, "q_gamma", (dh,), torch.float32, dev)
+    k_gamma = _vector(k_gamma, "k_gamma", (dh,), torch.float32, dev)
+    a = L.FactQkNorm(B=B, n=n, H=H, Hkv=k.shape[2], dh=dh, rotary_dim=dh if rotary_dim is None else int(rotary_dim),
+                     interleaved=1 if interleaved else 0, dtype=DTYPES[q.dtype], position0=int(position0), eps=float(eps),
+                     base=float(base), q_gamma=_p(q_gamma), k_gamma=_p(k_gamma))
+    if positions is not None:
+        _need(torch.is_tensor(positions) and positions.dtype == torch.int32 and positions.device == dev
+              and tuple(positions.shape) in ((B, n), (n,)), "positions must be an int32 tensor of shape %s or %s on %s",
+              (B, n), (n,), dev)
+        positions = positions.expand(B, n)
+        a.positions = positions.data_ptr()
+        a.position_stride[:] = positions.stride()
+    _set(a, "q", q)
+    _set(a, "k", k)
+    return a, (q, k, q_gamma, k_gamma, positions)
+
+
+def qk_norm_rope(q, k, q_gamma=None, k_gamma=None, eps=1e-6, rotary_dim=None, base=10000.0, interleaved=False, positions=None,
+                 position0=0, q_out=None, k_out=None):
+    """x * rsqrt(mean(x^2) + eps) * gamma of every head of q [B, n, H, dh] and k [B, n, Hkv, dh] (bf16 or fp32; gains fp32 [dh],
+    None: 1), then the first rotary_dim values (None: all, 0: none) of each head turned in pairs by
+    position * base^(-2 i / rotary_dim).  Pair i is (i, i + rotary_dim / 2), `interleaved` (2 i, 2 i + 1).  positions: int32
+    [B, n] or [n]; without it position0 + token.  Returns (q, k); q_out / k_out may be q / k themselves."""
+    a, held = _norm_args(q, k, q_gamma, k_gamma, eps, rotary_dim, base, interleaved, positions, position0)
+    dev = held[0].device
+    q_out = _dest(q_out, "q_out", q.shape, q.dtype, dev)
+    k_out = _dest(k_out, "k_out", k.shape, q.dtype, dev)
+    if a.B == 0 or a.n == 0:
+        return q_out, k_out
+    _set(a, "q_out", q_out)
+    _set(a, "k_out", k_out)
+    with _On(dev) as stream:
+        L.check(L.lib().fact_qk_norm(C.byref(a), None, 0, stream))
+    return q_out, k_out
+
+
+def qk_norm_rope_backward(dq_out, dk_out, q, k, q_gamma=None, k_gamma=None, eps=1e-6, rotary_dim=None, base=10000.0,
+                          interleaved=False, positions=None, position0=0, dq=None, dk=None):
+    """Gradients of qk_norm_rope for (dq_out, dk_out), from the forward's INPUTS q, k: (dq, dk, dq_gamma, dk_gamma), the last two
+    fp32 [dh].  dq / dk may be dq_out / dk_out themselves."""
+    a, held = _norm_args(q, k, q_gamma, k_gamma, eps, rotary_dim, base, interleaved, positions, position0)
+    dev = held[0].device
+    dq_in, dk_in = _heads(dq_out, "dq_out", q.dtype, dev), _heads(dk_out, "dk_out", q.dtype, dev)
+    _need(dq_in.shape == q.shape and dk_in.shape == k.shape, "dq_out and dk_out must have the shapes of q and k")
+    dq, dk = _dest(dq, "dq", q.shape, q.dtype, dev), _dest(dk, "dk", k.shape, q.dtype, dev)
+    gains = torch.empty((2, a.dh), dtype=torch.float32, device=dev)
+    if a.B == 0 or a.n == 0:
+        gains.zero_()
+        return dq, dk, gains[0], gains[1]
+    for name, t in (("dq_out", dq_in), ("dk_out", dk_in), ("dq", dq), ("dk", dk)):
+        _set(a, name, t)
+    a.dq_gamma, a.dk_gamma = gains.data_ptr(), gains.data_ptr() + 4 * a.dh
+    with _On(dev) as stream:
+        ws, n = _workspace(L.lib().fact_qk_norm_workspace, a, 1, dev)
+        L.check(L.lib().fact_qk_norm_backward(C.byref(a), _p(ws), n, stream))
+    return dq, dk, gains[0], gains[1]

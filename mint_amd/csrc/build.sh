@@ -22,7 +22,7 @@ pids=()
 stale() {  # $1 = object, $2 = source
   [ ! -f "$1" ] || [ "$2" -nt "$1" ] || [ -n "$(find . ../../include -name '*.h' -newer "$1" 2>/dev/null)" ]
 }
-for f in gemm gemm_big rowops attention engine probe; do
+for f in gemm gemm_big rowops attention rel_attention qk_norm engine probe; do
   if stale "$OUT/obj/$f.o" "$f.hip"; then
     $HIPCC $FLAGS -c "$f.hip" -o "$OUT/obj/$f.o" &
     pids+=($!)
@@ -35,7 +35,7 @@ for f in engine probe; do
   fi
 done
 for p in "${pids[@]}"; do wait "$p"; done
-COMMON="$OUT/obj/gemm.o $OUT/obj/gemm_big.o $OUT/obj/rowops.o $OUT/obj/attention.o"
+COMMON="$OUT/obj/gemm.o $OUT/obj/gemm_big.o $OUT/obj/rowops.o $OUT/obj/attention.o $OUT/obj/rel_attention.o $OUT/obj/qk_norm.o"
 $HIPCC --offload-arch=gfx950 -shared -fPIC -Wl,--version-script=exports.map -o "$OUT/libfact_hip.so" $COMMON "$OUT/obj/engine.o" "$OUT/obj/probe.o"
 $HIPCC --offload-arch=gfx950 -shared -fPIC -Wl,--version-script=exports.map -o "$OUT/libfact_hip_dbg.so" $COMMON "$OUT/obj/engine_dbg.o" "$OUT/obj/probe_dbg.o"
 echo "built $OUT/libfact_hip.so $OUT/libfact_hip_dbg.so"

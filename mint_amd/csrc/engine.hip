@@ -15,6 +15,7 @@
 #include "../../include/fact_hip_debug.h"
 #include "attention.h"
 #include "gemm.h"
+#include "rel_attention.h"
 #include "rowops.h"
 
 #include <algorithm>
@@ -2631,6 +2632,69 @@ int fact_loss(const float* target, const float* pred, int B, int n, int T, int D
   if (B <= 0 || n <= 0 || T <= 0 || T > n || D <= 0) return fail(-1, "loss: need 0 < T <= n");
   HIPCHK(hipMemsetAsync(loss_out, 0, sizeof(float), (hipStream_t)stream));
   CHK(launch_mse_loss(pred, target, loss_out, nullptr, B, n, T, D, rup(D, 32), 1.0f, (hipStream_t)stream));
+  return 0;
+}
+
+// ---- attention with relative positions, q / k norm (rel_attention.hip, qk_norm.hip) -------------------------------------
+namespace {
+int fail_op(int rc, const char* op, const char* why) { return fail(rc, std::string(op) + ": " + why); }
+int check_ws(const char* op, const void* ws, size_t have, size_t need) {
+  if (need && (!ws || have < need)) return fail(-4, std::string(op) + ": workspace of " + std::to_string(need) + " bytes needed");
+  if ((uintptr_t)ws & 15) return fail(-1, std::string(op) + ": the workspace must be 16-byte aligned");
+  return 0;
+}
+}  // namespace
+
+int fact_attention_workspace(const FactAttention* a, int backward, size_t* bytes) {
+  if (!a || !bytes) return fail(-1, "null argument");
+  const char* why = "";
+  if (int rc = rel_attention_check(*a, backward != 0, &why)) return fail_op(rc, "fact_attention_workspace", why);
+  *bytes = rel_attention_ws(*a, backward != 0);
+  return 0;
+}
+int fact_attention(const FactAttention* a, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!a) return fail(-1, "null argument");
+  const char* why = "";
+  if (int rc = rel_attention_check(*a, false, &why)) return fail_op(rc, "fact_attention", why);
+  if (int rc = check_ws("fact_attention", workspace, workspace_bytes, rel_attention_ws(*a, false))) return rc;
+  CHK(launch_rel_attention_fwd(*a, workspace, (hipStream_t)stream));
+  return 0;
+}
+int fact_attention_backward(const FactAttention* a, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!a) return fail(-1, "null argument");
+  const char* why = "";
+  if (int rc = rel_attention_check(*a, true, &why)) return fail_op(rc, "fact_attention_backward", why);
+  if (int rc = check_ws("fact_attention_backward", workspace, workspace_bytes, rel_attention_ws(*a, true))) return rc;
+  CHK(launch_rel_attention_bwd(*a, workspace, (hipStream_t)stream));
+  return 0;
+}
+int fact_relative_buckets(int num_buckets, int max_distance, int bidirectional, int32_t* map) {
+  if (relative_buckets(num_buckets, max_distance, bidirectional, map))
+    return fail(-1, "fact_relative_buckets: 2..256 buckets (an even number when bidirectional), at least 2 a side, and a largest "
+                    "distance above the exact ones, at most 1024");
+  return 0;
+}
+int fact_qk_norm_workspace(const FactQkNorm* a, int backward, size_t* bytes) {
+  if (!a || !bytes) return fail(-1, "null argument");
+  const char* why = "";
+  if (int rc = qk_norm_check(*a, backward != 0, &why)) return fail_op(rc, "fact_qk_norm_workspace", why);
+  *bytes = qk_norm_ws(*a, backward != 0);
+  return 0;
+}
+int fact_qk_norm(const FactQkNorm* a, void* workspace, size_t workspace_bytes, void* stream) {
+  (void)workspace; (void)workspace_bytes;
+  if (!a) return fail(-1, "null argument");
+  const char* why = "";
+  if (int rc = qk_norm_check(*a, false, &why)) return fail_op(rc, "fact_qk_norm", why);
+  CHK(launch_qk_norm_fwd(*a, (hipStream_t)stream));
+  return 0;
+}
+int fact_qk_norm_backward(const FactQkNorm* a, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!a) return fail(-1, "null argument");
+  const char* why = "";
+  if (int rc = qk_norm_check(*a, true, &why)) return fail_op(rc, "fact_qk_norm_backward", why);
+  if (int rc = check_ws("fact_qk_norm_backward", workspace, workspace_bytes, qk_norm_ws(*a, true))) return rc;
+  CHK(launch_qk_norm_bwd(*a, workspace, (hipStream_t)stream));
   return 0;
 }
 

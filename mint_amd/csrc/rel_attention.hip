@@ -1,0 +1,1145 @@
+// Attention with a sliding window, sinks and a learned relative position bias by buckets, forward and backward
+// (definition: include/fact_hip.h, FactAttention).
+//
+// Fragment conventions (common.h): scores are computed transposed, S^T = K Q^T, on 16x16x32 bf16 MFMAs, so that one query
+// lives in one lane column: lane (g = lane >> 4, c = lane & 15) holds keys 4 g .. 4 g + 3 of query c.  Two stacked 16-key
+// score tiles are the B operand of the products that contract over keys (slot j < 4: key 4 g + j, j >= 4: key 16 + 4 g + j - 4),
+// their A operands come from the same row-major LDS tiles through the LDS transpose read.  Any [token][head][dh] strides are
+// read in place: where dh is no multiple of 32 the last contraction step is padded with zeros in registers and in the LDS rows
+// (a 16-deep MFMA costs the same cycles, and one that took up the accumulator right behind a 32-deep one read it too early).
+#include "rel_attention.h"
+
+#include <algorithm>
+#include <climits>
+#include <vector>
+
+namespace {
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr int PAD = 64;  // distances past +-D that a 32 x 32 tile which still touches (-D, D) can reach: 62
+typedef __attribute__((address_space(3))) bf16x4 lds_bf16x4;
+
+struct RelP {
+  FactAttention a;
+  float sc;       // scale * log2 e
+  float rscale;   // 1 / scale: the bias enters through the accumulator, which is multiplied by scale afterwards
+  int qblocks, nwg;
+  int splits;
+  float* dsum;    // [B][H][nq] rowsum(dO . O)
+  float* part;    // per-workgroup bias gradients [B * H * qblocks][2 D + 1] / partial rows of the few-row kernel
+};
+
+template <int DH>
+struct Geo {
+  static constexpr int ND = DH / 16;        // 16-wide head-dim tiles
+  static constexpr int KD = (DH + 31) / 32; // 32-deep contraction steps over the head dim
+  static constexpr int CH = DH / 8;         // 16-byte chunks of a row
+  static constexpr int KP = KD * 32 + 8;    // LDS row pitch (elements): 16 consecutive rows start in different banks
+  static constexpr int IMG = 32 * KP;       // one 32-row tile
+};
+
+// one operand fragment set over the head dim: rows of 16 tokens
+template <int DH>
+struct Frag {
+  bf16x8 f[Geo<DH>::KD];
+};
+template <int DH>
+DEVINL void frag_load(Frag<DH>& r, const bf16_t* row, int g) {  // `row`: this lane's row in global memory
+#pragma unroll
+  for (int kd = 0; kd < Geo<DH>::KD; ++kd) {
+    r.f[kd] = zero_bf16x8();
+    if (kd * 32 + 32 <= DH || kd * 32 + g * 8 < DH) r.f[kd] = *reinterpret_cast<const bf16x8*>(row + kd * 32 + g * 8);
+  }
+}
+template <int DH>
+DEVINL void frag_lds(Frag<DH>& r, const bf16_t* row, int g) {  // an LDS row: its padding columns are zero
+#pragma unroll
+  for (int kd = 0; kd < Geo<DH>::KD; ++kd) r.f[kd] = *reinterpret_cast<const bf16x8*>(row + kd * 32 + g * 8);
+}
+template <int DH>
+DEVINL f32x4 frag_dot(const Frag<DH>& a, const Frag<DH>& b, f32x4 c) {
+#pragma unroll
+  for (int kd = 0; kd < Geo<DH>::KD; ++kd) c = mfma16(a.f[kd], b.f[kd], c);
+  return c;
+}
+// zeros into the padding columns of `tiles` LDS tiles, once per workgroup
+template <int DH>
+DEVINL void pad_zero(bf16_t* lds, int tiles, int tid, int nthr) {
+  if constexpr (DH % 32 != 0) {
+    constexpr int PC = (Geo<DH>::KD * 32 - DH) / 8;
+    for (int i = tid; i < tiles * 32 * PC; i += nthr)
+      *reinterpret_cast<u32x4*>(lds + (i / PC) * Geo<DH>::KP + DH + (i % PC) * 8) = u32x4{0u, 0u, 0u, 0u};
+  }
+}
+
+DEVINL bf16x8 cat4(bf16x4 a, bf16x4 b) { return bf16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]}; }
+DEVINL bf16x8 pack8(f32x4 a, f32x4 b) {
+  return bf16x8{(bf16_t)a[0], (bf16_t)a[1], (bf16_t)a[2], (bf16_t)a[3], (bf16_t)b[0], (bf16_t)b[1], (bf16_t)b[2], (bf16_t)b[3]};
+}
+// A operand [16 dims of tile dt][32 tokens] of a row-major LDS tile, token slots as in the header comment
+template <int DH>
+DEVINL bf16x8 frag_tr(const bf16_t* t, int dt, int lane) {
+  const int g = lane >> 4, s = lane & 15;
+  const bf16_t* p = t + (g * 4 + (s >> 2)) * Geo<DH>::KP + dt * 16 + (s & 3) * 4;
+  const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)p);
+  const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(p + 16 * Geo<DH>::KP));
+  return cat4(lo, hi);
+}
+
+DEVINL float allmax4(float v) {  // over the 4 lanes of a query
+  v = fmaxf(v, __shfl_xor(v, 16, 64));
+  return fmaxf(v, __shfl_xor(v, 32, 64));
+}
+DEVINL float allsum4(float v) {
+  v += __shfl_xor(v, 16, 64);
+  return v + __shfl_xor(v, 32, 64);
+}
+
+// ---- which keys a query sees ----------------------------------------------------------------------------------------
+struct Vis {
+  int len, lo, hi, sinks;  // key j of position p: j < len, j - p <= hi, j - p >= lo or j < sinks
+  DEVINL bool seen(int j, int p) const {
+    const int d = j - p;  // (selects, no branches: hipcc dropped one of the branchy form's stores)
+    return (j < len) & (d <= hi) & ((d >= lo) | (j < sinks));
+  }
+  // a 32-key tile at j0 against positions p0 .. p0 + 31
+  DEVINL bool none(int j0, int p0) const {
+    return j0 >= len || j0 - (p0 + 31) > hi || (j0 + 31 - p0 < lo && j0 >= sinks);
+  }
+  DEVINL bool full(int j0, int p0) const {
+    return j0 + 31 < len && j0 + 31 - p0 <= hi && (j0 - (p0 + 31) >= lo || j0 + 31 < sinks);
+  }
+};
+// Lengths are below 2^30 (checked) and first positions clamped to +-(2^30 - 64), so no key - position overflows.
+DEVINL Vis vis_of(const FactAttention& a, int b) {
+  Vis v;
+  v.len = a.kv_len ? min(max(a.kv_len[b], 0), a.nk) : a.nk;
+  v.lo = a.window_left < 0 ? INT_MIN : -a.window_left;
+  v.hi = a.window_right < 0 ? INT_MAX : a.window_right;
+  v.sinks = a.window_left < 0 ? 0 : a.sinks;
+  return v;
+}
+DEVINL int start_of(const FactAttention& a, int b) {
+  return a.q_start ? min(max(a.q_start[b], 64 - (1 << 30)), (1 << 30) - 64) : 0;
+}
+// the 32-key tiles that positions pa .. pb can see: tiles 0 .. ns - 1 (sinks), then t0 .. t0 + (T - ns) - 1
+struct Tiles {
+  int ns, t0, T;
+  DEVINL int at(int t) const { return t < ns ? t : t - ns + t0; }
+};
+DEVINL Tiles tiles_of(const Vis& v, long long pa, long long pb) {
+  const long long hi = min((long long)v.len, v.hi == INT_MAX ? (long long)v.len : pb + v.hi + 1);
+  const long long lo = v.lo == INT_MIN ? 0 : max(0ll, pa + v.lo);
+  Tiles t;
+  const int t1 = hi > 0 ? (int)((hi + 31) >> 5) : 0;
+  t.ns = hi > 0 ? (int)((min(hi, (long long)v.sinks) + 31) >> 5) : 0;
+  t.t0 = max(t.ns, (int)(min(lo, 1ll << 30) >> 5));
+  t.T = t.ns + (lo < hi ? max(0, t1 - t.t0) : 0);
+  return t;
+}
+
+// Workgroups of one head (and of the heads that share its keys) are neighbours on one XCD (consecutive workgroups go to
+// consecutive XCDs): they then read the same K / V rows through one L2.  Speed only.
+DEVINL int xcd_order(int id, int n) {
+  const int x = id & 7, per = n >> 3, rem = n & 7;
+  return (x < rem ? x * (per + 1) : rem * (per + 1) + (x - rem) * per) + (id >> 3);
+}
+
+// ---- staging of two 32-row tiles (K and V, or Q and dO) through registers into LDS -------------------------------------
+template <int DH>
+struct Stage {
+  static constexpr int N = (2 * 32 * Geo<DH>::CH + 255) / 256;
+  u32x4 r[N];
+  const bf16_t* src[N];
+  long long ld[N];
+  int row[N], dst[N];
+  DEVINL void init(const bf16_t* a, long long lda, const bf16_t* b, long long ldb, int tid) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int c = min(tid + i * 256, 2 * 32 * Geo<DH>::CH - 1);  // (the last threads of an uneven list repeat the last chunk)
+      const int im = c / (32 * Geo<DH>::CH), q = c - im * 32 * Geo<DH>::CH;
+      row[i] = q / Geo<DH>::CH;
+      const int ch = q - row[i] * Geo<DH>::CH;
+      src[i] = (im ? b : a) + ch * 8;
+      ld[i] = im ? ldb : lda;
+      dst[i] = im * Geo<DH>::IMG + row[i] * Geo<DH>::KP + ch * 8;
+    }
+  }
+  DEVINL void load(int row0, int last) {  // rows past `last` repeat it: finite values that the caller masks
+#pragma unroll
+    for (int i = 0; i < N; ++i) r[i] = *reinterpret_cast<const u32x4*>(src[i] + (long long)min(row0 + row[i], last) * ld[i]);
+  }
+  DEVINL void store(bf16_t* lds) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) *reinterpret_cast<u32x4*>(lds + dst[i]) = r[i];
+  }
+};
+
+// bias of head h for distances -(D + PAD) .. D + PAD, divided by scale
+DEVINL void load_bias(float* eb, const RelP& p, int h, int tid, int nthr) {
+  const int D = p.a.rel_max_distance;
+  for (int i = tid; i < 2 * (D + PAD) + 1; i += nthr) {
+    const int d = min(max(i - (D + PAD), -D), D);
+    const int bk = min(max(p.a.rel_map[d + D], 0), p.a.rel_buckets - 1);
+    eb[i] = p.a.rel_table[(size_t)bk * p.a.H + h] * p.rscale;
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// forward: workgroup = 128 queries of one head, 4 waves x 32 queries; 32-key tiles double-buffered in LDS
+// ---------------------------------------------------------------------------------------------------------------------
+// MODE 0: no bias, 1: bias, 2: bias, and the probabilities enter P V as a sum of two bf16 values: with one, the rounding of P
+// moves rowsum(dO . O) by 1e-3 of itself, and the fp32 gradient of the table, a sum of dS over whole diagonals, with it
+template <int DH, int MODE>
+__global__ __launch_bounds__(256, 2) void rel_fwd_kernel(const RelP p) {
+  using G = Geo<DH>;
+  constexpr int ND = G::ND;
+  constexpr bool REL = MODE > 0;
+  extern __shared__ __attribute__((aligned(16))) bf16_t smem[];
+  float* eb = reinterpret_cast<float*>(smem + 4 * G::IMG);
+  const FactAttention& a = p.a;
+  const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, c = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int id = xcd_order(blockIdx.x, p.nwg);
+  const int bh = id / p.qblocks, qb = p.qblocks - 1 - (id - bh * p.qblocks);
+  const int b = bh / a.H, h = bh - b * a.H, hk = h / (a.H / a.Hkv);
+  const Vis v = vis_of(a, b);
+  const int start = start_of(a, b);
+  const int q0 = qb * 128 + wave * 32, p0 = start + q0;
+  const bool active = q0 < a.nq;
+  const Tiles tl = tiles_of(v, (long long)start + qb * 128, (long long)start + min(qb * 128 + 127, a.nq - 1));
+
+  Frag<DH> Q[2];
+#pragma unroll
+  for (int qs = 0; qs < 2; ++qs)
+    frag_load<DH>(Q[qs], (const bf16_t*)a.q + b * a.q_stride[0] + (long long)min(q0 + qs * 16 + c, a.nq - 1) * a.q_stride[1] +
+                             h * a.q_stride[2], g);
+  Stage<DH> st;
+  st.init((const bf16_t*)a.k + b * a.k_stride[0] + hk * a.k_stride[2], a.k_stride[1],
+          (const bf16_t*)a.v + b * a.v_stride[0] + hk * a.v_stride[2], a.v_stride[1], tid);
+  pad_zero<DH>(smem, 4, tid, 256);
+  if (REL) load_bias(eb, p, h, tid, 256);
+  f32x4 O[2][ND];
+  float m[2], l[2];
+#pragma unroll
+  for (int qs = 0; qs < 2; ++qs) {
+    m[qs] = -INFINITY;
+    l[qs] = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < ND; ++dt) O[qs][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  if (tl.T > 0) {
+    st.load(tl.at(0) * 32, v.len - 1);
+    st.store(smem);
+    if (tl.T > 1) st.load(tl.at(1) * 32, v.len - 1);
+  }
+  const int D = a.rel_max_distance;
+  for (int t = 0; t < tl.T; ++t) {
+    __syncthreads();
+    if (t + 1 < tl.T) {
+      st.store(smem + ((t + 1) & 1) * 2 * G::IMG);
+      if (t + 2 < tl.T) st.load(tl.at(t + 2) * 32, v.len - 1);
+    }
+    const int j0 = tl.at(t) * 32;
+    if (!active || v.none(j0, p0)) continue;
+    const bf16_t* Ks = smem + (t & 1) * 2 * G::IMG;
+    const bf16_t* Vs = Ks + G::IMG;
+    f32x4 s[2][2];  // [key sub-tile][query sub-tile]
+    if (REL) {
+      const int d0 = j0 - p0;  // distance of the tile's first key and the wave's first query
+      if (d0 - 31 >= D || d0 + 31 <= -D) {
+        const float f = eb[d0 > 0 ? 2 * (D + PAD) : 0];
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+          for (int qs = 0; qs < 2; ++qs) s[ks][qs] = f32x4{f, f, f, f};
+      } else {
+        const float* e = eb + d0 + D + PAD + 4 * g - c;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          s[0][1][r] = e[r - 16];
+          s[0][0][r] = s[1][1][r] = e[r];
+          s[1][0][r] = e[r + 16];
+        }
+      }
+    } else {
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+        for (int qs = 0; qs < 2; ++qs) s[ks][qs] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      Frag<DH> K;
+      frag_lds<DH>(K, Ks + (ks * 16 + c) * G::KP, g);
+#pragma unroll
+      for (int qs = 0; qs < 2; ++qs) s[ks][qs] = frag_dot<DH>(K, Q[qs], s[ks][qs]);
+    }
+    if (!v.full(j0, p0)) {
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+        for (int qs = 0; qs < 2; ++qs)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            s[ks][qs][r] = v.seen(j0 + ks * 16 + 4 * g + r, p0 + qs * 16 + c) ? s[ks][qs][r] : -INFINITY;
+    }
+    bf16x8 pb[2], pl[2];
+#pragma unroll
+    for (int qs = 0; qs < 2; ++qs) {
+      float mx = fmaxf(fmaxf(fmaxf(s[0][qs][0], s[0][qs][1]), fmaxf(s[0][qs][2], s[0][qs][3])),
+                       fmaxf(fmaxf(s[1][qs][0], s[1][qs][1]), fmaxf(s[1][qs][2], s[1][qs][3])));
+      mx = allmax4(mx) * p.sc;
+      if (__any(mx > m[qs])) {
+        const float mn = fmaxf(m[qs], mx);
+        const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[qs] - mn);
+        m[qs] = mn;
+        l[qs] *= alpha;
+#pragma unroll
+        for (int dt = 0; dt < ND; ++dt) O[qs][dt] *= alpha;
+      }
+      const float mu = m[qs] == -INFINITY ? 0.f : m[qs];  // a row that has seen no key yet: every p below is 0
+      f32x4 e0, e1;
+      float ls = 0.f;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        e0[r] = __builtin_amdgcn_exp2f(fmaf(s[0][qs][r], p.sc, -mu));
+        e1[r] = __builtin_amdgcn_exp2f(fmaf(s[1][qs][r], p.sc, -mu));
+        ls += e0[r] + e1[r];
+      }
+      l[qs] += ls;
+      pb[qs] = pack8(e0, e1);
+      if (MODE == 2) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          e0[r] -= (float)pb[qs][r];
+          e1[r] -= (float)pb[qs][4 + r];
+        }
+        pl[qs] = pack8(e0, e1);
+      }
+    }
+#pragma unroll
+    for (int dt = 0; dt < ND; ++dt) {
+      const bf16x8 vf = frag_tr<DH>(Vs, dt, lane);
+#pragma unroll
+      for (int qs = 0; qs < 2; ++qs) {
+        O[qs][dt] = mfma16(vf, pb[qs], O[qs][dt]);
+        if (MODE == 2) O[qs][dt] = mfma16(vf, pl[qs], O[qs][dt]);
+      }
+    }
+  }
+  if (!active) return;
+#pragma unroll
+  for (int qs = 0; qs < 2; ++qs) {
+    const float lt = allsum4(l[qs]);
+    const float inv = lt == 0.f ? 0.f : 1.0f / lt;
+    const int q = q0 + qs * 16 + c;
+    if (q >= a.nq) continue;
+    if (a.lse && g == 0) a.lse[((size_t)b * a.H + h) * a.nq + q] = lt == 0.f ? INFINITY : m[qs] + __log2f(lt);
+    const long long off = b * a.out_stride[0] + (long long)q * a.out_stride[1] + h * a.out_stride[2] + g * 4;
+#pragma unroll
+    for (int dt = 0; dt < ND; ++dt) {
+      bf16x4 o, lo;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float x = O[qs][dt][r] * inv;
+        o[r] = (bf16_t)x;
+        lo[r] = (bf16_t)(x - (float)o[r]);
+      }
+      *reinterpret_cast<bf16x4*>((bf16_t*)a.out + off + dt * 16) = o;
+      if (a.out_lo) *reinterpret_cast<bf16x4*>((bf16_t*)a.out_lo + off + dt * 16) = lo;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// backward dQ and the bias gradient: workgroup = 128 queries of one head
+//   P = exp2(S c - L);  dP = V dO^T;  dS = P (dP - D), D = rowsum(dO . O);  dQ^T += K^T dS;  dbias[j - p] += dS
+// ---------------------------------------------------------------------------------------------------------------------
+template <int DH, bool REL>
+__global__ __launch_bounds__(256, 2) void rel_dq_kernel(const RelP p) {
+  using G = Geo<DH>;
+  constexpr int ND = G::ND;
+  extern __shared__ __attribute__((aligned(16))) bf16_t smem[];
+  const FactAttention& a = p.a;
+  const int D = a.rel_max_distance, NB = 2 * (D + PAD) + 1;
+  float* eb = reinterpret_cast<float*>(smem + 4 * G::IMG);
+  const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, c = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  float* bins = eb + NB * (1 + wave);  // this wave's bias gradient by distance: its own, so sums have one order
+  const int id = xcd_order(blockIdx.x, p.nwg);
+  const int bh = id / p.qblocks, qb = p.qblocks - 1 - (id - bh * p.qblocks);
+  const int b = bh / a.H, h = bh - b * a.H, hk = h / (a.H / a.Hkv);
+  const Vis v = vis_of(a, b);
+  const int start = start_of(a, b);
+  const int q0 = qb * 128 + wave * 32, p0 = start + q0;
+  const bool active = q0 < a.nq;
+  const Tiles tl = tiles_of(v, (long long)start + qb * 128, (long long)start + min(qb * 128 + 127, a.nq - 1));
+
+  Stage<DH> st;
+  st.init((const bf16_t*)a.k + b * a.k_stride[0] + hk * a.k_stride[2], a.k_stride[1],
+          (const bf16_t*)a.v + b * a.v_stride[0] + hk * a.v_stride[2], a.v_stride[1], tid);
+  if (tl.T > 0) st.load(tl.at(0) * 32, v.len - 1);
+  Frag<DH> Q[2], dO[2];
+  float nL[2], nD[2];
+#pragma unroll
+  for (int qs = 0; qs < 2; ++qs) {
+    const int q = min(q0 + qs * 16 + c, a.nq - 1);
+    frag_load<DH>(Q[qs], (const bf16_t*)a.q + b * a.q_stride[0] + (long long)q * a.q_stride[1] + h * a.q_stride[2], g);
+    frag_load<DH>(dO[qs], (const bf16_t*)a.dout + b * a.dout_stride[0] + (long long)q * a.dout_stride[1] + h * a.dout_stride[2], g);
+    const long long off = b * a.out_stride[0] + (long long)q * a.out_stride[1] + h * a.out_stride[2];
+    float part = 0.f;
+    auto rowsum = [&](const bf16_t* o) {
+      Frag<DH> f;
+      frag_load<DH>(f, o, g);
+#pragma unroll
+      for (int kd = 0; kd < G::KD; ++kd)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) part += (float)dO[qs].f[kd][j] * (float)f.f[kd][j];
+    };
+    rowsum((const bf16_t*)a.out + off);
+    if (a.out_lo) rowsum((const bf16_t*)a.out_lo + off);
+    part = allsum4(part);
+    const size_t at = ((size_t)b * a.H + h) * a.nq + q;
+    nL[qs] = -a.lse[at];
+    nD[qs] = -part;
+    if (active && g == 0) p.dsum[at] = part;  // for the dK / dV kernel (repeated rows write the same value)
+  }
+  pad_zero<DH>(smem, 4, tid, 256);
+  f32x4 dQ[2][ND];
+#pragma unroll
+  for (int qs = 0; qs < 2; ++qs)
+#pragma unroll
+    for (int dt = 0; dt < ND; ++dt) dQ[qs][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float farl = 0.f, farr = 0.f;
+  if (REL) {
+    load_bias(eb, p, h, tid, 256);
+    for (int i = lane; i < NB; i += 64) bins[i] = 0.f;
+  }
+  if (tl.T > 0) {
+    st.store(smem);
+    if (tl.T > 1) st.load(tl.at(1) * 32, v.len - 1);
+  }
+  for (int t = 0; t < tl.T; ++t) {
+    __syncthreads();
+    if (t + 1 < tl.T) {
+      st.store(smem + ((t + 1) & 1) * 2 * G::IMG);
+      if (t + 2 < tl.T) st.load(tl.at(t + 2) * 32, v.len - 1);
+    }
+    const int j0 = tl.at(t) * 32;
+    if (!active || v.none(j0, p0)) continue;
+    const bf16_t* Ks = smem + (t & 1) * 2 * G::IMG;
+    const bf16_t* Vs = Ks + G::IMG;
+    f32x4 s[2][2], dp[2][2];
+    const int d0 = j0 - p0;
+    const bool left = REL && d0 + 31 <= -D, right = REL && d0 - 31 >= D;
+    if (REL) {
+      if (left || right) {
+        const float f = eb[right ? NB - 1 : 0];
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+          for (int qs = 0; qs < 2; ++qs) s[ks][qs] = f32x4{f, f, f, f};
+      } else {
+        const float* e = eb + d0 + D + PAD + 4 * g - c;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          s[0][1][r] = e[r - 16];
+          s[0][0][r] = s[1][1][r] = e[r];
+          s[1][0][r] = e[r + 16];
+        }
+      }
+    } else {
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+        for (int qs = 0; qs < 2; ++qs) s[ks][qs] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      Frag<DH> K, V;
+      frag_lds<DH>(K, Ks + (ks * 16 + c) * G::KP, g);
+      frag_lds<DH>(V, Vs + (ks * 16 + c) * G::KP, g);
+#pragma unroll
+      for (int qs = 0; qs < 2; ++qs) {
+        dp[ks][qs] = f32x4{nD[qs], nD[qs], nD[qs], nD[qs]};
+        s[ks][qs] = frag_dot<DH>(K, Q[qs], s[ks][qs]);
+        dp[ks][qs] = frag_dot<DH>(V, dO[qs], dp[ks][qs]);
+      }
+    }
+    f32x4 ds[2][2];
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+      for (int qs = 0; qs < 2; ++qs)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          ds[ks][qs][r] = __builtin_amdgcn_exp2f(fmaf(s[ks][qs][r], p.sc, nL[qs])) * dp[ks][qs][r];
+    if (!v.full(j0, p0) || q0 + 31 >= a.nq) {  // (queries past the last repeat it: kept out of the bias gradient)
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+        for (int qs = 0; qs < 2; ++qs)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            ds[ks][qs][r] = (v.seen(j0 + ks * 16 + 4 * g + r, p0 + qs * 16 + c) & (q0 + qs * 16 + c < a.nq)) ? ds[ks][qs][r] : 0.f;
+    }
+    if (REL) {
+      if (left || right) {
+        float x = 0.f;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x += (ds[0][0][r] + ds[1][1][r]) + (ds[0][1][r] + ds[1][0][r]);
+        if (left) farl += x;
+        else farr += x;
+      } else {
+        float* e = bins + d0 + D + PAD + 4 * g - c;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          atomicAdd(e + r - 16, ds[0][1][r]);
+          atomicAdd(e + r, ds[0][0][r] + ds[1][1][r]);
+          atomicAdd(e + r + 16, ds[1][0][r]);
+        }
+      }
+    }
+    bf16x8 dsb[2];
+#pragma unroll
+    for (int qs = 0; qs < 2; ++qs) dsb[qs] = pack8(ds[0][qs], ds[1][qs]);
+#pragma unroll
+    for (int dt = 0; dt < ND; ++dt) {
+      const bf16x8 kf = frag_tr<DH>(Ks, dt, lane);
+#pragma unroll
+      for (int qs = 0; qs < 2; ++qs) dQ[qs][dt] = mfma16(kf, dsb[qs], dQ[qs][dt]);
+    }
+  }
+  if (active) {
+#pragma unroll
+    for (int qs = 0; qs < 2; ++qs) {
+      const int q = q0 + qs * 16 + c;
+      if (q >= a.nq) continue;
+      bf16_t* row = (bf16_t*)a.dq + b * a.dq_stride[0] + (long long)q * a.dq_stride[1] + h * a.dq_stride[2] + g * 4;
+#pragma unroll
+      for (int dt = 0; dt < ND; ++dt) {
+        bf16x4 o;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[r] = (bf16_t)(dQ[qs][dt][r] * a.scale);
+        *reinterpret_cast<bf16x4*>(row + dt * 16) = o;
+      }
+    }
+  }
+  if (REL) {
+    farl = wave_sum(farl);
+    farr = wave_sum(farr);
+    if (lane == 0) {
+      bins[PAD] += farl;
+      bins[NB - 1 - PAD] += farr;
+    }
+    __syncthreads();
+    float* out = p.part + (size_t)id * (2 * D + 1);
+    float* b0 = eb + NB;
+    for (int i = tid; i < 2 * D + 1; i += 256) {
+      const int k = i + PAD;
+      float x = (b0[k] + b0[NB + k]) + (b0[2 * NB + k] + b0[3 * NB + k]);
+      if (i > 0 && i < 2 * D) out[i] = x;
+    }
+    // the two ends take the PAD distances beyond them as well
+    if (wave < 2) {
+      float x = 0.f;
+      for (int i = lane; i <= PAD; i += 64) {
+        const int k = wave ? NB - 1 - PAD + i : i;
+        x += (b0[k] + b0[NB + k]) + (b0[2 * NB + k] + b0[3 * NB + k]);
+      }
+      x = wave_sum(x);
+      if (lane == 0) out[wave ? 2 * D : 0] = x;
+    }
+  }
+}
+
+// drel[bucket][h]: sums over the batch and the query blocks in index order, then over the distances of a bucket
+__global__ __launch_bounds__(1024) void rel_dtable_kernel(const RelP p) {
+  const FactAttention& a = p.a;
+  const int D = a.rel_max_distance, n = 2 * D + 1, h = blockIdx.x, tid = threadIdx.x;
+  __shared__ float val[2049];
+  __shared__ short bk[2049];
+  for (int i = tid; i < n; i += 1024) {
+    float x = 0.f;
+    for (int b = 0; b < a.B; ++b) {
+      const float* src = p.part + ((size_t)b * a.H + h) * p.qblocks * n + i;
+      for (int q = 0; q < p.qblocks; ++q) x += src[(size_t)q * n];
+    }
+    val[i] = x;
+    bk[i] = (short)min(max(a.rel_map[i], 0), a.rel_buckets - 1);
+  }
+  __syncthreads();
+  // 4 lanes a bucket
+  const int bu = tid >> 2;
+  if (bu < a.rel_buckets) {
+    float x = 0.f;
+    for (int i = tid & 3; i < n; i += 4)
+      if (bk[i] == bu) x += val[i];
+    x += __shfl_xor(x, 1, 64);
+    x += __shfl_xor(x, 2, 64);
+    if ((tid & 3) == 0) {
+      float* o = a.drel + (size_t)bu * a.H + h;
+      *o = a.drel_accumulate ? *o + x : x;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// backward dK / dV: workgroup = 128 keys of one key head, 4 waves x 32 keys; the query tiles of every head that reads them
+// are streamed (heads of a group one after another, so their sum has one order)
+// ---------------------------------------------------------------------------------------------------------------------
+template <int DH, bool REL>
+__global__ __launch_bounds__(256, DH > 96 ? 1 : 2) void rel_dkdv_kernel(const RelP p) {
+  using G = Geo<DH>;
+  constexpr int ND = G::ND;
+  extern __shared__ __attribute__((aligned(16))) bf16_t smem[];
+  const FactAttention& a = p.a;
+  const int D = a.rel_max_distance, NB = 2 * (D + PAD) + 1;
+  float* stat = reinterpret_cast<float*>(smem + 4 * G::IMG);  // [2][64]: -L, -D of the tile's queries
+  float* eb = stat + 128;
+  const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, c = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int kblocks = (a.nk + 127) / 128, group = a.H / a.Hkv;
+  const int id = xcd_order(blockIdx.x, p.nwg);
+  const int bh = id / kblocks, kb = id - bh * kblocks;
+  const int b = bh / a.Hkv, hk = bh - b * a.Hkv;
+  const Vis v = vis_of(a, b);
+  const int start = start_of(a, b);
+  const int j0 = kb * 128 + wave * 32;
+  const bool active = j0 < v.len;
+  // query rows that see any key of the block: positions [ka - hi, ke - lo], or all later ones if it holds a sink
+  const long long ka = kb * 128, ke = min(kb * 128 + 127, v.len - 1);
+  long long qa = v.hi == INT_MAX ? 0 : max(0ll, ka - v.hi - start);
+  long long qe = (v.lo == INT_MIN || ka < v.sinks) ? a.nq - 1 : min((long long)a.nq - 1, ke - v.lo - start);
+  if (ka >= v.len) qe = -1;
+  const int t0 = (int)(min(qa, 1ll << 30) >> 5), T = qe >= qa ? (int)(qe >> 5) - t0 + 1 : 0, TT = T * group;
+
+  Frag<DH> K[2], V[2];
+#pragma unroll
+  for (int ks = 0; ks < 2; ++ks) {
+    const long long j = max(0, min(j0 + ks * 16 + c, v.len - 1));
+    frag_load<DH>(K[ks], (const bf16_t*)a.k + b * a.k_stride[0] + j * a.k_stride[1] + hk * a.k_stride[2], g);
+    frag_load<DH>(V[ks], (const bf16_t*)a.v + b * a.v_stride[0] + j * a.v_stride[1] + hk * a.v_stride[2], g);
+  }
+  pad_zero<DH>(smem, 4, tid, 256);
+  f32x4 dK[2][ND], dV[2][ND];
+#pragma unroll
+  for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+    for (int dt = 0; dt < ND; ++dt) dK[ks][dt] = dV[ks][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  Stage<DH> st;
+  float sv = 0.f;
+  auto load = [&](int i) {  // i-th tile of the stream: head i / T of the group, query tile t0 + i % T
+    const int hh = i / T, h = hk * group + hh, q0 = (t0 + i - hh * T) * 32;
+    st.init((const bf16_t*)a.q + b * a.q_stride[0] + h * a.q_stride[2], a.q_stride[1],
+            (const bf16_t*)a.dout + b * a.dout_stride[0] + h * a.dout_stride[2], a.dout_stride[1], tid);
+    st.load(q0, a.nq - 1);
+    if (tid < 64) {
+      const size_t at = ((size_t)b * a.H + h) * a.nq + min(q0 + (tid & 31), a.nq - 1);
+      sv = tid < 32 ? -a.lse[at] : -p.dsum[at];
+    }
+  };
+  auto store = [&](int buf) {
+    st.store(smem + buf * 2 * G::IMG);
+    if (tid < 64) stat[buf * 64 + tid] = sv;
+  };
+  if (TT > 0) {
+    load(0);
+    store(0);
+    if (TT > 1) load(1);
+  }
+  for (int i = 0; i < TT; ++i) {
+    const int hh = i / T, qt = i - hh * T;
+    if (REL && qt == 0) {  // the next head's bias: after the last tile of the head before has been read
+      __syncthreads();
+      load_bias(eb, p, hk * group + hh, tid, 256);
+    }
+    __syncthreads();
+    if (i + 1 < TT) {
+      store((i + 1) & 1);
+      if (i + 2 < TT) load(i + 2);
+    }
+    const int q0 = (t0 + qt) * 32, p0 = start + q0;
+    if (!active || v.none(j0, p0)) continue;
+    const bf16_t* Qs = smem + (i & 1) * 2 * G::IMG;
+    const bf16_t* Os = Qs + G::IMG;
+    const float* sl = stat + (i & 1) * 64;
+    f32x4 s[2][2], dp[2][2];  // [query sub-tile][key sub-tile]: lane = key c, queries 4 g .. 4 g + 3
+    if (REL) {
+      const int d0 = j0 - p0;
+      if (d0 - 31 >= D || d0 + 31 <= -D) {
+        const float f = eb[d0 > 0 ? NB - 1 : 0];
+#pragma unroll
+        for (int qs = 0; qs < 2; ++qs)
+#pragma unroll
+          for (int ks = 0; ks < 2; ++ks) s[qs][ks] = f32x4{f, f, f, f};
+      } else {
+        const float* e = eb + d0 + D + PAD + c - 4 * g;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          s[1][0][r] = e[-r - 16];
+          s[0][0][r] = s[1][1][r] = e[-r];
+          s[0][1][r] = e[16 - r];
+        }
+      }
+    } else {
+#pragma unroll
+      for (int qs = 0; qs < 2; ++qs)
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) s[qs][ks] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    f32x4 nl[2], nd[2];
+#pragma unroll
+    for (int qs = 0; qs < 2; ++qs) {
+      nl[qs] = *reinterpret_cast<const f32x4*>(sl + qs * 16 + g * 4);
+      nd[qs] = *reinterpret_cast<const f32x4*>(sl + 32 + qs * 16 + g * 4);
+      Frag<DH> Q, dO;
+      frag_lds<DH>(Q, Qs + (qs * 16 + c) * G::KP, g);
+      frag_lds<DH>(dO, Os + (qs * 16 + c) * G::KP, g);
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        s[qs][ks] = frag_dot<DH>(Q, K[ks], s[qs][ks]);
+        dp[qs][ks] = frag_dot<DH>(dO, V[ks], nd[qs]);
+      }
+    }
+    f32x4 pr[2][2];
+#pragma unroll
+    for (int qs = 0; qs < 2; ++qs)
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          pr[qs][ks][r] = __builtin_amdgcn_exp2f(fmaf(s[qs][ks][r], p.sc, nl[qs][r]));
+          dp[qs][ks][r] *= pr[qs][ks][r];
+        }
+    if (!v.full(j0, p0) || q0 + 31 >= a.nq) {
+#pragma unroll
+      for (int qs = 0; qs < 2; ++qs)
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const bool ok = v.seen(j0 + ks * 16 + c, p0 + qs * 16 + 4 * g + r) & (q0 + qs * 16 + 4 * g + r < a.nq);
+            pr[qs][ks][r] = ok ? pr[qs][ks][r] : 0.f;
+            dp[qs][ks][r] = ok ? dp[qs][ks][r] : 0.f;
+          }
+    }
+    bf16x8 pb[2], db[2];
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      pb[ks] = pack8(pr[0][ks], pr[1][ks]);
+      db[ks] = pack8(dp[0][ks], dp[1][ks]);
+    }
+#pragma unroll
+    for (int dt = 0; dt < ND; ++dt) {
+      const bf16x8 of = frag_tr<DH>(Os, dt, lane);
+      const bf16x8 qf = frag_tr<DH>(Qs, dt, lane);
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        dV[ks][dt] = mfma16(of, pb[ks], dV[ks][dt]);
+        dK[ks][dt] = mfma16(qf, db[ks], dK[ks][dt]);
+      }
+    }
+  }
+#pragma unroll
+  for (int ks = 0; ks < 2; ++ks) {
+    const int j = j0 + ks * 16 + c;
+    if (j >= a.nk) continue;
+    bf16_t* kr = (bf16_t*)a.dk + b * a.dk_stride[0] + (long long)j * a.dk_stride[1] + hk * a.dk_stride[2] + g * 4;
+    bf16_t* vr = (bf16_t*)a.dv + b * a.dv_stride[0] + (long long)j * a.dv_stride[1] + hk * a.dv_stride[2] + g * 4;
+#pragma unroll
+    for (int dt = 0; dt < ND; ++dt) {
+      bf16x4 x, y;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        x[r] = (bf16_t)(dK[ks][dt][r] * a.scale);
+        y[r] = (bf16_t)dV[ks][dt][r];
+      }
+      *reinterpret_cast<bf16x4*>(kr + dt * 16) = x;
+      *reinterpret_cast<bf16x4*>(vr + dt * 16) = y;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// few rows: all nq * group <= 16 query rows of one key head are the 16 columns of a score tile; the waves of a workgroup and
+// the splits of a head take different key tiles and are joined by their maxima and sums at the end
+// ---------------------------------------------------------------------------------------------------------------------
+template <int DH, bool REL>
+__global__ __launch_bounds__(256, 2) void rel_rows_kernel(const RelP p) {
+  using G = Geo<DH>;
+  constexpr int ND = G::ND, NV = G::CH / 2;  // 16-byte chunks of V a lane moves per 32-key tile
+  constexpr int OP = DH + 4;                 // pitch of the joined rows (floats)
+  constexpr int BYTES = 4 * 16 * OP * 4 > 4 * G::IMG * 2 ? 4 * 16 * OP * 4 : 4 * G::IMG * 2;
+  __shared__ __attribute__((aligned(16))) unsigned char smem[BYTES];
+  __shared__ float ml[4][2][16];
+  const FactAttention& a = p.a;
+  const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, c = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int split = blockIdx.x % p.splits, bh = blockIdx.x / p.splits;
+  const int b = bh / a.Hkv, hk = bh - b * a.Hkv, group = a.H / a.Hkv, R = group * a.nq;
+  const Vis v = vis_of(a, b);
+  const int start = start_of(a, b);
+  const Tiles tl = tiles_of(v, start, (long long)start + a.nq - 1);
+  const int row = min(c, R - 1), h = hk * group + row / a.nq, qi = row - (row / a.nq) * a.nq, pos = start + qi;
+  Frag<DH> Q;
+  frag_load<DH>(Q, (const bf16_t*)a.q + b * a.q_stride[0] + (long long)qi * a.q_stride[1] + h * a.q_stride[2], g);
+  const int per = (tl.T + p.splits - 1) / p.splits;
+  const int tb = split * per, te = min(tl.T, tb + per);
+  const bf16_t* kb = (const bf16_t*)a.k + b * a.k_stride[0] + hk * a.k_stride[2];
+  const bf16_t* vb = (const bf16_t*)a.v + b * a.v_stride[0] + hk * a.v_stride[2];
+  bf16_t* Vs = reinterpret_cast<bf16_t*>(smem) + wave * G::IMG;
+  const int D = a.rel_max_distance;
+
+  Frag<DH> K[2];
+  u32x4 vr[NV];
+  auto load = [&](int t) {
+    const int j0 = tl.at(t) * 32;
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks)
+      frag_load<DH>(K[ks], kb + (long long)min(j0 + ks * 16 + c, v.len - 1) * a.k_stride[1], g);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int q = lane + i * 64, r = q / G::CH, ch = q - r * G::CH;
+      vr[i] = *reinterpret_cast<const u32x4*>(vb + (long long)min(j0 + r, v.len - 1) * a.v_stride[1] + ch * 8);
+    }
+  };
+  f32x4 O[ND];
+#pragma unroll
+  for (int dt = 0; dt < ND; ++dt) O[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, l = 0.f;
+  if (tb + wave < te) load(tb + wave);
+  for (int t = tb + wave; t < te; t += 4) {
+    const int j0 = tl.at(t) * 32;
+    f32x4 s[2];
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      s[ks] = frag_dot<DH>(K[ks], Q, f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int j = j0 + ks * 16 + 4 * g + r;
+        if (REL) {
+          const int bk = min(max(a.rel_map[min(max(j - pos, -D), D) + D], 0), a.rel_buckets - 1);
+          s[ks][r] += a.rel_table[(size_t)bk * a.H + h] * p.rscale;
+        }
+        s[ks][r] = v.seen(j, pos) ? s[ks][r] : -INFINITY;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int q = lane + i * 64, r = q / G::CH, ch = q - r * G::CH;
+      *reinterpret_cast<u32x4*>(Vs + r * G::KP + ch * 8) = vr[i];
+    }
+    if (t + 4 < te) load(t + 4);
+    float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
+                     fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+    mx = allmax4(mx) * p.sc;
+    const float mn = fmaxf(m, mx);
+    const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+    const float mu = mn == -INFINITY ? 0.f : mn;
+    m = mn;
+    f32x4 e0, e1;
+    float ls = 0.f;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      e0[r] = __builtin_amdgcn_exp2f(fmaf(s[0][r], p.sc, -mu));
+      e1[r] = __builtin_amdgcn_exp2f(fmaf(s[1][r], p.sc, -mu));
+      ls += e0[r] + e1[r];
+    }
+    l = l * alpha + ls;
+    const bf16x8 pb = pack8(e0, e1);
+    bf16x8 pl = zero_bf16x8();
+    if (a.out_lo) {  // as in the forward above
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        e0[r] -= (float)pb[r];
+        e1[r] -= (float)pb[4 + r];
+      }
+      pl = pack8(e0, e1);
+    }
+    __builtin_amdgcn_wave_barrier();  // the tile below was written by this wave alone: its LDS accesses stay in order
+#pragma unroll
+    for (int dt = 0; dt < ND; ++dt) {
+      const bf16x8 vf = frag_tr<DH>(Vs, dt, lane);
+      O[dt] = mfma16(vf, pb, O[dt] * alpha);
+      if (a.out_lo) O[dt] = mfma16(vf, pl, O[dt]);
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+  l = allsum4(l);
+  __syncthreads();
+  float* Oj = reinterpret_cast<float*>(smem);
+  if (g == 0) {
+    ml[wave][0][c] = m;
+    ml[wave][1][c] = l;
+  }
+#pragma unroll
+  for (int dt = 0; dt < ND; ++dt) *reinterpret_cast<f32x4*>(Oj + (wave * 16 + c) * OP + dt * 16 + g * 4) = O[dt];
+  __syncthreads();
+  // join the 4 waves: a thread takes 4 dims of a row
+  for (int i = tid; i < R * (DH / 4); i += 256) {
+    const int r = i / (DH / 4), d = (i - r * (DH / 4)) * 4;
+    float M = fmaxf(fmaxf(ml[0][0][r], ml[1][0][r]), fmaxf(ml[2][0][r], ml[3][0][r]));
+    const float mu = M == -INFINITY ? 0.f : M;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    float lt = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float f = __builtin_amdgcn_exp2f(ml[w][0][r] - mu);
+      lt += ml[w][1][r] * f;
+      o += *reinterpret_cast<const f32x4*>(Oj + (w * 16 + r) * OP + d) * f;
+    }
+    if (p.splits > 1) {
+      float* out = p.part + ((size_t)blockIdx.x * R + r) * (DH + 4);
+      if (d == 0) {
+        out[0] = M;
+        out[1] = lt;
+      }
+      *reinterpret_cast<f32x4*>(out + 4 + d) = o;
+    } else {
+      const int hh = hk * group + r / a.nq, q = r - (r / a.nq) * a.nq;
+      const float inv = lt == 0.f ? 0.f : 1.0f / lt;
+      if (a.lse && d == 0) a.lse[((size_t)b * a.H + hh) * a.nq + q] = lt == 0.f ? INFINITY : M + __log2f(lt);
+      const long long off = b * a.out_stride[0] + (long long)q * a.out_stride[1] + hh * a.out_stride[2] + d;
+      bf16x4 x, y;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        x[k] = (bf16_t)(o[k] * inv);
+        y[k] = (bf16_t)(o[k] * inv - (float)x[k]);
+      }
+      *reinterpret_cast<bf16x4*>((bf16_t*)a.out + off) = x;
+      if (a.out_lo) *reinterpret_cast<bf16x4*>((bf16_t*)a.out_lo + off) = y;
+    }
+  }
+}
+
+// join the splits of the few-row kernel: one wave per row, 2 dims a lane
+__global__ __launch_bounds__(64) void rel_join_kernel(const RelP p) {
+  const FactAttention& a = p.a;
+  const int group = a.H / a.Hkv, R = group * a.nq, lane = threadIdx.x;
+  const int bh = blockIdx.x / R, r = blockIdx.x - bh * R, b = bh / a.Hkv, hk = bh - b * a.Hkv;
+  const size_t pitch = a.dh + 4;
+  const float* src = p.part + ((size_t)bh * p.splits * R + r) * pitch;
+  float M = -INFINITY;
+  for (int s = lane; s < p.splits; s += 64) M = fmaxf(M, src[(size_t)s * R * pitch]);
+  M = wave_max(M);
+  const float mu = M == -INFINITY ? 0.f : M;
+  float lt = 0.f, o0 = 0.f, o1 = 0.f;
+  const int d = min(lane * 2, a.dh - 2);
+  for (int s = 0; s < p.splits; ++s) {
+    const float* x = src + (size_t)s * R * pitch;
+    const float f = __builtin_amdgcn_exp2f(x[0] - mu);
+    lt += x[1] * f;
+    const f32x2 o = *reinterpret_cast<const f32x2*>(x + 4 + d);
+    o0 += o[0] * f;
+    o1 += o[1] * f;
+  }
+  const int h = hk * group + r / a.nq, q = r - (r / a.nq) * a.nq;
+  const float inv = lt == 0.f ? 0.f : 1.0f / lt;
+  if (a.lse && lane == 0) a.lse[((size_t)b * a.H + h) * a.nq + q] = lt == 0.f ? INFINITY : M + __log2f(lt);
+  if (lane * 2 >= a.dh) return;
+  const long long off = b * a.out_stride[0] + (long long)q * a.out_stride[1] + h * a.out_stride[2] + d;
+  bf16x2 x = {(bf16_t)(o0 * inv), (bf16_t)(o1 * inv)};
+  *reinterpret_cast<bf16x2*>((bf16_t*)a.out + off) = x;
+  if (a.out_lo) {
+    bf16x2 y = {(bf16_t)(o0 * inv - (float)x[0]), (bf16_t)(o1 * inv - (float)x[1])};
+    *reinterpret_cast<bf16x2*>((bf16_t*)a.out_lo + off) = y;
+  }
+}
+
+// ---- host ------------------------------------------------------------------------------------------------------------
+int launched() { return hipGetLastError() == hipSuccess ? 0 : -100; }
+
+// dynamic LDS above 64 KiB has to be allowed once per kernel and device
+template <typename K>
+int allow_lds(K kernel, size_t bytes) {
+  if (bytes <= 65536) return 0;
+  return hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
+                             160 * 1024) == hipSuccess ? 0 : -101;
+}
+
+bool few_rows(const FactAttention& a) { return (long long)a.nq * (a.H / a.Hkv) <= 16; }
+
+// keys that one sequence's rows can see at most
+long long span(const FactAttention& a) {
+  if (a.window_left < 0) return a.nk;
+  const long long right = a.window_right < 0 ? a.nk : a.window_right;
+  return std::min<long long>(a.nk, (long long)a.window_left + right + a.nq + a.sinks + 62);
+}
+
+// splits of the few-row kernel: enough workgroups to fill 256 CUs twice, at least 8 tiles (2 a wave) each
+int row_splits(const FactAttention& a) {
+  const long long tiles = (span(a) + 31) / 32, wgs = (long long)a.B * a.Hkv;
+  long long s = std::min((512 + wgs - 1) / wgs, tiles / 8);
+  return (int)std::max(1ll, std::min(s, 256ll));
+}
+
+size_t up16(size_t x) { return (x + 15) & ~(size_t)15; }
+
+RelP params(const FactAttention& a) {
+  RelP p;
+  p.a = a;
+  p.sc = a.scale * LOG2E;
+  p.rscale = 1.0f / a.scale;
+  p.qblocks = (a.nq + 127) / 128;
+  p.nwg = 0;
+  p.splits = 1;
+  p.dsum = nullptr;
+  p.part = nullptr;
+  return p;
+}
+
+template <int DH, bool REL>
+int fwd_t(const FactAttention& a, void* ws, hipStream_t s) {
+  RelP p = params(a);
+  if (few_rows(a)) {
+    p.splits = row_splits(a);
+    p.part = (float*)ws;
+    FACT_LAUNCH((rel_rows_kernel<DH, REL>), dim3(p.splits * a.B * a.Hkv), dim3(256), 0, s, p);
+    if (p.splits > 1) FACT_LAUNCH(rel_join_kernel, dim3(a.B * a.H * a.nq), dim3(64), 0, s, p);
+    return launched();
+  }
+  p.nwg = p.qblocks * a.B * a.H;
+  const size_t lds = 4 * Geo<DH>::IMG * 2 + (REL ? (2 * (a.rel_max_distance + PAD) + 1) * 4 : 0);
+  auto go = [&](auto kernel) {
+    if (int rc = allow_lds(kernel, lds)) return rc;
+    FACT_LAUNCH(kernel, dim3(p.nwg), dim3(256), lds, s, p);
+    return launched();
+  };
+  if constexpr (REL)
+    if (a.out_lo) return go(rel_fwd_kernel<DH, 2>);
+  return go(rel_fwd_kernel<DH, REL ? 1 : 0>);
+}
+
+template <int DH, bool REL>
+int bwd_t(const FactAttention& a, void* ws, hipStream_t s) {
+  RelP p = params(a);
+  const size_t nb = REL ? 2 * (a.rel_max_distance + PAD) + 1 : 0;
+  p.dsum = (float*)ws;
+  p.part = (float*)((char*)ws + up16((size_t)a.B * a.H * a.nq * 4));
+  p.nwg = p.qblocks * a.B * a.H;
+  const size_t lds1 = 4 * Geo<DH>::IMG * 2 + 5 * nb * 4, lds2 = 4 * Geo<DH>::IMG * 2 + 512 + nb * 4;
+  if (int rc = allow_lds(rel_dq_kernel<DH, REL>, lds1)) return rc;
+  if (int rc = allow_lds(rel_dkdv_kernel<DH, REL>, lds2)) return rc;
+  FACT_LAUNCH((rel_dq_kernel<DH, REL>), dim3(p.nwg), dim3(256), lds1, s, p);
+  if (REL) FACT_LAUNCH(rel_dtable_kernel, dim3(a.H), dim3(1024), 0, s, p);
+  p.nwg = (a.nk + 127) / 128 * a.B * a.Hkv;
+  FACT_LAUNCH((rel_dkdv_kernel<DH, REL>), dim3(p.nwg), dim3(256), lds2, s, p);
+  return launched();
+}
+
+template <int DH>
+int run(const FactAttention& a, bool backward, void* ws, hipStream_t s) {
+  if (backward) return a.rel_table ? bwd_t<DH, true>(a, ws, s) : bwd_t<DH, false>(a, ws, s);
+  return a.rel_table ? fwd_t<DH, true>(a, ws, s) : fwd_t<DH, false>(a, ws, s);
+}
+int run(const FactAttention& a, bool backward, void* ws, hipStream_t s) {
+  switch (a.dh) {
+    case 32: return run<32>(a, backward, ws, s);
+    case 64: return run<64>(a, backward, ws, s);
+    case 80: return run<80>(a, backward, ws, s);
+    case 96: return run<96>(a, backward, ws, s);
+    case 128: return run<128>(a, backward, ws, s);
+  }
+  return -10;
+}
+
+}  // namespace
+
+int rel_attention_check(const FactAttention& a, bool backward, const char** why) {
+  auto bad = [&](int rc, const char* w) { *why = w; return rc; };
+  const int big = 1 << 30;
+  if (a.B <= 0 || a.H <= 0 || a.Hkv <= 0 || a.nq <= 0 || a.nk <= 0) return bad(-1, "B, H, Hkv, nq and nk must be positive");
+  if (a.nq >= big || a.nk >= big) return bad(-1, "nq and nk must be below 2^30");
+  if (a.H % a.Hkv) return bad(-1, "H must be a multiple of Hkv");
+  if (a.dh != 32 && a.dh != 64 && a.dh != 80 && a.dh != 96 && a.dh != 128)
+    return bad(-3, "unsupported head dim (supported: 32, 64, 80, 96, 128)");
+  if ((long long)a.B * a.H > INT_MAX / 256 || ((long long)a.nq + 127) / 128 * a.B * a.H > INT_MAX / 4 ||
+      ((long long)a.nk + 127) / 128 * a.B * a.Hkv > INT_MAX / 4)
+    return bad(-1, "too many heads and blocks for one launch");
+  if (!(a.scale >= 5.9604645e-8f) || !(a.scale <= 3.0e38f)) return bad(-1, "scale must be finite and at least 2^-24");
+  if (a.sinks < 0) return bad(-1, "sinks must not be negative");
+  if (a.rel_table) {
+    if (!a.rel_map) return bad(-1, "rel_table needs rel_map");
+    if (a.rel_buckets < 1 || a.rel_buckets > 256) return bad(-1, "rel_buckets must be 1..256");
+    if (a.rel_max_distance < 1 || a.rel_max_distance > 1024) return bad(-1, "rel_max_distance must be 1..1024");
+  }
+  struct T { const void* p; const int64_t* st; bool out; };
+  const T t[] = {{a.q, a.q_stride, false}, {a.k, a.k_stride, false}, {a.v, a.v_stride, false}, {a.out, a.out_stride, !backward},
+                 {a.dout, a.dout_stride, false}, {a.dq, a.dq_stride, true}, {a.dk, a.dk_stride, true}, {a.dv, a.dv_stride, true}};
+  for (int i = 0; i < (backward ? 8 : 4); ++i) {
+    if (!t[i].p) return bad(-1, "null tensor");
+    if ((uintptr_t)t[i].p & 15) return bad(-1, "tensors must be 16-byte aligned");
+    for (int k = 0; k < 3; ++k) {
+      if (t[i].st[k] & 7) return bad(-1, "strides must be multiples of 8 elements");
+      const int n[3] = {a.B, i == 1 || i == 2 || i == 6 || i == 7 ? a.nk : a.nq, i == 1 || i == 2 || i == 6 || i == 7 ? a.Hkv : a.H};
+      if (t[i].out && t[i].st[k] == 0 && n[k] > 1) return bad(-1, "an output must not be broadcast");
+    }
+  }
+  if ((uintptr_t)a.out_lo & 15) return bad(-1, "tensors must be 16-byte aligned");
+  if (backward && !a.lse) return bad(-1, "the backward needs the forward's lse");
+  if (backward && a.rel_table && !a.drel) return bad(-1, "the backward with rel_table needs drel");
+  return 0;
+}
+
+size_t rel_attention_ws(const FactAttention& a, bool backward) {
+  if (backward) {
+    size_t n = up16((size_t)a.B * a.H * a.nq * 4);
+    if (a.rel_table) n += (size_t)a.B * a.H * ((a.nq + 127) / 128) * (2 * a.rel_max_distance + 1) * 4;
+    return up16(n);
+  }
+  if (!few_rows(a)) return 0;
+  const int s = row_splits(a);
+  return s > 1 ? up16((size_t)s * a.B * a.H * a.nq * (a.dh + 4) * 4) : 0;
+}
+
+int launch_rel_attention_fwd(const FactAttention& a, void* ws, hipStream_t s) { return run(a, false, ws, s); }
+int launch_rel_attention_bwd(const FactAttention& a, void* ws, hipStream_t s) { return run(a, true, ws, s); }
+
+namespace {
+// little-endian base-2^32 number times a small one
+void times(std::vector<uint32_t>& x, uint32_t m) {
+  uint64_t carry = 0;
+  for (uint32_t& w : x) {
+    carry += (uint64_t)w * m;
+    w = (uint32_t)carry;
+    carry >>= 32;
+  }
+  if (carry) x.push_back((uint32_t)carry);
+}
+bool not_less(const std::vector<uint32_t>& x, const std::vector<uint32_t>& y) {
+  if (x.size() != y.size()) return x.size() > y.size();
+  for (size_t i = x.size(); i-- > 0;)
+    if (x[i] != y[i]) return x[i] > y[i];
+  return true;
+}
+}  // namespace
+
+// floor(log(d / e) / log(D / e) * w) >= t  <=>  d^w e^t >= D^t e^w, with e = exact buckets and w the logarithmic ones
+int relative_buckets(int num_buckets, int max_distance, int bidirectional, int32_t* map) {
+  const int n = bidirectional ? num_buckets / 2 : num_buckets, e = n / 2, w = n - e;
+  if (!map || num_buckets > 256 || n < 2 || (bidirectional && (num_buckets & 1)) || max_distance <= e || max_distance > 1024)
+    return -1;
+  std::vector<int> side(max_distance + 1);
+  for (int d = 0; d <= max_distance; ++d) {
+    if (d < e) {
+      side[d] = d;
+      continue;
+    }
+    int t = d > e ? side[d - 1] - e : 0;  // (buckets do not fall with the distance)
+    while (t + 1 < w) {
+      std::vector<uint32_t> x(1, 1), y(1, 1);
+      for (int i = 0; i < w; ++i) { times(x, d); times(y, e); }
+      for (int i = 0; i < t + 1; ++i) { times(x, e); times(y, max_distance); }
+      if (!not_less(x, y)) break;
+      ++t;
+    }
+    side[d] = e + t;
+  }
+  for (int d = -max_distance; d <= max_distance; ++d) {
+    int b = d > 0 ? (bidirectional ? n + side[d] : 0) : side[-d];
+    map[d + max_distance] = b;
+  }
+  return 0;
+}

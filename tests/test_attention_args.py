@@ -1,0 +1,168 @@
+"""What the attention operators refuse, and the bucket map, without a GPU: the C entry points check their arguments before they
+touch the device (the pointers below are never read)."""
+import ctypes as C
+import math
+import os
+from fractions import Fraction
+
+import pytest
+import torch
+
+from mint_amd import _lib as L
+from mint_amd import attention as A
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+@pytest.fixture(scope="module")
+def lib():
+    if not os.path.exists(L.LIB_PATH):
+        import __graft_entry__ as g
+        g.build()
+    return L.lib()
+
+
+def _attention(backward=True, **kw):
+    a = L.FactAttention(B=2, H=4, Hkv=2, nq=8, nk=24, dh=64, window_left=-1, window_right=-1, scale=0.125)
+    for i, n in enumerate(("q", "k", "v", "out", "lse", "dout", "dq", "dk", "dv")):
+        setattr(a, n, 4096 * (i + 1))
+    for n in ("q", "out", "dout", "dq"):
+        getattr(a, n + "_stride")[:] = (8 * 256, 256, 64)
+    for n in ("k", "v", "dk", "dv"):
+        getattr(a, n + "_stride")[:] = (24 * 128, 128, 64)
+    for n, v in kw.items():
+        if n.endswith("_stride"):
+            getattr(a, n)[:] = v
+        else:
+            setattr(a, n, v)
+    return a
+
+
+BIAS = dict(rel_table=1 << 20, rel_map=1 << 21, rel_buckets=32, rel_max_distance=128, drel=1 << 22)
+
+
+def test_struct_sizes_match_the_header(lib, tmp_path):
+    """The ctypes mirrors against a C compiler's layout of include/fact_hip.h."""
+    import subprocess
+    src = tmp_path / "s.c"
+    fields = [("FactAttention", f) for f, _ in L.FactAttention._fields_] + [("FactQkNorm", f) for f, _ in L.FactQkNorm._fields_]
+    src.write_text('#include <stdio.h>\n#include <stddef.h>\n#include "fact_hip.h"\nint main(void){printf("%zu %zu\\n",'
+                   "sizeof(FactAttention),sizeof(FactQkNorm));"
+                   + "".join('printf("%%zu\\n",offsetof(%s,%s));' % f for f in fields) + "return 0;}\n")
+    exe = str(tmp_path / "s")
+    subprocess.check_call(["gcc", "-I", os.path.join(ROOT, "include"), str(src), "-o", exe])
+    got = subprocess.check_output([exe], text=True).split()
+    assert [int(x) for x in got[:2]] == [C.sizeof(L.FactAttention), C.sizeof(L.FactQkNorm)]
+    assert [int(x) for x in got[2:]] == [getattr(getattr(L, s), f).offset for s, f in fields]
+
+
+@pytest.mark.parametrize("kw,rc,word", [
+    (dict(B=0), -1, "positive"), (dict(nk=0), -1, "positive"), (dict(Hkv=3), -1, "multiple"), (dict(dh=72), -3, "head dim"),
+    (dict(dh=48), -3, "head dim"), (dict(nq=1 << 30), -1, "2^30"), (dict(B=1 << 20, H=1 << 12, Hkv=1 << 12), -1, "too many"),
+    (dict(scale=0.0), -1, "scale"), (dict(scale=-1.0), -1, "scale"), (dict(scale=math.nan), -1, "scale"),
+    (dict(scale=math.inf), -1, "scale"), (dict(scale=1e-9), -1, "scale"), (dict(sinks=-1), -1, "sinks"),
+    (dict(q=None), -1, "null"), (dict(v=4096 + 8), -1, "aligned"), (dict(out_lo=4096 + 2), -1, "aligned"),
+    (dict(k_stride=(24 * 128, 132, 64)), -1, "multiples of 8"), (dict(dq_stride=(8 * 256, 0, 64)), -1, "broadcast"),
+    (dict(dk_stride=(0, 128, 64)), -1, "broadcast"), (dict(lse=None), -1, "lse"),
+    (dict(BIAS, rel_map=None), -1, "rel_map"), (dict(BIAS, rel_buckets=0), -1, "rel_buckets"),
+    (dict(BIAS, rel_buckets=257), -1, "rel_buckets"), (dict(BIAS, rel_max_distance=0), -1, "rel_max_distance"),
+    (dict(BIAS, rel_max_distance=1025), -1, "rel_max_distance"), (dict(BIAS, drel=None), -1, "drel")])
+def test_attention_refuses(lib, kw, rc, word):
+    a = _attention(**kw)
+    n = C.c_size_t(0)
+    assert lib.fact_attention_workspace(C.byref(a), 1, C.byref(n)) == rc
+    assert word in lib.fact_last_error().decode()
+    assert lib.fact_attention_backward(C.byref(a), 1 << 23, 1 << 40, None) == rc
+
+
+def test_attention_asks_for_its_workspace(lib):
+    n = C.c_size_t(0)
+    a = _attention()
+    assert lib.fact_attention_workspace(C.byref(a), 0, C.byref(n)) == 0 and n.value == 0
+    assert lib.fact_attention_workspace(C.byref(a), 1, C.byref(n)) == 0 and n.value >= 2 * 4 * 8 * 4
+    assert lib.fact_attention_backward(C.byref(a), None, 0, None) == -4
+    assert lib.fact_attention_backward(C.byref(a), 4096, n.value - 1, None) == -4
+    assert lib.fact_attention_backward(C.byref(a), 4100, n.value, None) == -1
+    # broadcast inputs are fine, an output with a zero stride over one element too
+    assert lib.fact_attention_workspace(C.byref(_attention(k_stride=(0, 128, 0), dq_stride=(0, 256, 64), B=1)), 1, C.byref(n)) == 0
+    # one row against a long cache: split over workgroups, so partial rows are kept
+    a = _attention(nq=1, nk=1 << 20)
+    assert lib.fact_attention_workspace(C.byref(a), 0, C.byref(n)) == 0 and n.value > 0
+    assert lib.fact_attention(C.byref(a), None, 0, None) == -4
+    assert lib.fact_attention_workspace(None, 0, C.byref(n)) == -1 and lib.fact_attention(None, None, 0, None) == -1
+
+
+def _norm(**kw):
+    a = L.FactQkNorm(B=2, n=8, H=4, Hkv=2, dh=64, rotary_dim=64, base=10000.0, eps=1e-6)
+    for i, n in enumerate(("q", "k", "q_out", "k_out", "dq_out", "dk_out", "dq", "dk")):
+        setattr(a, n, 4096 * (i + 1))
+        getattr(a, n + "_stride")[:] = (8 * 256, 256, 64)
+    for n, v in kw.items():
+        if n.endswith("_stride"):
+            getattr(a, n)[:] = v
+        else:
+            setattr(a, n, v)
+    return a
+
+
+@pytest.mark.parametrize("kw,rc,word", [
+    (dict(B=0), -1, "positive"), (dict(Hkv=0), -1, "positive"), (dict(n=1 << 30, B=1 << 10), -1, "too many"),
+    (dict(dh=132), -3, "head dim"), (dict(dh=20), -3, "head dim"), (dict(rotary_dim=72), -1, "rotary_dim"),
+    (dict(rotary_dim=-8), -1, "rotary_dim"), (dict(rotary_dim=12), -1, "rotary_dim"), (dict(dtype=2), -1, "dtype"),
+    (dict(eps=-1.0), -1, "eps"), (dict(eps=math.nan), -1, "eps"), (dict(base=0.0), -1, "base"), (dict(base=math.nan), -1, "base"),
+    (dict(k=None), -1, "null"), (dict(dq=4096 + 4), -1, "aligned"), (dict(q_gamma=4096 + 4), -1, "aligned"),
+    (dict(q_stride=(8 * 256, 252, 64)), -1, "multiples of 8"), (dict(dk_stride=(8 * 256, 0, 64)), -1, "broadcast")])
+def test_norm_refuses(lib, kw, rc, word):
+    n = C.c_size_t(0)
+    a = _norm(**kw)
+    assert lib.fact_qk_norm_workspace(C.byref(a), 1, C.byref(n)) == rc
+    assert word in lib.fact_last_error().decode()
+    assert lib.fact_qk_norm_backward(C.byref(a), 1 << 23, 1 << 40, None) == rc
+
+
+def test_norm_asks_for_its_workspace(lib):
+    n = C.c_size_t(0)
+    assert lib.fact_qk_norm_workspace(C.byref(_norm()), 0, C.byref(n)) == 0 and n.value == 0
+    assert lib.fact_qk_norm_workspace(C.byref(_norm()), 1, C.byref(n)) == 0 and n.value > 0
+    assert lib.fact_qk_norm_backward(C.byref(_norm()), None, 0, None) == -4
+    assert lib.fact_qk_norm(None, None, 0, None) == -1
+
+
+@pytest.mark.parametrize("buckets,dist,both", [(32, 128, True), (32, 128, False), (64, 512, True), (8, 20, True), (2, 5, False),
+                                               (4, 100, True), (256, 1024, False), (256, 1000, True), (6, 7, False), (18, 77, True)])
+def test_bucket_map_against_exact_powers(lib, buckets, dist, both):
+    m = A.relative_buckets(buckets, dist, both).tolist()
+    n = buckets // 2 if both else buckets
+    e = n // 2
+    for d in range(-dist, dist + 1):
+        far = abs(d) if both else max(-d, 0)
+        if far < e:
+            b = far
+        else:  # floor(log(far / e) / log(dist / e) * (n - e)) in exact arithmetic
+            t = 0
+            while t + 1 < n - e and Fraction(far, e) ** (n - e) >= Fraction(dist, e) ** (t + 1):
+                t += 1
+            b = e + t
+        assert m[d + dist] == b + (n if both and d > 0 else 0), d
+
+
+@pytest.mark.parametrize("args", [(1, 10, False), (3, 10, True), (258, 1000, False), (32, 8, True), (32, 1025, True), (0, 5, False),
+                                  (2, 1, False)])
+def test_bucket_map_refuses(lib, args):
+    with pytest.raises(L.FactError):
+        A.relative_buckets(*args)
+
+
+def test_python_calls_refuse_host_tensors():
+    q = torch.zeros(2, 4, 2, 64, dtype=torch.bfloat16)
+    for call in (lambda: A.attention(q, q, q), lambda: A.qk_norm_rope(q, q), lambda: A.attention(None, q, q),
+                 lambda: A.attention(q[0], q, q)):
+        with pytest.raises(ValueError):
+            call()
+
+
+def test_operator_sources_hold_nothing_that_a_graph_cannot_replay():
+    """Calls are captured into graphs: no memset nodes, no allocation, no synchronisation on the way."""
+    for f in ("rel_attention.hip", "qk_norm.hip"):
+        text = open(os.path.join(ROOT, "mint_amd", "csrc", f)).read()
+        assert "hipMemset" not in text and "hipMalloc" not in text and "Synchronize" not in text
