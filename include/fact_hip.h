@@ -227,9 +227,10 @@ int fact_set_option(FactHandle* h, const char* key, int value);
 typedef struct FactAttention {
   const void *q, *k, *v;   /* [B][nq][H][dh], [B][nk][Hkv][dh] twice */
   void* out;               /* [B][nq][H][dh] */
-  void* out_lo;            /* may be NULL: bf16 rounding residual of `out` (layout of out).  With it the forward's product with v
-                            * carries the probabilities to 16 bits and the backward's row sums dO . O take out + out_lo: what
-                            * the fp32 gradient of the table needs */
+  float* out_lo;           /* may be NULL: what the rounding of `out` left, fp32 [B][nq][H][dh] without gaps.  A forward that is
+                            * given it carries the probabilities to 24 bits through the product with v, and the backward's row
+                            * sums dO . O take out + out_lo: the fp32 gradient of the table needs it, the gradients of short
+                            * sequences (up to some 512 keys) gain from it */
   float* lse;              /* [B][H][nq] base-2 log-sum-exp of the scaled scores (+inf: row without keys); forward: may be NULL */
   const void* dout;        /* backward: gradient of out */
   void *dq, *dk, *dv;      /* backward: written */

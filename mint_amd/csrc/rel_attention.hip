@@ -86,6 +86,22 @@ DEVINL bf16x8 frag_tr(const bf16_t* t, int dt, int lane) {
   return cat4(lo, hi);
 }
 
+// x = hi + mid + lo to 24 bits; hi is given
+DEVINL void split3(f32x4 a, f32x4 b, const bf16x8& hi, bf16x8& mid, bf16x8& lo) {
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    a[r] -= (float)hi[r];
+    b[r] -= (float)hi[4 + r];
+  }
+  mid = pack8(a, b);
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    a[r] -= (float)mid[r];
+    b[r] -= (float)mid[4 + r];
+  }
+  lo = pack8(a, b);
+}
+
 DEVINL float allmax4(float v) {  // over the 4 lanes of a query
   v = fmaxf(v, __shfl_xor(v, 16, 64));
   return fmaxf(v, __shfl_xor(v, 32, 64));
@@ -101,6 +117,13 @@ struct Vis {
   DEVINL bool seen(int j, int p) const {
     const int d = j - p;  // (selects, no branches: hipcc dropped one of the branchy form's stores)
     return (j < len) & (d <= hi) & ((d >= lo) | (j < sinks));
+  }
+  // sees one key only: its softmax is 1 whatever the score, its dS exactly 0 (which P (dP - D) misses by a rounding).  Such a
+  // row never lies in a tile that is full.
+  DEVINL bool lone(int p) const {
+    const long long top = min((long long)len, hi == INT_MAX ? (long long)len : (long long)p + hi + 1);
+    const long long low = lo == INT_MIN ? 0 : max(0ll, (long long)p + lo), sk = min((long long)sinks, top);
+    return max(0ll, top - max(low, sk)) + max(0ll, sk) == 1;
   }
   // a 32-key tile at j0 against positions p0 .. p0 + 31
   DEVINL bool none(int j0, int p0) const {
@@ -137,6 +160,9 @@ DEVINL Tiles tiles_of(const Vis& v, long long pa, long long pb) {
   t.T = t.ns + (lo < hi ? max(0, t1 - t.t0) : 0);
   return t;
 }
+
+// row of the residual a.out_lo: [B][nq][H][dh] without gaps
+DEVINL size_t low_row(const FactAttention& a, int b, int h, int q) { return (((size_t)b * a.nq + q) * a.H + h) * a.dh; }
 
 // Workgroups of one head (and of the heads that share its keys) are neighbours on one XCD (consecutive workgroups go to
 // consecutive XCDs): they then read the same K / V rows through one L2.  Speed only.
@@ -188,13 +214,13 @@ DEVINL void load_bias(float* eb, const RelP& p, int h, int tid, int nthr) {
 // ---------------------------------------------------------------------------------------------------------------------
 // forward: workgroup = 128 queries of one head, 4 waves x 32 queries; 32-key tiles double-buffered in LDS
 // ---------------------------------------------------------------------------------------------------------------------
-// MODE 0: no bias, 1: bias, 2: bias, and the probabilities enter P V as a sum of two bf16 values: with one, the rounding of P
-// moves rowsum(dO . O) by 1e-3 of itself, and the fp32 gradient of the table, a sum of dS over whole diagonals, with it
-template <int DH, int MODE>
+// EXACT (a.out_lo given): the probabilities enter P V as a sum of three bf16 values, 24 bits, and the output's rounding residual
+// is kept in fp32.  The backward takes D = rowsum(dO . O) from them: from the rounded P and O it is off by 1e-3 of itself, which
+// dS = P (dP - D) and with it the fp32 gradient of the table inherit (two values: 3e-6 of the table's gradient, three: 3e-7).
+template <int DH, bool REL, bool EXACT>
 __global__ __launch_bounds__(256, 2) void rel_fwd_kernel(const RelP p) {
   using G = Geo<DH>;
   constexpr int ND = G::ND;
-  constexpr bool REL = MODE > 0;
   extern __shared__ __attribute__((aligned(16))) bf16_t smem[];
   float* eb = reinterpret_cast<float*>(smem + 4 * G::IMG);
   const FactAttention& a = p.a;
@@ -284,7 +310,7 @@ __global__ __launch_bounds__(256, 2) void rel_fwd_kernel(const RelP p) {
           for (int r = 0; r < 4; ++r)
             s[ks][qs][r] = v.seen(j0 + ks * 16 + 4 * g + r, p0 + qs * 16 + c) ? s[ks][qs][r] : -INFINITY;
     }
-    bf16x8 pb[2], pl[2];
+    bf16x8 pb[2], pl[2], pm[2];
 #pragma unroll
     for (int qs = 0; qs < 2; ++qs) {
       float mx = fmaxf(fmaxf(fmaxf(s[0][qs][0], s[0][qs][1]), fmaxf(s[0][qs][2], s[0][qs][3])),
@@ -309,14 +335,7 @@ __global__ __launch_bounds__(256, 2) void rel_fwd_kernel(const RelP p) {
       }
       l[qs] += ls;
       pb[qs] = pack8(e0, e1);
-      if (MODE == 2) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          e0[r] -= (float)pb[qs][r];
-          e1[r] -= (float)pb[qs][4 + r];
-        }
-        pl[qs] = pack8(e0, e1);
-      }
+      if (EXACT) split3(e0, e1, pb[qs], pm[qs], pl[qs]);
     }
 #pragma unroll
     for (int dt = 0; dt < ND; ++dt) {
@@ -324,7 +343,10 @@ __global__ __launch_bounds__(256, 2) void rel_fwd_kernel(const RelP p) {
 #pragma unroll
       for (int qs = 0; qs < 2; ++qs) {
         O[qs][dt] = mfma16(vf, pb[qs], O[qs][dt]);
-        if (MODE == 2) O[qs][dt] = mfma16(vf, pl[qs], O[qs][dt]);
+        if (EXACT) {
+          O[qs][dt] = mfma16(vf, pm[qs], O[qs][dt]);
+          O[qs][dt] = mfma16(vf, pl[qs], O[qs][dt]);
+        }
       }
     }
   }
@@ -339,15 +361,16 @@ __global__ __launch_bounds__(256, 2) void rel_fwd_kernel(const RelP p) {
     const long long off = b * a.out_stride[0] + (long long)q * a.out_stride[1] + h * a.out_stride[2] + g * 4;
 #pragma unroll
     for (int dt = 0; dt < ND; ++dt) {
-      bf16x4 o, lo;
+      bf16x4 o;
+      f32x4 lo;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const float x = O[qs][dt][r] * inv;
         o[r] = (bf16_t)x;
-        lo[r] = (bf16_t)(x - (float)o[r]);
+        lo[r] = x - (float)o[r];
       }
       *reinterpret_cast<bf16x4*>((bf16_t*)a.out + off + dt * 16) = o;
-      if (a.out_lo) *reinterpret_cast<bf16x4*>((bf16_t*)a.out_lo + off + dt * 16) = lo;
+      if (EXACT) *reinterpret_cast<f32x4*>(a.out_lo + low_row(a, b, h, q) + g * 4 + dt * 16) = lo;
     }
   }
 }
@@ -382,27 +405,45 @@ __global__ __launch_bounds__(256, 2) void rel_dq_kernel(const RelP p) {
   if (tl.T > 0) st.load(tl.at(0) * 32, v.len - 1);
   Frag<DH> Q[2], dO[2];
   float nL[2], nD[2];
+  bool live[2];  // a query of the call that sees more than one key
 #pragma unroll
   for (int qs = 0; qs < 2; ++qs) {
     const int q = min(q0 + qs * 16 + c, a.nq - 1);
+    live[qs] = (q0 + qs * 16 + c < a.nq) & !v.lone(start + q);
     frag_load<DH>(Q[qs], (const bf16_t*)a.q + b * a.q_stride[0] + (long long)q * a.q_stride[1] + h * a.q_stride[2], g);
     frag_load<DH>(dO[qs], (const bf16_t*)a.dout + b * a.dout_stride[0] + (long long)q * a.dout_stride[1] + h * a.dout_stride[2], g);
     const long long off = b * a.out_stride[0] + (long long)q * a.out_stride[1] + h * a.out_stride[2];
     float part = 0.f;
-    auto rowsum = [&](const bf16_t* o) {
+    {
       Frag<DH> f;
-      frag_load<DH>(f, o, g);
+      frag_load<DH>(f, (const bf16_t*)a.out + off, g);
 #pragma unroll
       for (int kd = 0; kd < G::KD; ++kd)
 #pragma unroll
         for (int j = 0; j < 8; ++j) part += (float)dO[qs].f[kd][j] * (float)f.f[kd][j];
-    };
-    rowsum((const bf16_t*)a.out + off);
-    if (a.out_lo) rowsum((const bf16_t*)a.out_lo + off);
+      if (a.out_lo) {
+        const float* lo = a.out_lo + low_row(a, b, h, q);
+#pragma unroll
+        for (int kd = 0; kd < G::KD; ++kd)
+          if (kd * 32 + 32 <= DH || kd * 32 + g * 8 < DH) {
+            const f32x4 x = *reinterpret_cast<const f32x4*>(lo + kd * 32 + g * 8);
+            const f32x4 y = *reinterpret_cast<const f32x4*>(lo + kd * 32 + g * 8 + 4);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) part += (float)dO[qs].f[kd][j] * x[j] + (float)dO[qs].f[kd][4 + j] * y[j];
+          }
+      }
+    }
     part = allsum4(part);
     const size_t at = ((size_t)b * a.H + h) * a.nq + q;
     nL[qs] = -a.lse[at];
-    nD[qs] = -part;
+    nD[qs] = qs ? part : -part;
+    // The second sub-tile of queries is carried with its sign turned over (dS, hence dQ): the matrix pipe adds with a rounding
+    // that leans down by 0.02 of a last place, which the millions of dS behind one table entry add up to 3.5e-6 of its gradient.
+    if (qs) {
+#pragma unroll
+      for (int kd = 0; kd < G::KD; ++kd)
+        dO[qs].f[kd] = __builtin_bit_cast(bf16x8, __builtin_bit_cast(u32x4, dO[qs].f[kd]) ^ 0x80008000u);
+    }
     if (active && g == 0) p.dsum[at] = part;  // for the dK / dV kernel (repeated rows write the same value)
   }
   pad_zero<DH>(smem, 4, tid, 256);
@@ -482,21 +523,21 @@ __global__ __launch_bounds__(256, 2) void rel_dq_kernel(const RelP p) {
         for (int qs = 0; qs < 2; ++qs)
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            ds[ks][qs][r] = (v.seen(j0 + ks * 16 + 4 * g + r, p0 + qs * 16 + c) & (q0 + qs * 16 + c < a.nq)) ? ds[ks][qs][r] : 0.f;
+            ds[ks][qs][r] = (v.seen(j0 + ks * 16 + 4 * g + r, p0 + qs * 16 + c) & live[qs]) ? ds[ks][qs][r] : 0.f;
     }
     if (REL) {
       if (left || right) {
         float x = 0.f;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) x += (ds[0][0][r] + ds[1][1][r]) + (ds[0][1][r] + ds[1][0][r]);
+        for (int r = 0; r < 4; ++r) x += (ds[0][0][r] - ds[1][1][r]) + (ds[1][0][r] - ds[0][1][r]);
         if (left) farl += x;
         else farr += x;
       } else {
         float* e = bins + d0 + D + PAD + 4 * g - c;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          atomicAdd(e + r - 16, ds[0][1][r]);
-          atomicAdd(e + r, ds[0][0][r] + ds[1][1][r]);
+          atomicAdd(e + r - 16, -ds[0][1][r]);
+          atomicAdd(e + r, ds[0][0][r] - ds[1][1][r]);
           atomicAdd(e + r + 16, ds[1][0][r]);
         }
       }
@@ -521,7 +562,7 @@ __global__ __launch_bounds__(256, 2) void rel_dq_kernel(const RelP p) {
       for (int dt = 0; dt < ND; ++dt) {
         bf16x4 o;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) o[r] = (bf16_t)(dQ[qs][dt][r] * a.scale);
+        for (int r = 0; r < 4; ++r) o[r] = (bf16_t)(dQ[qs][dt][r] * (qs ? -a.scale : a.scale));
         *reinterpret_cast<bf16x4*>(row + dt * 16) = o;
       }
     }
@@ -714,6 +755,11 @@ __global__ __launch_bounds__(256, DH > 96 ? 1 : 2) void rel_dkdv_kernel(const Re
           dp[qs][ks][r] *= pr[qs][ks][r];
         }
     if (!v.full(j0, p0) || q0 + 31 >= a.nq) {
+      bool lone[2][4];
+#pragma unroll
+      for (int qs = 0; qs < 2; ++qs)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) lone[qs][r] = v.lone(p0 + qs * 16 + 4 * g + r);
 #pragma unroll
       for (int qs = 0; qs < 2; ++qs)
 #pragma unroll
@@ -722,7 +768,7 @@ __global__ __launch_bounds__(256, DH > 96 ? 1 : 2) void rel_dkdv_kernel(const Re
           for (int r = 0; r < 4; ++r) {
             const bool ok = v.seen(j0 + ks * 16 + c, p0 + qs * 16 + 4 * g + r) & (q0 + qs * 16 + 4 * g + r < a.nq);
             pr[qs][ks][r] = ok ? pr[qs][ks][r] : 0.f;
-            dp[qs][ks][r] = ok ? dp[qs][ks][r] : 0.f;
+            dp[qs][ks][r] = (ok & !lone[qs][r]) ? dp[qs][ks][r] : 0.f;
           }
     }
     bf16x8 pb[2], db[2];
@@ -849,21 +895,17 @@ __global__ __launch_bounds__(256, 2) void rel_rows_kernel(const RelP p) {
     }
     l = l * alpha + ls;
     const bf16x8 pb = pack8(e0, e1);
-    bf16x8 pl = zero_bf16x8();
-    if (a.out_lo) {  // as in the forward above
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        e0[r] -= (float)pb[r];
-        e1[r] -= (float)pb[4 + r];
-      }
-      pl = pack8(e0, e1);
-    }
+    bf16x8 pm = zero_bf16x8(), pl = zero_bf16x8();
+    if (a.out_lo) split3(e0, e1, pb, pm, pl);  // as in the forward above
     __builtin_amdgcn_wave_barrier();  // the tile below was written by this wave alone: its LDS accesses stay in order
 #pragma unroll
     for (int dt = 0; dt < ND; ++dt) {
       const bf16x8 vf = frag_tr<DH>(Vs, dt, lane);
       O[dt] = mfma16(vf, pb, O[dt] * alpha);
-      if (a.out_lo) O[dt] = mfma16(vf, pl, O[dt]);
+      if (a.out_lo) {
+        O[dt] = mfma16(vf, pm, O[dt]);
+        O[dt] = mfma16(vf, pl, O[dt]);
+      }
     }
     __builtin_amdgcn_wave_barrier();
   }
@@ -902,14 +944,15 @@ __global__ __launch_bounds__(256, 2) void rel_rows_kernel(const RelP p) {
       const float inv = lt == 0.f ? 0.f : 1.0f / lt;
       if (a.lse && d == 0) a.lse[((size_t)b * a.H + hh) * a.nq + q] = lt == 0.f ? INFINITY : M + __log2f(lt);
       const long long off = b * a.out_stride[0] + (long long)q * a.out_stride[1] + hh * a.out_stride[2] + d;
-      bf16x4 x, y;
+      bf16x4 x;
+      f32x4 y;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         x[k] = (bf16_t)(o[k] * inv);
-        y[k] = (bf16_t)(o[k] * inv - (float)x[k]);
+        y[k] = o[k] * inv - (float)x[k];
       }
       *reinterpret_cast<bf16x4*>((bf16_t*)a.out + off) = x;
-      if (a.out_lo) *reinterpret_cast<bf16x4*>((bf16_t*)a.out_lo + off) = y;
+      if (a.out_lo) *reinterpret_cast<f32x4*>(a.out_lo + low_row(a, b, hh, q) + d) = y;
     }
   }
 }
@@ -942,10 +985,7 @@ __global__ __launch_bounds__(64) void rel_join_kernel(const RelP p) {
   const long long off = b * a.out_stride[0] + (long long)q * a.out_stride[1] + h * a.out_stride[2] + d;
   bf16x2 x = {(bf16_t)(o0 * inv), (bf16_t)(o1 * inv)};
   *reinterpret_cast<bf16x2*>((bf16_t*)a.out + off) = x;
-  if (a.out_lo) {
-    bf16x2 y = {(bf16_t)(o0 * inv - (float)x[0]), (bf16_t)(o1 * inv - (float)x[1])};
-    *reinterpret_cast<bf16x2*>((bf16_t*)a.out_lo + off) = y;
-  }
+  if (a.out_lo) *reinterpret_cast<f32x2*>(a.out_lo + low_row(a, b, h, q) + d) = f32x2{o0 * inv - (float)x[0], o1 * inv - (float)x[1]};
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------
@@ -1007,9 +1047,7 @@ int fwd_t(const FactAttention& a, void* ws, hipStream_t s) {
     FACT_LAUNCH(kernel, dim3(p.nwg), dim3(256), lds, s, p);
     return launched();
   };
-  if constexpr (REL)
-    if (a.out_lo) return go(rel_fwd_kernel<DH, 2>);
-  return go(rel_fwd_kernel<DH, REL ? 1 : 0>);
+  return a.out_lo ? go(rel_fwd_kernel<DH, REL, true>) : go(rel_fwd_kernel<DH, REL, false>);
 }
 
 template <int DH, bool REL>

@@ -6,8 +6,8 @@ Bounds are elementwise and follow the roundings the kernels make (half a step of
   D     = rowsum(dO . out), with out off by the above                                    sum_d |dO| d(out)
   dS    = P (dP - D) enters its products as bf16                                         h |dS| + P d(D)
   dq    scale sum_j d(dS) |K| + h |dq|;  dk likewise;  dv  h (P^T |dO| + |dv|)
-With a bias the probabilities and the output are carried to 16 bits for D (d(out) = 2^-16 of the same sum) and the table's
-gradient sums dS unrounded.  fp32 arithmetic adds at most 2^-15 of the absolute sums (128 terms, exp2 of |x| < 64).
+With a bias (and up to 512 keys) the probabilities and the output are carried to 24 bits for D (d(out) = 2^-20 of the same sum)
+and the table's gradient sums dS unrounded.  fp32 arithmetic adds at most 2^-15 of the absolute sums (128 terms, exp2 of |x| < 64).
 """
 import math
 
@@ -73,7 +73,7 @@ def _reference(q, k, v, scale, window=(-1, -1), sinks=0, rel_table=None, rel_map
     dP = do @ vh.transpose(-1, -2)
     Dr = (do * out).sum(-1, keepdim=True)
     dS = P * (dP - Dr)
-    h_out = 2.0 ** -16 if rel_table is not None else H8
+    h_out = 2.0 ** -20 if rel_table is not None or nk <= A.EXACT_KEYS else H8
     dD = (do.abs() * (h_out * (Av + out.abs()) + F32 * Av)).sum(-1, keepdim=True)
     e32 = F32 * P * (do.abs() @ vh.abs().transpose(-1, -2) + (do.abs() * Av).sum(-1, keepdim=True))
     edS = H8 * dS.abs() + P * dD + e32
@@ -268,6 +268,7 @@ def test_strides_packed_views_broadcast_and_unaligned_inputs():
     assert torch.equal(A.attention(q, one, v), A.attention(q, one.contiguous(), v))
     # packed destinations; nothing around them is touched
     dst = torch.full((B, n, 3, H, dh), 7.0, dtype=torch.bfloat16, device=DEV)
+    base, _ = A.attention(q.contiguous(), k.contiguous(), v.contiguous(), training=True)
     o, saved = A.attention(q, k, v, training=True, out=dst[:, :, 1])
     assert o.data_ptr() == dst[:, :, 1].data_ptr() and torch.equal(dst[:, :, 1], base)
     assert (dst[:, :, 0] == 7).all() and (dst[:, :, 2] == 7).all()
@@ -307,6 +308,20 @@ def test_results_repeat_exactly():
     first = once()
     for _ in range(3):
         assert all(torch.equal(x, y) for x, y in zip(first, once()))
+
+
+def test_rows_with_one_key_have_no_score_gradient():
+    """A softmax over one key is constant: dq, dk and the table's gradient are exactly zero, dv is dout."""
+    gen = torch.Generator().manual_seed(30)
+    q, k, v, do = (_rand(gen, 3, 50, 4, 80) for _ in range(4))
+    t, m = _table(gen, 4)
+    for kw in (dict(window=(0, 0)), dict(kv_len=torch.ones(3, dtype=torch.int32, device=DEV)), dict(window=(0, -1), kv_len=torch.ones(3, dtype=torch.int32, device=DEV), sinks=1)):
+        for bias in ({}, dict(rel_table=t, rel_map=m)):
+            o, saved = A.attention(q, k, v, training=True, **kw, **bias)
+            g = A.attention_backward(do, q, k, v, o, saved, **kw, **bias)
+            assert (g[0] == 0).all() and (g[1] == 0).all() and (len(g) < 4 or (g[3] == 0).all())
+            if kw.get("window") == (0, 0):
+                assert torch.equal(o, v) and torch.equal(g[2], do)
 
 
 def test_gradients_against_differences():
