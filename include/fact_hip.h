@@ -206,6 +206,23 @@ int fact_set_grad_callback(FactHandle* h, fact_grad_cb cb, void* user, void* com
  *                        add a communication stream (data parallelism) set 0 to stay within the hardware queues */
 int fact_set_option(FactHandle* h, const char* key, int value);
 
+/* Attention options of one transformer stack.  All zero: the reference's attention (full, absolute position tables only,
+ * mint/core/base_models.py:66,82-85).  The learned tensors they add stand behind each layer's to_qkv kernel in the parameter
+ * table: attn/q_norm/gamma and attn/k_norm/gamma [1][dh] (kind 2), attn/relative_bias/table [rel_buckets][heads] (kind 4). */
+typedef struct FactAttnCfg {
+  int qk_norm;          /* 1: fact_qk_norm on the projected queries and keys, learned gains (eps = FactConfig.ln_eps) */
+  int rotary_dim;       /* with qk_norm: rotate the first rotary_dim values of each head by token index; a multiple of 8 */
+  float rotary_base;    /* 0: 10000 */
+  int window;           /* > 0: a token sees the tokens up to `window` before and after it */
+  int sinks;            /* with window: and the first `sinks` tokens */
+  int rel_buckets;      /* > 0: learned relative position bias, fact_relative_buckets(rel_buckets, rel_max_distance, 1) */
+  int rel_max_distance;
+} FactAttnCfg;
+/* fact_arena_size / fact_create with attention options: attn[3] = motion, audio, cross-modal stack; NULL = none. */
+int fact_arena_size_ex(const FactConfig* cfg, const FactAttnCfg* attn, size_t* arena_floats, int* n_tensors);
+int fact_create_ex(const FactConfig* cfg, const FactAttnCfg* attn, int max_batch, int training, const FactArenas* arenas,
+                   FactHandle** out);
+
 /* ---- attention operators with relative positions --------------------------------------------------------------------
  * Handle-free operators on caller tensors (bf16 unless stated); the engine runs the same kernels for a stack whose
  * FactAttnCfg asks for them (fact_create_ex).  No allocation, no host synchronisation and no memset nodes: every call can be

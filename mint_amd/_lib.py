@@ -46,6 +46,11 @@ class FactArenas(C.Structure):
                 ("adam_v", C.c_void_p)]
 
 
+class FactAttnCfg(C.Structure):
+    _fields_ = [("qk_norm", C.c_int), ("rotary_dim", C.c_int), ("rotary_base", C.c_float), ("window", C.c_int),
+                ("sinks", C.c_int), ("rel_buckets", C.c_int), ("rel_max_distance", C.c_int)]
+
+
 class FactAttention(C.Structure):
     _fields_ = ([(n, C.c_void_p) for n in ("q", "k", "v", "out", "out_lo", "lse", "dout", "dq", "dk", "dv", "drel", "rel_table",
                                            "rel_map", "kv_len", "q_start")]
@@ -76,6 +81,8 @@ SIGNATURES = {
     "fact_last_error": (C.c_char_p, []),
     "fact_arena_size": (_i, [C.POINTER(FactConfig), C.POINTER(_sz), C.POINTER(_i)]),
     "fact_create": (_i, [C.POINTER(FactConfig), _i, _i, C.POINTER(FactArenas), C.POINTER(_vp)]),
+    "fact_arena_size_ex": (_i, [C.POINTER(FactConfig), C.POINTER(FactAttnCfg), C.POINTER(_sz), C.POINTER(_i)]),
+    "fact_create_ex": (_i, [C.POINTER(FactConfig), C.POINTER(FactAttnCfg), _i, _i, C.POINTER(FactArenas), C.POINTER(_vp)]),
     "fact_destroy": (_i, [_vp]),
     "fact_param_table": (_i, [_vp, C.POINTER(C.POINTER(FactParamDesc)), C.POINTER(_i)]),
     "fact_arenas": (_i, [_vp, C.POINTER(FactArenas), C.POINTER(_sz)]),

@@ -69,6 +69,7 @@ struct DenseW {
 struct LayerP {
   Tensor ln1_g, ln1_b, bo, ln2_g, ln2_b, b1, b2;
   DenseW wqkv, wo, w1, w2;
+  Tensor qn_g, kn_g, rel;  // FactAttnCfg: gains of the q / k norm [1][dh], relative bias table [buckets][heads]
 };
 
 struct LayerA {
@@ -76,6 +77,8 @@ struct LayerA {
   float *mean1 = nullptr, *rstd1 = nullptr, *mean2 = nullptr, *rstd2 = nullptr;
   bf16_t *h1 = nullptr, *a = nullptr, *h2 = nullptr, *pre = nullptr, *g = nullptr;
   bf16_t* row[3] = {nullptr, nullptr, nullptr};
+  bf16_t* nrow[2] = {nullptr, nullptr};  // q / k norm: normalised queries and keys (without it, and in inference: row[0], row[1])
+  float* out_lo = nullptr;               // attention options, training: what the rounding of `a` left (FactAttention)
   float* lse2 = nullptr;
   bool h1_ready = false;  // transient: the previous layer's FFN2 epilogue pass already wrote h1 / mean1 / rstd1 (ln_fuse)
 };
@@ -91,6 +94,10 @@ struct Stack {
   Tensor emb_b, pos;
   bf16_t* xin16 = nullptr;  // [B*n][featp]
   float* x0 = nullptr;      // stack input  [B*n][d]
+  FactAttnCfg at = {};      // attention options
+  int32_t* rel_map = nullptr;
+  char* attn_ws = nullptr;  // forward workspace (few query rows)
+  bool ext() const { return at.window > 0 || at.rel_buckets > 0; }  // runs rel_attention.hip
   float* out() { return L ? la[L - 1].x_out : x0; }
 };
 
@@ -159,6 +166,7 @@ struct BwScratch {
   bf16_t* dh = nullptr;      // [M][d pitch] dgrad output feeding the LayerNorm backward (fused-kernel path)
   bf16_t* dorow = nullptr;   // per-head dO rows
   float* dsum = nullptr;     // rowsum(dO o O)
+  char* attn_ws = nullptr;   // workspace of the attention options' backward kernels
   float* ln_ws = nullptr;    // LayerNorm-backward per-block partial column sums (fused-kernel path)
   // buffers both the dgrad chain and the wgrad stream touch, indexed by layer parity q = layer count % 3
   bf16_t* dpre_pp[kBwBuf] = {};   // [M][ff pitch]
@@ -397,6 +405,11 @@ void build_stack_params(TableBuilder& tb, Stack& st, const std::string& prefix) 
     p.ln1_g = tb.add(b + "/attn_norm/gamma", 1, st.d, 2);
     p.ln1_b = tb.add(b + "/attn_norm/beta", 1, st.d, 3);
     p.wqkv.w = tb.add(b + "/attn/to_qkv/kernel", st.d, 3 * st.d, 0);
+    if (st.at.qk_norm) {
+      p.qn_g = tb.add(b + "/attn/q_norm/gamma", 1, st.dh, 2);
+      p.kn_g = tb.add(b + "/attn/k_norm/gamma", 1, st.dh, 2);
+    }
+    if (st.at.rel_buckets > 0) p.rel = tb.add(b + "/attn/relative_bias/table", st.at.rel_buckets, st.H, 4);
     p.wo.w = tb.add(b + "/attn/to_out/kernel", st.d, st.d, 0);
     p.bo = tb.add(b + "/attn/to_out/bias", 1, st.d, 1);
     p.ln2_g = tb.add(b + "/mlp_norm/gamma", 1, st.d, 2);
@@ -467,6 +480,30 @@ int validate(const FactConfig& c) {
   return 0;
 }
 
+int validate_attn(const FactConfig& c, const FactAttnCfg* attn) {
+  if (!attn) return 0;
+  const FactStackCfg* s[3] = {&c.motion, &c.audio, &c.cross};
+  for (int i = 0; i < 3; ++i) {
+    const FactAttnCfg& a = attn[i];
+    const int dh = s[i]->hidden / s[i]->heads;
+    if (a.qk_norm != 0 && a.qk_norm != 1) return fail(-1, "qk_norm must be 0 or 1");
+    if (a.rotary_dim && !a.qk_norm) return fail(-1, "rotary_dim needs qk_norm");
+    if (a.rotary_dim < 0 || a.rotary_dim > dh || a.rotary_dim % 8)
+      return fail(-1, "rotary_dim must be a multiple of 8 up to the head dim " + std::to_string(dh));
+    if (!(a.rotary_base >= 0.f) || !(a.rotary_base < 3.0e38f)) return fail(-1, "rotary_base must be finite and not negative");
+    if (a.window < 0) return fail(-1, "the attention window must not be negative");
+    if (a.sinks < 0 || (a.sinks > 0 && a.window == 0)) return fail(-1, "attention sinks need an attention window");
+    if (a.rel_buckets < 0 || a.rel_buckets > 256) return fail(-1, "relative attention buckets must be 0..256");
+    if (a.rel_buckets > 0) {
+      if (a.rel_max_distance < 1 || a.rel_max_distance > 1024) return fail(-1, "relative attention max distance must be 1..1024");
+      std::vector<int32_t> map((size_t)2 * a.rel_max_distance + 1);
+      if (relative_buckets(a.rel_buckets, a.rel_max_distance, 1, map.data()))
+        return fail(-1, "relative attention: an even number of buckets, at least 2 a side, and a largest distance above the exact ones");
+    }
+  }
+  return 0;
+}
+
 void layout_dense(Bump& b, DenseW& w) {
   w.lds = rup(w.w.cols, kPitch);
   w.ldt = rup(w.w.rows, kPitch);
@@ -487,6 +524,57 @@ void layout_shadow(FactHandle* h, Bump& b) {
   layout_dense(b, h->head);
   layout_dense(b, h->motion.emb);
   layout_dense(b, h->audio.emb);
+}
+
+// The attention of layer l for the first nq query rows of every sequence (include/fact_hip.h FactAttention).
+FactAttention ext_attn(FactHandle* h, const Stack& st, const LayerP& p, const LayerA& a, int B, int nq) {
+  FactAttention f;
+  memset(&f, 0, sizeof(f));
+  auto strides = [](int64_t* s, int64_t b, int64_t n, int64_t hd) { s[0] = b; s[1] = n; s[2] = hd; };
+  const int64_t hp = (int64_t)st.NP * st.dhp;
+  f.q = a.nrow[0]; f.k = a.nrow[1]; f.v = a.row[2];
+  strides(f.q_stride, st.H * hp, st.dhp, hp);
+  strides(f.k_stride, st.H * hp, st.dhp, hp);
+  strides(f.v_stride, st.H * hp, st.dhp, hp);
+  f.out = a.a; f.out_lo = a.out_lo; f.lse = a.lse2;
+  strides(f.out_stride, (int64_t)st.n * st.dp, st.dp, st.dh);
+  f.B = B; f.H = f.Hkv = st.H; f.nq = nq; f.nk = st.n; f.dh = st.dh;
+  f.window_left = f.window_right = st.at.window > 0 ? st.at.window : -1;
+  f.sinks = st.at.sinks;
+  f.scale = 1.0f / sqrtf((float)st.d);  // dim**-0.5 with dim = hidden_size (base_models.py:66,104)
+  if (st.at.rel_buckets > 0) {
+    f.rel_table = h->params + p.rel.off;
+    f.rel_map = st.rel_map;
+    f.rel_buckets = st.at.rel_buckets;
+    f.rel_max_distance = st.at.rel_max_distance;
+    f.drel = h->grads ? h->grads + p.rel.off : nullptr;
+    f.drel_accumulate = 1;
+  }
+  return f;
+}
+FactQkNorm ext_norm(FactHandle* h, const Stack& st, const LayerP& p, const LayerA& a, int B) {
+  FactQkNorm f;
+  memset(&f, 0, sizeof(f));
+  const int64_t hp = (int64_t)st.NP * st.dhp;
+  f.q = a.row[0]; f.k = a.row[1]; f.q_out = a.nrow[0]; f.k_out = a.nrow[1];
+  for (int64_t* s : {f.q_stride, f.k_stride, f.q_out_stride, f.k_out_stride}) { s[0] = st.H * hp; s[1] = st.dhp; s[2] = hp; }
+  f.q_gamma = h->params + p.qn_g.off; f.k_gamma = h->params + p.kn_g.off;
+  f.B = B; f.n = st.n; f.H = f.Hkv = st.H; f.dh = st.dh; f.rotary_dim = st.at.rotary_dim;
+  f.base = st.at.rotary_base > 0.f ? st.at.rotary_base : 10000.0;
+  f.eps = h->cfg.ln_eps;
+  f.dgamma_accumulate = 1;
+  return f;
+}
+// bytes of the largest workspace a stack's attention options ask for
+size_t ext_ws(FactHandle* h, const Stack& st, int B, bool backward) {
+  size_t need = 0;
+  if (st.ext() && st.L)
+    for (int nq = backward ? st.n : 1; nq <= st.n; nq = (nq < 32 && nq + 1 < st.n) ? nq + 1 : (nq < st.n ? st.n : st.n + 1)) {
+      FactAttention f = ext_attn(h, st, st.lp[0], st.la[0], B, nq);
+      need = std::max(need, rel_attention_ws(f, backward));
+    }
+  if (st.at.qk_norm && st.L && backward) need = std::max(need, qk_norm_ws(ext_norm(h, st, st.lp[0], st.la[0], B), true));
+  return need;
 }
 
 void layout_stack_acts(FactHandle* h, Bump& b, Stack& st, int B) {
@@ -512,6 +600,10 @@ void layout_stack_acts(FactHandle* h, Bump& b, Stack& st, int B) {
     for (int w = 0; w < 3; ++w) {
       a.row[w] = b.take<bf16_t>(BH * st.NP * st.dhp);
     }
+    for (int w = 0; w < 2; ++w)
+      a.nrow[w] = (st.at.qk_norm && h->training) ? b.take<bf16_t>(BH * st.NP * st.dhp) : a.row[w];
+    // (short sequences gain from it without a bias too: FactAttention.out_lo)
+    if (st.ext() && h->training && (st.at.rel_buckets > 0 || st.n <= 512)) a.out_lo = b.take<float>(M * st.d);
     a.lse2 = b.take<float>(BH * st.NP);
   }
   float* pp[2] = {nullptr, nullptr};
@@ -525,6 +617,8 @@ void layout_stack_acts(FactHandle* h, Bump& b, Stack& st, int B) {
     a.x_out = h->training ? b.take<float>(M * st.d) : pp[l & 1];
     st.la[l] = a;
   }
+  if (st.at.rel_buckets > 0) st.rel_map = b.take<int32_t>((size_t)2 * st.at.rel_max_distance + 1);
+  if (st.ext()) st.attn_ws = b.take<char>(ext_ws(h, st, B, false));
 }
 
 void layout_work(FactHandle* h, Bump& b) {
@@ -598,6 +692,10 @@ void layout_work(FactHandle* h, Bump& b) {
       }
       sc.dorow = b.take<bf16_t>(rows);
       sc.dsum = b.take<float>(lse);
+      size_t aw = 0;
+      if (c) aw = ext_ws(h, h->motion, B, true);
+      else for (const Stack* st : sts) aw = std::max(aw, ext_ws(h, *st, B, true));
+      sc.attn_ws = b.take<char>(aw);
       sc.ln_ws = b.take<float>(ln_bwd_ws_floats((int)Mx, d));
       if (c) {  // chain 1 queues its weight gradients behind its own dgrad chain: own slabs
         sc.slab = b.take<float>((size_t)6 * rups((size_t)d * (ffmax > 3 * d ? ffmax : 3 * d), 4));
@@ -943,7 +1041,7 @@ void heads_ep(EpiParams& ep, const Stack& st, bf16_t* const* row, int nwhich) {
 AttnParams attn_params(const Stack& st, const LayerA& a, int B) {
   AttnParams ap;
   memset(&ap, 0, sizeof(ap));
-  ap.qrow = a.row[0]; ap.krow = a.row[1]; ap.vrow = a.row[2];
+  ap.qrow = a.nrow[0]; ap.krow = a.nrow[1]; ap.vrow = a.row[2];
   ap.out = a.a; ap.o = a.a; ap.lse2 = a.lse2;
   ap.B = B; ap.H = st.H; ap.n = st.n; ap.NP = st.NP; ap.hid = st.d; ap.dh = st.dh;
   ap.ldo = st.dp; ap.ldq = st.qp;
@@ -965,6 +1063,49 @@ hipEvent_t stream_after(FactHandle* h, hipStream_t from, hipStream_t to) {
   return e;
 }
 hipStream_t side_of(FactHandle* h, hipStream_t s) { return (h->use_side && h->side) ? h->side : s; }
+
+// q / k norm and attention of one layer; nq > 0: only the first nq query rows of every sequence are wanted
+int attn_forward(FactHandle* h, Stack& st, const LayerP& p, const LayerA& a, int B, int nq, hipStream_t s) {
+  if (st.at.qk_norm) CHK(launch_qk_norm_fwd(ext_norm(h, st, p, a, B), s));
+  if (st.ext()) {
+    CHK(launch_rel_attention_fwd(ext_attn(h, st, p, a, B, nq > 0 ? std::min(nq, st.n) : st.n), st.attn_ws, s));
+    return 0;
+  }
+  AttnParams ap = attn_params(st, a, B);
+  ap.nq = nq;
+  CHK(launch_attn_fwd(ap, s));
+  return 0;
+}
+// dqkv of one layer from the per-head dO rows in sc.dorow (nq > 0: rows past the first nq of every sequence are zero)
+int attn_backward(FactHandle* h, Stack& st, const LayerP& p, const LayerA& a, int B, int nq, BwScratch& sc, bf16_t* dqkv,
+                  hipStream_t s) {
+  const int64_t bs = (int64_t)st.n * st.qp;
+  if (st.ext()) {
+    const int rows = nq > 0 ? std::min(nq, st.n) : st.n;
+    FactAttention f = ext_attn(h, st, p, a, B, rows);
+    f.dout = sc.dorow;
+    for (int i = 0; i < 3; ++i) f.dout_stride[i] = f.q_stride[i];
+    f.dq = dqkv; f.dk = dqkv + st.d; f.dv = dqkv + 2 * st.d;
+    for (int64_t* t : {f.dq_stride, f.dk_stride, f.dv_stride}) { t[0] = bs; t[1] = st.qp; t[2] = st.dh; }
+    CHK(launch_rel_attention_bwd(f, sc.attn_ws, s));
+    if (rows < st.n) CHK(launch_zero_rows(dqkv, B, st.n, rows, st.qp, st.d, s));
+  } else {
+    AttnParams ap = attn_params(st, a, B);
+    ap.dorow = sc.dorow; ap.dsum = sc.dsum; ap.dqkv = dqkv;
+    ap.nq = nq;
+    CHK(launch_attn_bwd(ap, s));
+  }
+  if (st.at.qk_norm) {
+    FactQkNorm f = ext_norm(h, st, p, a, B);
+    f.dq_out = f.dq = dqkv;
+    f.dk_out = f.dk = dqkv + st.d;
+    for (int64_t* t : {f.dq_out_stride, f.dk_out_stride, f.dq_stride, f.dk_stride}) { t[0] = bs; t[1] = st.qp; t[2] = st.dh; }
+    f.dq_gamma = G(h, p.qn_g);
+    f.dk_gamma = G(h, p.kn_g);
+    CHK(launch_qk_norm_bwd(f, sc.attn_ws, s));
+  }
+  return 0;
+}
 
 int layer_forward(FactHandle* h, Stack& st, int l, int B, hipStream_t s) {
   const int M = B * st.n, d = st.d, dp = st.dp, fp = st.fp;
@@ -988,7 +1129,7 @@ int layer_forward(FactHandle* h, Stack& st, int l, int B, hipStream_t s) {
   }
   {
     KScope k(h, KP_ATTN_FWD, s, fl_attn);
-    CHK(launch_attn_fwd(attn_params(st, a, B), s));
+    CHK(attn_forward(h, st, p, a, B, 0, s));
   }
   {
     KScope k(h, KP_OUTPROJ, s, 2.0 * Md * d * d);
@@ -1052,9 +1193,7 @@ int layer_forward_sr(FactHandle* h, Stack& st, int l, int B, int T, hipStream_t 
   }
   {
     KScope k(h, KP_ATTN_FWD, s, 4.0 * (double)B * st.H * (double)T * st.n * st.dh);
-    AttnParams ap = attn_params(st, a, B);
-    ap.nq = T;
-    CHK(launch_attn_fwd(ap, s));
+    CHK(attn_forward(h, st, p, a, B, T, s));
   }
   CHK(launch_gather_rows(a.x_in, a.a, B, st.n, T, d, dp, r.x_in_c, r.a_c, s));
   {
@@ -1317,9 +1456,7 @@ int layer_backward(FactHandle* h, Stack& st, int l, int B, float* dx, bf16_t*& d
   }
   {
     KScope k(h, KP_ATTN_BWD, s, 2.5 * fl_attn, 0, 2);
-    AttnParams ap = attn_params(st, a, B);
-    ap.dorow = sc.dorow; ap.dsum = sc.dsum; ap.dqkv = dqkv;
-    if (!(h->skip & 4)) CHK(launch_attn_bwd(ap, s));
+    if (!(h->skip & 4)) CHK(attn_backward(h, st, p, a, B, 0, sc, dqkv, s));
   }
   {
     KScope k(h, KP_DQKV, s, 2.0 * Md * 3 * d * d);
@@ -1420,10 +1557,7 @@ int layer_backward_sr(FactHandle* h, Stack& st, int l, int B, int T, float* dx, 
   }
   {
     KScope k(h, KP_ATTN_BWD, s, 2.5 * 4.0 * (double)B * st.H * (double)T * st.n * st.dh, 0, 2);
-    AttnParams ap = attn_params(st, a, B);
-    ap.dorow = sc.dorow; ap.dsum = sc.dsum; ap.dqkv = dqkv;
-    ap.nq = T;
-    CHK(launch_attn_bwd(ap, s));
+    CHK(attn_backward(h, st, p, a, B, T, sc, dqkv, s));
   }
   {
     KScope k(h, KP_DQKV, s, 2.0 * Md * 3 * d * d);
@@ -1595,21 +1729,31 @@ static hipError_t make_stream(hipStream_t* s, const char* env) {
   return hipStreamCreateWithPriority(s, hipStreamNonBlocking, want > 0 ? least : greatest);
 }
 
-static void init_geo(FactHandle* h, const FactConfig* cfg) {
+static void init_geo(FactHandle* h, const FactConfig* cfg, const FactAttnCfg* attn) {
   h->cfg = *cfg;
   if (h->cfg.ln_eps <= 0.f) h->cfg.ln_eps = 1e-5f;
   init_stack_geo(h->motion, "motion", cfg->motion, cfg->motion.seq_len, cfg->motion.feature_dim);
   init_stack_geo(h->audio, "audio", cfg->audio, cfg->audio.seq_len, cfg->audio.feature_dim);
   init_stack_geo(h->cross, "cross", cfg->cross, cfg->motion.seq_len + cfg->audio.seq_len, 0);
   h->outp = rup(cfg->out_dim, 32);
+  if (attn) {
+    h->motion.at = attn[0];
+    h->audio.at = attn[1];
+    h->cross.at = attn[2];
+  }
 }
 
 int fact_arena_size(const FactConfig* cfg, size_t* arena_floats, int* n_tensors) {
+  return fact_arena_size_ex(cfg, nullptr, arena_floats, n_tensors);
+}
+
+int fact_arena_size_ex(const FactConfig* cfg, const FactAttnCfg* attn, size_t* arena_floats, int* n_tensors) {
   if (!cfg) return fail(-1, "null config");
   int rc = validate(*cfg);
+  if (!rc) rc = validate_attn(*cfg, attn);
   if (rc) return rc;
   FactHandle tmp;
-  init_geo(&tmp, cfg);
+  init_geo(&tmp, cfg, attn);
   std::vector<FactParamDesc> t;
   size_t total = 0;
   build_table(&tmp, &t, &total);
@@ -1620,12 +1764,18 @@ int fact_arena_size(const FactConfig* cfg, size_t* arena_floats, int* n_tensors)
 
 int fact_create(const FactConfig* cfg, int max_batch, int training, const FactArenas* arenas,
                 FactHandle** out) {
+  return fact_create_ex(cfg, nullptr, max_batch, training, arenas, out);
+}
+
+int fact_create_ex(const FactConfig* cfg, const FactAttnCfg* attn, int max_batch, int training, const FactArenas* arenas,
+                   FactHandle** out) {
   if (!cfg || !out) return fail(-1, "null argument");
   if (max_batch <= 0) return fail(-1, "max_batch must be positive");
   int rc = validate(*cfg);
+  if (!rc) rc = validate_attn(*cfg, attn);
   if (rc) return rc;
   FactHandle* h = new FactHandle();
-  init_geo(h, cfg);
+  init_geo(h, cfg, attn);
   h->max_batch = max_batch;
   h->training = training != 0;
   h->keep_pre_infer = getenv("FACT_KEEP_PRE") != nullptr;
@@ -1676,6 +1826,12 @@ int fact_create(const FactConfig* cfg, int max_batch, int training, const FactAr
     Bump b2;
     b2.base = h->work;
     layout_work(h, b2);
+    for (const Stack* st : {&h->motion, &h->audio, &h->cross})
+      if (st->at.rel_buckets > 0) {
+        std::vector<int32_t> map((size_t)2 * st->at.rel_max_distance + 1);
+        if (relative_buckets(st->at.rel_buckets, st->at.rel_max_distance, 1, map.data())) return fail(-1, "relative buckets");
+        HIPCHK(hipMemcpy(st->rel_map, map.data(), map.size() * sizeof(int32_t), hipMemcpyHostToDevice));
+      }
   }
   {
     int rc2 = build_buckets(h);

@@ -10,6 +10,9 @@ size_t rel_attention_ws(const FactAttention& a, bool backward);  // bytes, of a 
 int launch_rel_attention_fwd(const FactAttention& a, void* ws, hipStream_t s);
 int launch_rel_attention_bwd(const FactAttention& a, void* ws, hipStream_t s);
 
+// rows t0 .. n - 1 of every sequence of a [B * n][ld] bf16 matrix: `width` columns (a multiple of 8) cleared
+int launch_zero_rows(bf16_t* x, int B, int n, int t0, int ld, int width, hipStream_t s);
+
 int qk_norm_check(const FactQkNorm& a, bool backward, const char** why);
 size_t qk_norm_ws(const FactQkNorm& a, bool backward);
 int launch_qk_norm_fwd(const FactQkNorm& a, hipStream_t s);

@@ -988,6 +988,14 @@ __global__ __launch_bounds__(64) void rel_join_kernel(const RelP p) {
   if (a.out_lo) *reinterpret_cast<f32x2*>(a.out_lo + low_row(a, b, h, q) + d) = f32x2{o0 * inv - (float)x[0], o1 * inv - (float)x[1]};
 }
 
+__global__ __launch_bounds__(256) void zero_rows_kernel(bf16_t* x, int n, int t0, int ld, int chunks, long long total) {
+  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
+    const long long r = i / chunks;
+    const long long b = r / (n - t0), t = t0 + r - b * (n - t0);
+    *reinterpret_cast<u32x4*>(x + (b * n + t) * ld + (i - r * chunks) * 8) = u32x4{0u, 0u, 0u, 0u};
+  }
+}
+
 // ---- host ------------------------------------------------------------------------------------------------------------
 int launched() { return hipGetLastError() == hipSuccess ? 0 : -100; }
 
@@ -1130,6 +1138,15 @@ size_t rel_attention_ws(const FactAttention& a, bool backward) {
   if (!few_rows(a)) return 0;
   const int s = row_splits(a);
   return s > 1 ? up16((size_t)s * a.B * a.H * a.nq * (a.dh + 4) * 4) : 0;
+}
+
+int launch_zero_rows(bf16_t* x, int B, int n, int t0, int ld, int width, hipStream_t s) {
+  if (width & 7 || ld & 7 || (uintptr_t)x & 15) return -1;
+  const long long total = (long long)B * (n - t0) * (width / 8);
+  if (total <= 0) return 0;
+  FACT_LAUNCH(zero_rows_kernel, dim3((unsigned)std::min<long long>((total + 255) / 256, 4096)), dim3(256), 0, s, x, n, t0, ld,
+              width / 8, total);
+  return launched();
 }
 
 int launch_rel_attention_fwd(const FactAttention& a, void* ws, hipStream_t s) { return run(a, false, ws, s); }

@@ -86,6 +86,15 @@ class FACTModel:
             audio=stack(self._audio_cfg, p["audio"]["sequence_length"], self._feat["audio"]),
             cross=stack(self._cross_cfg, 0, 0), out_dim=self._out_dim, ln_eps=1e-5)
 
+    def _attn_structs(self):
+        """Attention options of the three stacks (transformer fields past the reference's schema, mint_amd/protos.py)."""
+        def one(t):
+            return L.FactAttnCfg(qk_norm=1 if t.qk_norm else 0, rotary_dim=t.rotary_dim, rotary_base=t.rotary_base,
+                                 window=t.attention_window, sinks=t.attention_sinks,
+                                 rel_buckets=t.relative_attention_num_buckets,
+                                 rel_max_distance=t.relative_attention_max_distance)
+        return (L.FactAttnCfg * 3)(*(one(t) for t in (self._motion_cfg, self._audio_cfg, self._cross_cfg)))
+
     def _check_config(self, motion_width, audio_width):
         cross = self.config.cross_modal_model
         # base_models.py:184-189
@@ -114,7 +123,8 @@ class FACTModel:
         torch.cuda.set_device(self._device)
         cfg = self._cfg_struct()
         n_floats, n_tensors = C.c_size_t(0), C.c_int(0)
-        L.check(lib.fact_arena_size(C.byref(cfg), C.byref(n_floats), C.byref(n_tensors)))
+        attn = self._attn_structs()
+        L.check(lib.fact_arena_size_ex(C.byref(cfg), attn, C.byref(n_floats), C.byref(n_tensors)))
         first = self._arena is None
         if first:
             names = ["params"] + (["grads", "adam_m", "adam_v"] if self.is_training else [])
@@ -129,8 +139,8 @@ class FACTModel:
                           adam_m=self._arena["adam_m"].data_ptr() if self.is_training else None,
                           adam_v=self._arena["adam_v"].data_ptr() if self.is_training else None)
         h = C.c_void_p()
-        L.check(lib.fact_create(C.byref(cfg), int(max_batch), 1 if self.is_training else 0, C.byref(ar),
-                                C.byref(h)))
+        L.check(lib.fact_create_ex(C.byref(cfg), attn, int(max_batch), 1 if self.is_training else 0, C.byref(ar),
+                                   C.byref(h)))
         self._h = h
         self._max_batch = int(max_batch)
         tab, n = C.POINTER(L.FactParamDesc)(), C.c_int(0)

@@ -167,6 +167,15 @@ Transformer = _msg("Transformer", {
     "sp_num_hidden_layers": ("int32", "optional", 12, None),
     "add_cls_token": ("bool", "optional", False, None),
     "weight_decay": ("float", "optional", 0.0, None),
+    # Attention options of this framework, past the reference's schema (include/fact_hip.h FactAttnCfg); the defaults are the
+    # reference's attention.
+    "qk_norm": ("bool", "optional", False, None),                # RMS norm of each query and key head, learned gains
+    "rotary_dim": ("int32", "optional", 0, None),                # with qk_norm: values of a head that turn with the position
+    "rotary_base": ("float", "optional", 10000.0, None),
+    "attention_window": ("int32", "optional", 0, None),          # tokens seen to either side; 0: all
+    "attention_sinks": ("int32", "optional", 0, None),           # first tokens that stay visible outside the window
+    "relative_attention_num_buckets": ("int32", "optional", 0, None),  # learned relative position bias; 0: none
+    "relative_attention_max_distance": ("int32", "optional", 128, None),
 })
 MLP = _msg("MLP", {
     "initializer_range": ("float", "optional", 0.02, None),

@@ -355,6 +355,10 @@ def tf_variable_path(name):
             "attn/to_qkv/kernel": attn + ["fn", "fn", "to_qkv", "kernel"],
             "attn/to_out/kernel": attn + ["fn", "fn", "to_out", "kernel"],
             "attn/to_out/bias": attn + ["fn", "fn", "to_out", "bias"],
+            # attention options of this framework (no counterpart in the reference's graph)
+            "attn/q_norm/gamma": attn + ["fn", "fn", "q_norm", "gamma"],
+            "attn/k_norm/gamma": attn + ["fn", "fn", "k_norm", "gamma"],
+            "attn/relative_bias/table": attn + ["fn", "fn", "relative_bias", "table"],
             "mlp_norm/gamma": mlp + ["fn", "norm", "gamma"], "mlp_norm/beta": mlp + ["fn", "norm", "beta"],
             "mlp/dense_1/kernel": mlp + ["fn", "fn", "net", "layer_with_weights-0", "kernel"],
             "mlp/dense_1/bias": mlp + ["fn", "fn", "net", "layer_with_weights-0", "bias"],

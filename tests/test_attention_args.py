@@ -166,3 +166,43 @@ def test_operator_sources_hold_nothing_that_a_graph_cannot_replay():
     for f in ("rel_attention.hip", "qk_norm.hip"):
         text = open(os.path.join(ROOT, "mint_amd", "csrc", f)).read()
         assert "hipMemset" not in text and "hipMalloc" not in text and "Synchronize" not in text
+
+
+def _model_cfg(**at):
+    st = lambda seq, feat: L.FactStackCfg(seq, feat, 800, 2, 10, 3072)
+    cfg = L.FactConfig(st(120, 225), st(240, 35), st(0, 0), 225, 1e-5)
+    return cfg, (L.FactAttnCfg * 3)(L.FactAttnCfg(), L.FactAttnCfg(), L.FactAttnCfg(**at))
+
+
+def test_model_options_add_their_variables(lib):
+    n0, t0, n, t = C.c_size_t(0), C.c_int(0), C.c_size_t(0), C.c_int(0)
+    cfg, none = _model_cfg()
+    assert lib.fact_arena_size(C.byref(cfg), C.byref(n0), C.byref(t0)) == 0
+    assert lib.fact_arena_size_ex(C.byref(cfg), none, C.byref(n), C.byref(t)) == 0 and (n.value, t.value) == (n0.value, t0.value)
+    assert lib.fact_arena_size_ex(C.byref(cfg), None, C.byref(n), C.byref(t)) == 0 and (n.value, t.value) == (n0.value, t0.value)
+    cfg, at = _model_cfg(qk_norm=1, rel_buckets=32, rel_max_distance=128, window=64, sinks=4)
+    assert lib.fact_arena_size_ex(C.byref(cfg), at, C.byref(n), C.byref(t)) == 0 and t.value == t0.value + 2 * 3
+
+
+@pytest.mark.parametrize("at,word", [
+    (dict(qk_norm=2), "qk_norm"), (dict(rotary_dim=16), "qk_norm"), (dict(qk_norm=1, rotary_dim=12), "rotary_dim"),
+    (dict(qk_norm=1, rotary_dim=88), "rotary_dim"), (dict(qk_norm=1, rotary_base=math.nan), "rotary_base"), (dict(window=-1), "window"),
+    (dict(sinks=3), "sinks"), (dict(window=4, sinks=-1), "sinks"), (dict(rel_buckets=300), "buckets"),
+    (dict(rel_buckets=32), "distance"), (dict(rel_buckets=31, rel_max_distance=128), "even"),
+    (dict(rel_buckets=32, rel_max_distance=8), "largest distance"), (dict(rel_buckets=32, rel_max_distance=5000), "distance")])
+def test_model_options_refuse(lib, at, word):
+    cfg, a = _model_cfg(**at)
+    assert lib.fact_arena_size_ex(C.byref(cfg), a, None, None) == -1
+    assert word in lib.fact_last_error().decode()
+    assert lib.fact_create_ex(C.byref(cfg), a, 1, 0, None, C.byref(C.c_void_p())) == -1
+
+
+def test_options_parse_from_a_text_config():
+    from mint_amd import protos
+    m = protos.Merge("""fact_model { cross_modal_model { transformer { hidden_size: 800 qk_norm: true rotary_dim: 80
+        attention_window: 64 attention_sinks: 4 relative_attention_num_buckets: 32 } } }""", protos.MultiModalModel())
+    t = m.fact_model.cross_modal_model.transformer
+    assert t.qk_norm and (t.rotary_dim, t.rotary_base, t.attention_window, t.attention_sinks) == (80, 10000.0, 64, 4)
+    assert (t.relative_attention_num_buckets, t.relative_attention_max_distance) == (32, 128)
+    again = protos.Merge(protos.MessageToString(m), protos.MultiModalModel())
+    assert again == m
