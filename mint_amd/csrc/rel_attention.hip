@@ -16,7 +16,7 @@
 namespace {
 
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr int PAD = 64;  // distances past +-D that a 32 x 32 tile which still touches (-D, D) can reach: 62
+constexpr int PAD = 80;  // distances past +-D that a 32 x 32 tile which still touches (-D, D) can reach (62), and its folds (75)
 typedef __attribute__((address_space(3))) bf16x4 lds_bf16x4;
 
 struct RelP {
@@ -25,6 +25,8 @@ struct RelP {
   float rscale;   // 1 / scale: the bias enters through the accumulator, which is multiplied by scale afterwards
   int qblocks, nwg;
   int splits;
+  int kblocks, sblocks, chunks, schunks;  // dK / dV: 128-key blocks, the first of them with sinks, workgroups of a block
+  float* dkv;     // partial dK, dV of blocks with several workgroups
   float* dsum;    // [B][H][nq] rowsum(dO . O)
   float* part;    // per-workgroup bias gradients [B * H * qblocks][2 D + 1] / partial rows of the few-row kernel
 };
@@ -375,6 +377,54 @@ __global__ __launch_bounds__(256, 2) void rel_fwd_kernel(const RelP p) {
   }
 }
 
+// Sums of a 16 x 16 sub-tile of dS along its diagonals.  Lane (g, c) holds distances base + 4 g + r - c, r = 0 .. 3: moving each
+// partial sum one lane on before the next row is added collects a diagonal in one lane without touching memory:
+//   w (lane c): distance base + 4 g + 3 - c;  the three diagonals that leave the 16 lanes come back in lanes 0 .. 2 of the rotated
+// chain, `up`: distance base - 16 + 4 g + 3 - c.  Key tiles are visited in ascending order, so `up` joins the w of the
+// sub-tile before it and a sub-tile costs one LDS add (12 adds a 32 x 32 tile without the folds: 88 us for dQ at B 16, H 10,
+// n 360, dh 80, of which 45 were the adds).
+template <int CTRL>
+DEVINL float dpp_add(float x, float y) {  // x + y moved by CTRL inside rows of 16 lanes, zeros from outside
+  return x + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, y), CTRL, 0xf, 0xf, true));
+}
+DEVINL void fold_diagonals(f32x4 v, float& w, float& up) {
+  constexpr int SHR1 = 0x111, ROR1 = 0x121;
+  w = dpp_add<SHR1>(v[3], dpp_add<SHR1>(v[2], dpp_add<SHR1>(v[1], v[0])));
+  up = dpp_add<ROR1>(v[3], dpp_add<ROR1>(v[2], dpp_add<ROR1>(v[1], v[0]))) - w;
+}
+struct Diagonals {
+  float* bins;   // this wave's sums by distance, at distance 3 + 4 g - c of a sub-tile's base 0
+  f32x4 next;    // sub-tile at base `at` + 16 that the next key tile adds to
+  float w;       // sub-tile at base `at`, without its `up`
+  int at;
+  bool open;
+  DEVINL void add(int base, float x) { atomicAdd(bins + base, x); }
+  DEVINL void close() {
+    if (!open) return;
+    float w2, up;
+    fold_diagonals(next, w2, up);
+    add(at, w + up);
+    add(at + 16, w2);
+    open = false;
+  }
+  // the sub-tiles at bases d0 - 16, d0, d0 + 16
+  DEVINL void tile(int d0, f32x4 a, f32x4 b, f32x4 c) {
+    float wa, ua, wb, ub;
+    const bool on = open && at + 32 == d0;
+    if (!on) close();
+    if (on) a += next;
+    fold_diagonals(a, wa, ua);
+    fold_diagonals(b, wb, ub);
+    if (on) add(d0 - 32, w + ua);
+    else add(d0 - 32, ua);
+    add(d0 - 16, wa + ub);
+    w = wb;
+    next = c;
+    at = d0;
+    open = true;
+  }
+};
+
 // ---------------------------------------------------------------------------------------------------------------------
 // backward dQ and the bias gradient: workgroup = 128 queries of one head
 //   P = exp2(S c - L);  dP = V dO^T;  dS = P (dP - D), D = rowsum(dO . O);  dQ^T += K^T dS;  dbias[j - p] += dS
@@ -453,6 +503,12 @@ __global__ __launch_bounds__(256, 2) void rel_dq_kernel(const RelP p) {
 #pragma unroll
     for (int dt = 0; dt < ND; ++dt) dQ[qs][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
   float farl = 0.f, farr = 0.f;
+  Diagonals diag;
+  diag.bins = bins + D + PAD + 4 * g + 3 - c;
+  diag.open = false;
+  diag.next = f32x4{0.f, 0.f, 0.f, 0.f};
+  diag.w = 0.f;
+  diag.at = 0;
   if (REL) {
     load_bias(eb, p, h, tid, 256);
     for (int i = lane; i < NB; i += 64) bins[i] = 0.f;
@@ -533,13 +589,7 @@ __global__ __launch_bounds__(256, 2) void rel_dq_kernel(const RelP p) {
         if (left) farl += x;
         else farr += x;
       } else {
-        float* e = bins + d0 + D + PAD + 4 * g - c;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          atomicAdd(e + r - 16, -ds[0][1][r]);
-          atomicAdd(e + r, ds[0][0][r] - ds[1][1][r]);
-          atomicAdd(e + r + 16, ds[1][0][r]);
-        }
+        diag.tile(d0, -ds[0][1], ds[0][0] - ds[1][1], ds[1][0]);
       }
     }
     bf16x8 dsb[2];
@@ -568,6 +618,7 @@ __global__ __launch_bounds__(256, 2) void rel_dq_kernel(const RelP p) {
     }
   }
   if (REL) {
+    diag.close();
     farl = wave_sum(farl);
     farr = wave_sum(farr);
     if (lane == 0) {
@@ -595,41 +646,81 @@ __global__ __launch_bounds__(256, 2) void rel_dq_kernel(const RelP p) {
   }
 }
 
-// drel[bucket][h]: sums over the batch and the query blocks in index order, then over the distances of a bucket
-__global__ __launch_bounds__(1024) void rel_dtable_kernel(const RelP p) {
+// drel[bucket][h], a workgroup each: the distances of the bucket, listed in order, over the batch and the query blocks
+__global__ __launch_bounds__(256) void rel_dtable_kernel(const RelP p) {
   const FactAttention& a = p.a;
-  const int D = a.rel_max_distance, n = 2 * D + 1, h = blockIdx.x, tid = threadIdx.x;
-  __shared__ float val[2049];
-  __shared__ short bk[2049];
-  for (int i = tid; i < n; i += 1024) {
-    float x = 0.f;
-    for (int b = 0; b < a.B; ++b) {
-      const float* src = p.part + ((size_t)b * a.H + h) * p.qblocks * n + i;
-      for (int q = 0; q < p.qblocks; ++q) x += src[(size_t)q * n];
+  const int D = a.rel_max_distance, n = 2 * D + 1, h = blockIdx.x, bu = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  __shared__ short list[2049 + 63];
+  __shared__ int counts[4];
+  __shared__ float red[4];
+  int total = 0;
+  for (int i0 = 0; i0 < n; i0 += 256) {
+    const int i = i0 + tid;
+    const bool in = i < n && min(max(a.rel_map[min(i, n - 1)], 0), a.rel_buckets - 1) == bu;
+    const unsigned long long m = __ballot(in);
+    if (lane == 0) counts[wave] = __popcll(m);
+    __syncthreads();
+    int at = total;
+    for (int w = 0; w < 4; ++w) {
+      if (w < wave) at += counts[w];
+      total += counts[w];
     }
-    val[i] = x;
-    bk[i] = (short)min(max(a.rel_map[i], 0), a.rel_buckets - 1);
+    if (in) list[at + __popcll(m & ((1ull << lane) - 1))] = (short)i;
+    __syncthreads();
   }
-  __syncthreads();
-  // 4 lanes a bucket
-  const int bu = tid >> 2;
-  if (bu < a.rel_buckets) {
-    float x = 0.f;
-    for (int i = tid & 3; i < n; i += 4)
-      if (bk[i] == bu) x += val[i];
-    x += __shfl_xor(x, 1, 64);
-    x += __shfl_xor(x, 2, 64);
-    if ((tid & 3) == 0) {
-      float* o = a.drel + (size_t)bu * a.H + h;
-      *o = a.drel_accumulate ? *o + x : x;
+  // 2^k threads a row of partial sums, k by the length of the list
+  int per = 1;
+  while (per < total && per < 256) per <<= 1;
+  const int rows = a.B * p.qblocks;
+  float x = 0.f;
+  if (total > 0)
+    for (int r = tid / per; r < rows; r += 256 / per) {
+      const int b = r / p.qblocks, q = r - b * p.qblocks;
+      const float* src = p.part + (((size_t)b * a.H + h) * p.qblocks + q) * n;
+      for (int i = tid & (per - 1); i < total; i += per) x += src[list[i]];
     }
+  x = wave_sum(x);
+  if (lane == 0) red[wave] = x;
+  __syncthreads();
+  if (tid == 0) {
+    x = (red[0] + red[1]) + (red[2] + red[3]);
+    float* o = a.drel + (size_t)bu * a.H + h;
+    *o = a.drel_accumulate ? *o + x : x;
   }
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
 // backward dK / dV: workgroup = 128 keys of one key head, 4 waves x 32 keys; the query tiles of every head that reads them
-// are streamed (heads of a group one after another, so their sum has one order)
+// are streamed (heads of a group one after another).  A block's stream is cut into `chunks` workgroups where there are too few
+// blocks to fill the chip or a block holds sinks, which all later queries see: their fp32 sums go through the workspace and
+// rel_join_dkdv_kernel adds them in order.
 // ---------------------------------------------------------------------------------------------------------------------
+struct KBlock {
+  int bh, kb, chunk, chunks;
+  int slot;  // index among the chunks that go through the workspace, -1: the block is written directly
+};
+// grid: per (b, key head) first the blocks with sinks (p.schunks workgroups each), then the others (p.chunks each)
+DEVINL KBlock kblock_of(const RelP& p, int id) {
+  const int per = p.sblocks * p.schunks + (p.kblocks - p.sblocks) * p.chunks;
+  const int through = (p.schunks > 1 ? p.sblocks * p.schunks : 0) + (p.chunks > 1 ? (p.kblocks - p.sblocks) * p.chunks : 0);
+  KBlock k;
+  k.bh = id / per;
+  int r = id - k.bh * per;
+  if (r < p.sblocks * p.schunks) {
+    k.kb = r / p.schunks;
+    k.chunks = p.schunks;
+    k.chunk = r - k.kb * p.schunks;
+    k.slot = p.schunks > 1 ? k.bh * through + r : -1;
+  } else {
+    r -= p.sblocks * p.schunks;
+    k.kb = p.sblocks + r / p.chunks;
+    k.chunks = p.chunks;
+    k.chunk = r % p.chunks;
+    k.slot = p.chunks > 1 ? k.bh * through + (p.schunks > 1 ? p.sblocks * p.schunks : 0) + r : -1;
+  }
+  return k;
+}
+
 template <int DH, bool REL>
 __global__ __launch_bounds__(256, DH > 96 ? 1 : 2) void rel_dkdv_kernel(const RelP p) {
   using G = Geo<DH>;
@@ -641,10 +732,9 @@ __global__ __launch_bounds__(256, DH > 96 ? 1 : 2) void rel_dkdv_kernel(const Re
   float* eb = stat + 128;
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, c = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int kblocks = (a.nk + 127) / 128, group = a.H / a.Hkv;
-  const int id = xcd_order(blockIdx.x, p.nwg);
-  const int bh = id / kblocks, kb = id - bh * kblocks;
-  const int b = bh / a.Hkv, hk = bh - b * a.Hkv;
+  const int group = a.H / a.Hkv;
+  const KBlock blk = kblock_of(p, xcd_order(blockIdx.x, p.nwg));
+  const int kb = blk.kb, b = blk.bh / a.Hkv, hk = blk.bh - b * a.Hkv;
   const Vis v = vis_of(a, b);
   const int start = start_of(a, b);
   const int j0 = kb * 128 + wave * 32;
@@ -655,6 +745,7 @@ __global__ __launch_bounds__(256, DH > 96 ? 1 : 2) void rel_dkdv_kernel(const Re
   long long qe = (v.lo == INT_MIN || ka < v.sinks) ? a.nq - 1 : min((long long)a.nq - 1, ke - v.lo - start);
   if (ka >= v.len) qe = -1;
   const int t0 = (int)(min(qa, 1ll << 30) >> 5), T = qe >= qa ? (int)(qe >> 5) - t0 + 1 : 0, TT = T * group;
+  const int per = (TT + blk.chunks - 1) / blk.chunks, ib = min(TT, blk.chunk * per), ie = min(TT, ib + per);
 
   Frag<DH> K[2], V[2];
 #pragma unroll
@@ -685,21 +776,21 @@ __global__ __launch_bounds__(256, DH > 96 ? 1 : 2) void rel_dkdv_kernel(const Re
     st.store(smem + buf * 2 * G::IMG);
     if (tid < 64) stat[buf * 64 + tid] = sv;
   };
-  if (TT > 0) {
-    load(0);
-    store(0);
-    if (TT > 1) load(1);
+  if (ib < ie) {
+    load(ib);
+    store(ib & 1);
+    if (ib + 1 < ie) load(ib + 1);
   }
-  for (int i = 0; i < TT; ++i) {
+  for (int i = ib; i < ie; ++i) {
     const int hh = i / T, qt = i - hh * T;
-    if (REL && qt == 0) {  // the next head's bias: after the last tile of the head before has been read
+    if (REL && (qt == 0 || i == ib)) {  // the next head's bias: after the last tile of the head before has been read
       __syncthreads();
       load_bias(eb, p, hk * group + hh, tid, 256);
     }
     __syncthreads();
-    if (i + 1 < TT) {
+    if (i + 1 < ie) {
       store((i + 1) & 1);
-      if (i + 2 < TT) load(i + 2);
+      if (i + 2 < ie) load(i + 2);
     }
     const int q0 = (t0 + qt) * 32, p0 = start + q0;
     if (!active || v.none(j0, p0)) continue;
@@ -788,6 +879,17 @@ __global__ __launch_bounds__(256, DH > 96 ? 1 : 2) void rel_dkdv_kernel(const Re
       }
     }
   }
+  if (blk.slot >= 0) {
+    f32x4* out = reinterpret_cast<f32x4*>(p.dkv) + ((size_t)blk.slot * 4 + wave) * (4 * ND * 64) + lane;
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+      for (int dt = 0; dt < ND; ++dt) {
+        out[(ks * ND + dt) * 128] = dK[ks][dt];
+        out[(ks * ND + dt) * 128 + 64] = dV[ks][dt];
+      }
+    return;
+  }
 #pragma unroll
   for (int ks = 0; ks < 2; ++ks) {
     const int j = j0 + ks * 16 + c;
@@ -806,6 +908,33 @@ __global__ __launch_bounds__(256, DH > 96 ? 1 : 2) void rel_dkdv_kernel(const Re
       *reinterpret_cast<bf16x4*>(vr + dt * 16) = y;
     }
   }
+}
+
+// the chunks of a block, in order: a wave per accumulator fragment (wave, ks, dt, K or V) of the kernel above
+template <int DH>
+__global__ __launch_bounds__(256) void rel_join_dkdv_kernel(const RelP p) {
+  constexpr int ND = Geo<DH>::ND, FR = 4 * 4 * ND;  // fragments of a block
+  const FactAttention& a = p.a;
+  const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+  const int f = (blockIdx.x * 4 + (threadIdx.x >> 6)) % FR, blk = (blockIdx.x * 4 + (threadIdx.x >> 6)) / FR;
+  const int sj = p.schunks > 1 ? p.sblocks : 0, oj = p.chunks > 1 ? p.kblocks - p.sblocks : 0;
+  if (blk >= a.B * a.Hkv * (sj + oj)) return;
+  const int bh = blk / (sj + oj), r = blk - bh * (sj + oj), b = bh / a.Hkv, hk = bh - b * a.Hkv;
+  const bool sink = r < sj;
+  const int kb = sink ? r : p.sblocks + r - sj, n = sink ? p.schunks : p.chunks;
+  const int slot = bh * (sj * p.schunks + oj * p.chunks) + (sink ? r * p.schunks : sj * p.schunks + (r - sj) * p.chunks);
+  const f32x4* src = reinterpret_cast<const f32x4*>(p.dkv) + ((size_t)slot * FR + f) * 64 + lane;
+  f32x4 x = src[0];
+  for (int i = 1; i < n; ++i) x += src[(size_t)i * FR * 64];
+  const int wave = f / (4 * ND), ks = f / (2 * ND) & 1, dt = (f >> 1) % ND, isv = f & 1;
+  const int j = kb * 128 + wave * 32 + ks * 16 + c;
+  if (j >= a.nk) return;
+  const int64_t* st = isv ? a.dv_stride : a.dk_stride;
+  const float k = isv ? 1.f : a.scale;
+  bf16x4 o;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o[i] = (bf16_t)(x[i] * k);
+  *reinterpret_cast<bf16x4*>((bf16_t*)(isv ? a.dv : a.dk) + b * st[0] + (long long)j * st[1] + hk * st[2] + dt * 16 + g * 4) = o;
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -1035,7 +1164,30 @@ RelP params(const FactAttention& a) {
   p.splits = 1;
   p.dsum = nullptr;
   p.part = nullptr;
+  p.dkv = nullptr;
+  // dK / dV: streams of the blocks as long as lengths and positions allow (they are on the device), cut so that the grid fills
+  // 256 CUs twice but no piece is shorter than 4 tiles
+  const long long group = a.H / a.Hkv, all = ((long long)a.nq + 31) / 32 * group;
+  p.kblocks = (a.nk + 127) / 128;
+  p.sblocks = a.window_left < 0 ? 0 : (std::min(a.sinks, a.nk) + 127) / 128;
+  long long seen = a.nq;
+  if (a.window_left >= 0 && a.window_right >= 0)
+    seen = std::min<long long>(seen, 128ll + a.window_left + a.window_right + 62);
+  const long long t = (seen + 31) / 32 * group, blocks = (long long)a.B * a.Hkv * p.kblocks;
+  p.chunks = (int)std::max(1ll, std::min((512 + blocks / 2) / blocks, t / 4));
+  const long long piece = std::max(8ll, (t + p.chunks - 1) / p.chunks);
+  p.schunks = (int)std::max<long long>(p.chunks, std::min(all / piece, 64ll));
   return p;
+}
+// chunks of one (batch, key head) that go through the workspace
+size_t dkv_chunks(const RelP& p) {
+  return (p.schunks > 1 ? (size_t)p.sblocks * p.schunks : 0) + (p.chunks > 1 ? (size_t)(p.kblocks - p.sblocks) * p.chunks : 0);
+}
+size_t dkv_bytes(const RelP& p) { return dkv_chunks(p) * p.a.B * p.a.Hkv * 128 * 2 * p.a.dh * 4; }
+
+// the dQ kernel's partial bias gradients
+size_t part_bytes(const FactAttention& a) {
+  return a.rel_table ? up16((size_t)a.B * a.H * ((a.nq + 127) / 128) * (2 * a.rel_max_distance + 1) * 4) : 0;
 }
 
 template <int DH, bool REL>
@@ -1064,14 +1216,17 @@ int bwd_t(const FactAttention& a, void* ws, hipStream_t s) {
   const size_t nb = REL ? 2 * (a.rel_max_distance + PAD) + 1 : 0;
   p.dsum = (float*)ws;
   p.part = (float*)((char*)ws + up16((size_t)a.B * a.H * a.nq * 4));
+  p.dkv = (float*)((char*)p.part + part_bytes(a));
   p.nwg = p.qblocks * a.B * a.H;
   const size_t lds1 = 4 * Geo<DH>::IMG * 2 + 5 * nb * 4, lds2 = 4 * Geo<DH>::IMG * 2 + 512 + nb * 4;
   if (int rc = allow_lds(rel_dq_kernel<DH, REL>, lds1)) return rc;
   if (int rc = allow_lds(rel_dkdv_kernel<DH, REL>, lds2)) return rc;
   FACT_LAUNCH((rel_dq_kernel<DH, REL>), dim3(p.nwg), dim3(256), lds1, s, p);
-  if (REL) FACT_LAUNCH(rel_dtable_kernel, dim3(a.H), dim3(1024), 0, s, p);
-  p.nwg = (a.nk + 127) / 128 * a.B * a.Hkv;
+  if (REL) FACT_LAUNCH(rel_dtable_kernel, dim3(a.H, a.rel_buckets), dim3(256), 0, s, p);
+  p.nwg = (p.sblocks * p.schunks + (p.kblocks - p.sblocks) * p.chunks) * a.B * a.Hkv;
   FACT_LAUNCH((rel_dkdv_kernel<DH, REL>), dim3(p.nwg), dim3(256), lds2, s, p);
+  const int joined = ((p.schunks > 1 ? p.sblocks : 0) + (p.chunks > 1 ? p.kblocks - p.sblocks : 0)) * a.B * a.Hkv;
+  if (joined) FACT_LAUNCH(rel_join_dkdv_kernel<DH>, dim3(joined * 4 * Geo<DH>::ND), dim3(256), 0, s, p);
   return launched();
 }
 
@@ -1102,7 +1257,7 @@ int rel_attention_check(const FactAttention& a, bool backward, const char** why)
   if (a.dh != 32 && a.dh != 64 && a.dh != 80 && a.dh != 96 && a.dh != 128)
     return bad(-3, "unsupported head dim (supported: 32, 64, 80, 96, 128)");
   if ((long long)a.B * a.H > INT_MAX / 256 || ((long long)a.nq + 127) / 128 * a.B * a.H > INT_MAX / 4 ||
-      ((long long)a.nk + 127) / 128 * a.B * a.Hkv > INT_MAX / 4)
+      ((long long)a.nk + 127) / 128 * a.B * a.Hkv > INT_MAX / 512)
     return bad(-1, "too many heads and blocks for one launch");
   if (!(a.scale >= 5.9604645e-8f) || !(a.scale <= 3.0e38f)) return bad(-1, "scale must be finite and at least 2^-24");
   if (a.sinks < 0) return bad(-1, "sinks must not be negative");
@@ -1130,11 +1285,7 @@ int rel_attention_check(const FactAttention& a, bool backward, const char** why)
 }
 
 size_t rel_attention_ws(const FactAttention& a, bool backward) {
-  if (backward) {
-    size_t n = up16((size_t)a.B * a.H * a.nq * 4);
-    if (a.rel_table) n += (size_t)a.B * a.H * ((a.nq + 127) / 128) * (2 * a.rel_max_distance + 1) * 4;
-    return up16(n);
-  }
+  if (backward) return up16((size_t)a.B * a.H * a.nq * 4) + part_bytes(a) + dkv_bytes(params(a));
   if (!few_rows(a)) return 0;
   const int s = row_splits(a);
   return s > 1 ? up16((size_t)s * a.B * a.H * a.nq * (a.dh + 4) * 4) : 0;
