@@ -84,31 +84,54 @@ def _p(t):
 
 def _set(a, name, t):
     setattr(a, name, t.data_ptr())
-    s = t.stride()
-    getattr(a, name + "_stride")[:] = (s[0], s[1], s[2])
+    getattr(a, name + "_stride")[:] = t.stride()[:3]
 
 
-class _On:
-    """The device of a call's tensors made current, if it is not."""
-
-    def __init__(self, device):
-        self.device = device
-
-    def __enter__(self):
-        self.before = torch.cuda.current_device()
-        if self.before != self.device.index:
-            torch.cuda.set_device(self.device)
-        return C.c_void_p(torch.cuda.current_stream(self.device).cuda_stream)
-
-    def __exit__(self, *exc):
-        if self.before != self.device.index:
-            torch.cuda.set_device(self.before)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
 
 
-def _workspace(fn, a, backward, device):
+def _launch(fn, a, ws_bytes, device):
+    """fn(args, workspace, bytes, stream) on the device's current stream, with scratch memory of this call's own."""
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=device) if ws_bytes else None
+    index, before = device.index, torch.cuda.current_device()
+    if before != index:
+        torch.cuda.set_device(index)
+    try:
+        rc = fn(C.byref(a), ws.data_ptr() if ws_bytes else None, ws_bytes, _raw_stream(index))
+    finally:
+        if before != index:
+            torch.cuda.set_device(before)
+    if rc:
+        L.check(rc)
+
+
+def _ws_bytes(name, a, backward):
     n = C.c_size_t(0)
-    L.check(fn(C.byref(a), backward, C.byref(n)))
-    return (torch.empty(n.value, dtype=torch.uint8, device=device) if n.value else None), n.value
+    L.check(getattr(L.lib(), name)(C.byref(a), backward, C.byref(n)))
+    return n.value
+
+
+# Calls of one geometry (shapes, strides, types, devices, options) share their checks: the first one leaves its filled-in argument
+# struct and workspace size, the next ones copy it and set the pointers.  Nothing of the tensors themselves is kept.  (A call
+# costs the host 9 instead of 18 us; one new token of 32 sequences takes the GPU 4.)
+_PLANS = {}
+_MOST_PLANS = 512
+_Plan = collections.namedtuple("_Plan", ["args", "fn", "ws", "extra"])
+
+
+def _keep(key, args, fn, ws, extra=None):
+    if key is not None:
+        if len(_PLANS) >= _MOST_PLANS:
+            _PLANS.clear()
+        _PLANS[key] = _Plan(bytes(args), fn, ws, extra)
+
+
+def _key(op, tensors, options):
+    """None where an argument is no tensor: the checks say so."""
+    try:
+        return (op,) + tuple([None if t is None else (t.shape, t.stride(), t.dtype, t.device) for t in tensors]) + options
+    except AttributeError:
+        return None
 
 
 # ---- attention ------------------------------------------------------------------------------------------------------
@@ -121,7 +144,6 @@ def _attention_args(q, k, v, scale, window, sinks, rel_table, rel_map, kv_len, q
           B, dh, tuple(k.shape), tuple(v.shape))
     nk, Hkv = k.shape[1], k.shape[2]
     _need(Hkv > 0 and H % Hkv == 0, "the %d query heads must be a multiple of the %d key heads", H, Hkv)
-    window = (-1, -1) if window is None else window
     _need(len(window) == 2, "window must be (left, right)")
     a = L.FactAttention(B=B, H=H, Hkv=Hkv, nq=nq, nk=nk, dh=dh, window_left=int(window[0]), window_right=int(window[1]),
                         sinks=int(sinks), scale=float(dh ** -0.5 if scale is None else scale))
@@ -133,15 +155,35 @@ def _attention_args(q, k, v, scale, window, sinks, rel_table, rel_map, kv_len, q
               "rel_map must hold the bucket of 2 * max_distance + 1 distances")
         rel_table = _vector(rel_table, "rel_table", rel_table.shape, torch.float32, dev)
         rel_map = _vector(rel_map, "rel_map", rel_map.shape, torch.int32, dev)
-        a.rel_table, a.rel_map = rel_table.data_ptr(), rel_map.data_ptr()
         a.rel_buckets, a.rel_max_distance = rel_table.shape[0], rel_map.numel() // 2
     kv_len = _vector(kv_len, "kv_len", (B,), torch.int32, dev)
     q_start = _vector(q_start, "q_start", (B,), torch.int32, dev)
-    a.kv_len, a.q_start = _p(kv_len), _p(q_start)
-    _set(a, "q", q)
-    _set(a, "k", k)
-    _set(a, "v", v)
-    return a, (q, k, v, rel_table, rel_map, kv_len, q_start)  # (the copies live until the launch is enqueued)
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        _set(a, name, t)
+    held = (q, k, v, rel_table, rel_map, kv_len, q_start)
+    _inputs(a, held)
+    return a, held  # (the copies live until the launch is enqueued)
+
+
+def _inputs(a, held):
+    """Pointers of the forward's inputs; their alignment bits."""
+    q, k, v, rel_table, rel_map, kv_len, q_start = held
+    a.q, a.k, a.v = x, y, z = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    bits = x | y | z
+    if rel_table is not None:
+        a.rel_table, a.rel_map = x, y = rel_table.data_ptr(), rel_map.data_ptr()
+        bits |= x | y
+    if kv_len is not None:
+        a.kv_len = x = kv_len.data_ptr()
+        bits |= x
+    if q_start is not None:
+        a.q_start = x = q_start.data_ptr()
+        bits |= x
+    return bits
+
+
+def _options(scale, window, sinks):
+    return (None if scale is None else float(scale), (-1, -1) if window is None else tuple(window), int(sinks))
 
 
 def attention(q, k, v, scale=None, window=None, sinks=0, rel_table=None, rel_map=None, kv_len=None, q_start=None,
@@ -152,11 +194,27 @@ def attention(q, k, v, scale=None, window=None, sinks=0, rel_table=None, rel_map
     j <= position + window[1] and (j >= position - window[0] or j < sinks); a negative window side is open.  rel_table
     [buckets, H] fp32 adds rel_table[rel_map[clip(j - position)]][h] to scale * q . k.  A row that sees no key gives zeros.
     Keys and values at and after kv_len are never read.  Returns out [B, nq, H, dh], with `training` (out, AttentionSaved)."""
-    a, held = _attention_args(q, k, v, scale, window, sinks, rel_table, rel_map, kv_len, q_start)
-    dev = held[0].device
+    options = _options(scale, window, sinks)
+    held = (q, k, v, rel_table, rel_map, kv_len, q_start)
+    key = _key("attention", held + (out,), options + (bool(training),))
+    plan = _PLANS.get(key)
+    if plan is not None:
+        a = L.FactAttention.from_buffer_copy(plan.args)
+        if out is None:
+            out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
+        a.out = x = out.data_ptr()
+        if not (_inputs(a, held) | x) & 15:
+            dev, saved = q.device, None
+            if training:
+                lse = torch.empty(plan.extra[0], dtype=torch.float32, device=dev)
+                lo = torch.empty(q.shape, dtype=torch.float32, device=dev) if plan.extra[1] else None
+                a.lse, a.out_lo, saved = lse.data_ptr(), _p(lo), AttentionSaved(lse, lo)
+            _launch(plan.fn, a, plan.ws, dev)
+            return (out, saved) if training else out
+    a, given = _attention_args(*held[:3], *options, *held[3:])
+    dev = given[0].device
     shape = (a.B, a.nq, a.H, a.dh)
     out = _dest(out, "out", shape, torch.bfloat16, dev)
-    saved = None
     if 0 in shape:
         return (out, AttentionSaved(out.new_empty((a.B, a.H, a.nq), dtype=torch.float32), None)) if training else out
     if a.nk == 0:
@@ -164,15 +222,17 @@ def attention(q, k, v, scale=None, window=None, sinks=0, rel_table=None, rel_map
         lse = torch.full((a.B, a.H, a.nq), float("inf"), device=dev) if training else None
         return (out, AttentionSaved(lse, None)) if training else out
     _set(a, "out", out)
+    saved = None
     if training:
         lse = torch.empty((a.B, a.H, a.nq), dtype=torch.float32, device=dev)
         exact = rel_table is not None or a.nk <= EXACT_KEYS
         lo = torch.empty(shape, dtype=torch.float32, device=dev) if exact else None
         saved = AttentionSaved(lse, lo)
         a.lse, a.out_lo = lse.data_ptr(), _p(lo)
-    with _On(dev) as stream:
-        ws, n = _workspace(L.lib().fact_attention_workspace, a, 0, dev)
-        L.check(L.lib().fact_attention(C.byref(a), _p(ws), n, stream))
+    ws, fn = _ws_bytes("fact_attention_workspace", a, 0), L.lib().fact_attention
+    _launch(fn, a, ws, dev)
+    if all(x is y for x, y in zip(held, given)):
+        _keep(key, a, fn, ws, (saved.lse.shape, saved.out_lo is not None) if training else None)
     return (out, saved) if training else out
 
 
@@ -181,12 +241,40 @@ def attention_backward(dout, q, k, v, out, saved, scale=None, window=None, sinks
     """Gradients of attention(..., training=True) for dout [B, nq, H, dh]: (dq, dk, dv), with a relative bias also the fp32
     gradient of rel_table.  `out` and `saved` are what the forward returned; dq, dk, dv may be given (views of one packed
     gradient, for instance)."""
-    a, held = _attention_args(q, k, v, scale, window, sinks, rel_table, rel_map, kv_len, q_start)
-    dev = held[0].device
+    _need(isinstance(saved, AttentionSaved), "saved must be what attention(training=True) returned")
+    options = _options(scale, window, sinks)
+    held = (q, k, v, rel_table, rel_map, kv_len, q_start)
+    lse, lo = saved
+    key = _key("backward", held + (dout, out, lse, lo, dq, dk, dv), options)
+    plan = _PLANS.get(key)
+    if plan is not None:
+        dev = q.device
+        a = L.FactAttention.from_buffer_copy(plan.args)
+        dq = torch.empty(q.shape, dtype=torch.bfloat16, device=dev) if dq is None else dq
+        dk = torch.empty(k.shape, dtype=torch.bfloat16, device=dev) if dk is None else dk
+        dv = torch.empty(k.shape, dtype=torch.bfloat16, device=dev) if dv is None else dv
+        bits = _inputs(a, held)
+        for name, t in (("dout", dout), ("out", out), ("lse", lse), ("dq", dq), ("dk", dk), ("dv", dv)):
+            x = t.data_ptr()
+            setattr(a, name, x)
+            bits |= x
+        if lo is not None:
+            a.out_lo = x = lo.data_ptr()
+            bits |= x
+        if not bits & 15:
+            if rel_table is None:
+                _launch(plan.fn, a, plan.ws, dev)
+                return dq, dk, dv
+            drel = torch.empty(rel_table.shape, dtype=torch.float32, device=dev)
+            a.drel = drel.data_ptr()
+            _launch(plan.fn, a, plan.ws, dev)
+            return dq, dk, dv, drel
+    a, given = _attention_args(*held[:3], *options, *held[3:])
+    dev = given[0].device
     shape = torch.Size((a.B, a.nq, a.H, a.dh))
+    more = (dout, out, lse, lo)
     dout, out = _heads(dout, "dout", torch.bfloat16, dev), _heads(out, "out", torch.bfloat16, dev)
     _need(dout.shape == shape and out.shape == shape, "dout and out must be %s", tuple(shape))
-    _need(isinstance(saved, AttentionSaved), "saved must be what attention(training=True) returned")
     dq = _dest(dq, "dq", q.shape, torch.bfloat16, dev)
     dk = _dest(dk, "dk", k.shape, torch.bfloat16, dev)
     dv = _dest(dv, "dv", v.shape, torch.bfloat16, dev)
@@ -198,19 +286,20 @@ def attention_backward(dout, q, k, v, out, saved, scale=None, window=None, sinks
             if t is not None:
                 t.zero_()
         return (dq, dk, dv) if drel is None else (dq, dk, dv, drel)
-    lse = _vector(saved.lse, "saved.lse", (a.B, a.H, a.nq), torch.float32, dev)
-    lo = _vector(saved.out_lo, "saved.out_lo", shape, torch.float32, dev)
+    lse = _vector(lse, "saved.lse", (a.B, a.H, a.nq), torch.float32, dev)
+    lo = _vector(lo, "saved.out_lo", shape, torch.float32, dev)
     for name, t in (("out", out), ("dout", dout), ("dq", dq), ("dk", dk), ("dv", dv)):
         _set(a, name, t)
     a.lse, a.out_lo, a.drel = lse.data_ptr(), _p(lo), _p(drel)
-    with _On(dev) as stream:
-        ws, n = _workspace(L.lib().fact_attention_workspace, a, 1, dev)
-        L.check(L.lib().fact_attention_backward(C.byref(a), _p(ws), n, stream))
+    ws, fn = _ws_bytes("fact_attention_workspace", a, 1), L.lib().fact_attention_backward
+    _launch(fn, a, ws, dev)
+    if all(x is y for x, y in zip(held + more, given + (dout, out, lse, lo))):
+        _keep(key, a, fn, ws)
     return (dq, dk, dv) if drel is None else (dq, dk, dv, drel)
 
 
 # ---- norm of queries and keys with rotation ---------------------------------------------------------------------------
-def _norm_args(q, k, q_gamma, k_gamma, eps, rotary_dim, base, interleaved, positions, position0):
+def _norm_args(q, k, q_gamma, k_gamma, positions, eps, rotary_dim, base, interleaved, position0):
     q = _heads(q, "q", None)
     _need(q.dtype in DTYPES, "q must be bfloat16 or float32, not %s", q.dtype)
     dev = q.device
@@ -220,19 +309,37 @@ def _norm_args(q, k, q_gamma, k_gamma, eps, rotary_dim, base, interleaved, posit
           tuple(k.shape))
     q_gamma = _vector(q_gamma, "q_gamma", (dh,), torch.float32, dev)
     k_gamma = _vector(k_gamma, "k_gamma", (dh,), torch.float32, dev)
-    a = L.FactQkNorm(B=B, n=n, H=H, Hkv=k.shape[2], dh=dh, rotary_dim=dh if rotary_dim is None else int(rotary_dim),
-                     interleaved=1 if interleaved else 0, dtype=DTYPES[q.dtype], position0=int(position0), eps=float(eps),
-                     base=float(base), q_gamma=_p(q_gamma), k_gamma=_p(k_gamma))
+    a = L.FactQkNorm(B=B, n=n, H=H, Hkv=k.shape[2], dh=dh, rotary_dim=dh if rotary_dim is None else rotary_dim,
+                     interleaved=1 if interleaved else 0, dtype=DTYPES[q.dtype], position0=position0, eps=eps, base=base)
     if positions is not None:
         _need(torch.is_tensor(positions) and positions.dtype == torch.int32 and positions.device == dev
               and tuple(positions.shape) in ((B, n), (n,)), "positions must be an int32 tensor of shape %s or %s on %s",
               (B, n), (n,), dev)
-        positions = positions.expand(B, n)
+        a.position_stride[:] = positions.expand(B, n).stride()
+    for name, t in (("q", q), ("k", k)):
+        _set(a, name, t)
+    held = (q, k, q_gamma, k_gamma, positions)
+    _norm_inputs(a, held)
+    return a, held
+
+
+def _norm_inputs(a, held):
+    q, k, q_gamma, k_gamma, positions = held
+    a.q, a.k = x, y = q.data_ptr(), k.data_ptr()
+    bits = x | y
+    if q_gamma is not None:
+        a.q_gamma = x = q_gamma.data_ptr()
+        bits |= x
+    if k_gamma is not None:
+        a.k_gamma = x = k_gamma.data_ptr()
+        bits |= x
+    if positions is not None:
         a.positions = positions.data_ptr()
-        a.position_stride[:] = positions.stride()
-    _set(a, "q", q)
-    _set(a, "k", k)
-    return a, (q, k, q_gamma, k_gamma, positions)
+    return bits
+
+
+def _norm_options(eps, rotary_dim, base, interleaved, position0):
+    return float(eps), None if rotary_dim is None else int(rotary_dim), float(base), bool(interleaved), int(position0)
 
 
 def qk_norm_rope(q, k, q_gamma=None, k_gamma=None, eps=1e-6, rotary_dim=None, base=10000.0, interleaved=False, positions=None,
@@ -241,16 +348,31 @@ def qk_norm_rope(q, k, q_gamma=None, k_gamma=None, eps=1e-6, rotary_dim=None, ba
     None: 1), then the first rotary_dim values (None: all, 0: none) of each head turned in pairs by
     position * base^(-2 i / rotary_dim).  Pair i is (i, i + rotary_dim / 2), `interleaved` (2 i, 2 i + 1).  positions: int32
     [B, n] or [n]; without it position0 + token.  Returns (q, k); q_out / k_out may be q / k themselves."""
-    a, held = _norm_args(q, k, q_gamma, k_gamma, eps, rotary_dim, base, interleaved, positions, position0)
-    dev = held[0].device
+    options = _norm_options(eps, rotary_dim, base, interleaved, position0)
+    held = (q, k, q_gamma, k_gamma, positions)
+    key = _key("norm", held + (q_out, k_out), options)
+    plan = _PLANS.get(key)
+    if plan is not None:
+        dev = q.device
+        a = L.FactQkNorm.from_buffer_copy(plan.args)
+        q_out = torch.empty(q.shape, dtype=q.dtype, device=dev) if q_out is None else q_out
+        k_out = torch.empty(k.shape, dtype=q.dtype, device=dev) if k_out is None else k_out
+        a.q_out, a.k_out = x, y = q_out.data_ptr(), k_out.data_ptr()
+        if not (_norm_inputs(a, held) | x | y) & 15:
+            _launch(plan.fn, a, 0, dev)
+            return q_out, k_out
+    a, given = _norm_args(*held, *options)
+    dev = given[0].device
     q_out = _dest(q_out, "q_out", q.shape, q.dtype, dev)
     k_out = _dest(k_out, "k_out", k.shape, q.dtype, dev)
     if a.B == 0 or a.n == 0:
         return q_out, k_out
     _set(a, "q_out", q_out)
     _set(a, "k_out", k_out)
-    with _On(dev) as stream:
-        L.check(L.lib().fact_qk_norm(C.byref(a), None, 0, stream))
+    fn = L.lib().fact_qk_norm
+    _launch(fn, a, 0, dev)
+    if all(x is y for x, y in zip(held, given)):
+        _keep(key, a, fn, 0)
     return q_out, k_out
 
 
@@ -258,19 +380,41 @@ def qk_norm_rope_backward(dq_out, dk_out, q, k, q_gamma=None, k_gamma=None, eps=
                           interleaved=False, positions=None, position0=0, dq=None, dk=None):
     """Gradients of qk_norm_rope for (dq_out, dk_out), from the forward's INPUTS q, k: (dq, dk, dq_gamma, dk_gamma), the last two
     fp32 [dh].  dq / dk may be dq_out / dk_out themselves."""
-    a, held = _norm_args(q, k, q_gamma, k_gamma, eps, rotary_dim, base, interleaved, positions, position0)
-    dev = held[0].device
-    dq_in, dk_in = _heads(dq_out, "dq_out", q.dtype, dev), _heads(dk_out, "dk_out", q.dtype, dev)
-    _need(dq_in.shape == q.shape and dk_in.shape == k.shape, "dq_out and dk_out must have the shapes of q and k")
+    options = _norm_options(eps, rotary_dim, base, interleaved, position0)
+    held = (q, k, q_gamma, k_gamma, positions)
+    key = _key("norm backward", held + (dq_out, dk_out, dq, dk), options)
+    plan = _PLANS.get(key)
+    if plan is not None:
+        dev = q.device
+        a = L.FactQkNorm.from_buffer_copy(plan.args)
+        dq = torch.empty(q.shape, dtype=q.dtype, device=dev) if dq is None else dq
+        dk = torch.empty(k.shape, dtype=q.dtype, device=dev) if dk is None else dk
+        bits = _norm_inputs(a, held)
+        for name, t in (("dq_out", dq_out), ("dk_out", dk_out), ("dq", dq), ("dk", dk)):
+            x = t.data_ptr()
+            setattr(a, name, x)
+            bits |= x
+        if not bits & 15:
+            gains = torch.empty((2, a.dh), dtype=torch.float32, device=dev)
+            x = gains.data_ptr()
+            a.dq_gamma, a.dk_gamma = x, x + 4 * a.dh
+            _launch(plan.fn, a, plan.ws, dev)
+            return dq, dk, gains[0], gains[1]
+    a, given = _norm_args(*held, *options)
+    dev = given[0].device
+    more = (dq_out, dk_out)
+    dq_out, dk_out = _heads(dq_out, "dq_out", q.dtype, dev), _heads(dk_out, "dk_out", q.dtype, dev)
+    _need(dq_out.shape == q.shape and dk_out.shape == k.shape, "dq_out and dk_out must have the shapes of q and k")
     dq, dk = _dest(dq, "dq", q.shape, q.dtype, dev), _dest(dk, "dk", k.shape, q.dtype, dev)
     gains = torch.empty((2, a.dh), dtype=torch.float32, device=dev)
     if a.B == 0 or a.n == 0:
         gains.zero_()
         return dq, dk, gains[0], gains[1]
-    for name, t in (("dq_out", dq_in), ("dk_out", dk_in), ("dq", dq), ("dk", dk)):
+    for name, t in (("dq_out", dq_out), ("dk_out", dk_out), ("dq", dq), ("dk", dk)):
         _set(a, name, t)
     a.dq_gamma, a.dk_gamma = gains.data_ptr(), gains.data_ptr() + 4 * a.dh
-    with _On(dev) as stream:
-        ws, n = _workspace(L.lib().fact_qk_norm_workspace, a, 1, dev)
-        L.check(L.lib().fact_qk_norm_backward(C.byref(a), _p(ws), n, stream))
+    ws, fn = _ws_bytes("fact_qk_norm_workspace", a, 1), L.lib().fact_qk_norm_backward
+    _launch(fn, a, ws, dev)
+    if all(x is y for x, y in zip(held + more, given + (dq_out, dk_out))):
+        _keep(key, a, fn, ws)
     return dq, dk, gains[0], gains[1]

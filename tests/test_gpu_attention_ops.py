@@ -543,3 +543,30 @@ def test_norm_attention_run_as_a_block():
     for got, want, name in ((o, y, "out"), (dq, ref[0], "dq"), (dk, ref[1], "dk"), (dv, ref[2], "dv"), (dgq, ref[3], "dgq"),
                             (dgk, ref[4], "dgk"), (dt, ref[5], "dtable")):
         assert float((got.double() - want).norm() / want.norm()) <= tol, name
+
+
+def test_a_second_call_of_a_geometry_checks_and_computes_like_the_first():
+    """Calls of one geometry share their checks; alignment, copies and types are still looked at, and results follow the tensors."""
+    gen = torch.Generator().manual_seed(40)
+    B, n, H, dh = 2, 40, 2, 64
+    t, m = _table(gen, H)
+    for rep in range(3):
+        q, k, v, do = (_rand(gen, B, n, H, dh) for _ in range(4))
+        kw = dict(rel_table=t, rel_map=m, window=[9, 9], sinks=rep)
+        _check(q, k, v, 0.2, seed=rep, **kw)
+        want = A.attention(q, k, v, **kw)
+        odd = torch.empty(q.numel() + 4, dtype=torch.bfloat16, device=DEV)[4:].view(q.shape).copy_(q)
+        assert odd.data_ptr() % 16 == 8 and odd.stride() == q.stride()
+        assert torch.equal(A.attention(odd, k, v, **kw), want)
+        dst = torch.zeros_like(q)
+        assert A.attention(q, k, v, out=dst, **kw) is dst and torch.equal(dst, want)
+        with pytest.raises(ValueError):
+            A.attention(q, k, v, out=odd, **kw)
+        with pytest.raises(ValueError):
+            A.attention(q, k.float(), v, **kw)
+        a, b = A.qk_norm_rope(q, k, position0=rep)
+        c, d = A.qk_norm_rope(odd, k, position0=rep)
+        assert torch.equal(a, c) and torch.equal(b, d)
+        g = A.qk_norm_rope_backward(do, do, q, k, position0=rep)
+        h = A.qk_norm_rope_backward(do, do, odd, k, position0=rep)
+        assert all(torch.equal(x, y) for x, y in zip(g, h))
