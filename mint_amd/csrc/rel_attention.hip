@@ -25,6 +25,7 @@ struct RelP {
   float rscale;   // 1 / scale: the bias enters through the accumulator, which is multiplied by scale afterwards
   int qblocks, nwg;
   int splits;
+  int rowtab;     // few rows: the bias of the group's heads fits the workgroup's memory
   int kblocks, sblocks, chunks, schunks;  // dK / dV: 128-key blocks, the first of them with sinks, workgroups of a block
   float* dkv;     // partial dK, dV of blocks with several workgroups
   float* dsum;    // [B][H][nq] rowsum(dO . O)
@@ -127,12 +128,14 @@ struct Vis {
     const long long low = lo == INT_MIN ? 0 : max(0ll, (long long)p + lo), sk = min((long long)sinks, top);
     return max(0ll, top - max(low, sk)) + max(0ll, sk) == 1;
   }
-  // a 32-key tile at j0 against positions p0 .. p0 + 31
+  // keys j0 .. j0 + W - 1 against positions p0 .. p0 + 31
+  template <int W = 32>
   DEVINL bool none(int j0, int p0) const {
-    return j0 >= len || j0 - (p0 + 31) > hi || (j0 + 31 - p0 < lo && j0 >= sinks);
+    return j0 >= len || j0 - (p0 + 31) > hi || (j0 + W - 1 - p0 < lo && j0 >= sinks);
   }
+  template <int W = 32>
   DEVINL bool full(int j0, int p0) const {
-    return j0 + 31 < len && j0 + 31 - p0 <= hi && (j0 - (p0 + 31) >= lo || j0 + 31 < sinks);
+    return j0 + W - 1 < len && j0 + W - 1 - p0 <= hi && (j0 - (p0 + 31) >= lo || j0 + W - 1 < sinks);
   }
 };
 // Lengths are below 2^30 (checked) and first positions clamped to +-(2^30 - 64), so no key - position overflows.
@@ -174,9 +177,9 @@ DEVINL int xcd_order(int id, int n) {
 }
 
 // ---- staging of two 32-row tiles (K and V, or Q and dO) through registers into LDS -------------------------------------
-template <int DH>
+template <int DH, int NT = 256>
 struct Stage {
-  static constexpr int N = (2 * 32 * Geo<DH>::CH + 255) / 256;
+  static constexpr int N = (2 * 32 * Geo<DH>::CH + NT - 1) / NT;
   u32x4 r[N];
   const bf16_t* src[N];
   long long ld[N];
@@ -184,7 +187,7 @@ struct Stage {
   DEVINL void init(const bf16_t* a, long long lda, const bf16_t* b, long long ldb, int tid) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int c = min(tid + i * 256, 2 * 32 * Geo<DH>::CH - 1);  // (the last threads of an uneven list repeat the last chunk)
+      const int c = min(tid + i * NT, 2 * 32 * Geo<DH>::CH - 1);  // (the last threads of an uneven list repeat the last chunk)
       const int im = c / (32 * Geo<DH>::CH), q = c - im * 32 * Geo<DH>::CH;
       row[i] = q / Geo<DH>::CH;
       const int ch = q - row[i] * Geo<DH>::CH;
@@ -668,17 +671,14 @@ __global__ __launch_bounds__(256) void rel_dtable_kernel(const RelP p) {
     if (in) list[at + __popcll(m & ((1ull << lane) - 1))] = (short)i;
     __syncthreads();
   }
-  // 2^k threads a row of partial sums, k by the length of the list
-  int per = 1;
-  while (per < total && per < 256) per <<= 1;
   const int rows = a.B * p.qblocks;
+  const float* part = p.part + (size_t)h * p.qblocks * n;
   float x = 0.f;
-  if (total > 0)
-    for (int r = tid / per; r < rows; r += 256 / per) {
-      const int b = r / p.qblocks, q = r - b * p.qblocks;
-      const float* src = p.part + (((size_t)b * a.H + h) * p.qblocks + q) * n;
-      for (int i = tid & (per - 1); i < total; i += per) x += src[list[i]];
-    }
+#pragma unroll 4
+  for (int i = tid; i < rows * total; i += 256) {
+    const int r = i / total, b = r / p.qblocks;
+    x += part[((size_t)b * a.H * p.qblocks + (r - b * p.qblocks)) * n + list[i - r * total]];
+  }
   x = wave_sum(x);
   if (lane == 0) red[wave] = x;
   __syncthreads();
@@ -721,10 +721,16 @@ DEVINL KBlock kblock_of(const RelP& p, int id) {
   return k;
 }
 
+// KS 16-key sub-tiles a wave.  Two (4 waves) let every Q and dO fragment feed two products; dK, dV, K and V of 32 keys do not fit
+// 256 registers at dh 128 (the accumulators then travel through the other half of the register file, 320 moves a tile), so there
+// a wave has one and the workgroup 8 waves.
+template <int DH>
+constexpr int key_subs() { return DH > 96 ? 1 : 2; }
+
 template <int DH, bool REL>
-__global__ __launch_bounds__(256, DH > 96 ? 1 : 2) void rel_dkdv_kernel(const RelP p) {
+__global__ __launch_bounds__(512 / key_subs<DH>(), 2) void rel_dkdv_kernel(const RelP p) {
   using G = Geo<DH>;
-  constexpr int ND = G::ND;
+  constexpr int ND = G::ND, KS = key_subs<DH>(), NT = 512 / KS;
   extern __shared__ __attribute__((aligned(16))) bf16_t smem[];
   const FactAttention& a = p.a;
   const int D = a.rel_max_distance, NB = 2 * (D + PAD) + 1;
@@ -737,7 +743,7 @@ __global__ __launch_bounds__(256, DH > 96 ? 1 : 2) void rel_dkdv_kernel(const Re
   const int kb = blk.kb, b = blk.bh / a.Hkv, hk = blk.bh - b * a.Hkv;
   const Vis v = vis_of(a, b);
   const int start = start_of(a, b);
-  const int j0 = kb * 128 + wave * 32;
+  const int j0 = kb * 128 + wave * 16 * KS;
   const bool active = j0 < v.len;
   // query rows that see any key of the block: positions [ka - hi, ke - lo], or all later ones if it holds a sink
   const long long ka = kb * 128, ke = min(kb * 128 + 127, v.len - 1);
@@ -747,20 +753,20 @@ __global__ __launch_bounds__(256, DH > 96 ? 1 : 2) void rel_dkdv_kernel(const Re
   const int t0 = (int)(min(qa, 1ll << 30) >> 5), T = qe >= qa ? (int)(qe >> 5) - t0 + 1 : 0, TT = T * group;
   const int per = (TT + blk.chunks - 1) / blk.chunks, ib = min(TT, blk.chunk * per), ie = min(TT, ib + per);
 
-  Frag<DH> K[2], V[2];
+  Frag<DH> K[KS], V[KS];
 #pragma unroll
-  for (int ks = 0; ks < 2; ++ks) {
+  for (int ks = 0; ks < KS; ++ks) {
     const long long j = max(0, min(j0 + ks * 16 + c, v.len - 1));
     frag_load<DH>(K[ks], (const bf16_t*)a.k + b * a.k_stride[0] + j * a.k_stride[1] + hk * a.k_stride[2], g);
     frag_load<DH>(V[ks], (const bf16_t*)a.v + b * a.v_stride[0] + j * a.v_stride[1] + hk * a.v_stride[2], g);
   }
-  pad_zero<DH>(smem, 4, tid, 256);
-  f32x4 dK[2][ND], dV[2][ND];
+  pad_zero<DH>(smem, 4, tid, NT);
+  f32x4 dK[KS][ND], dV[KS][ND];
 #pragma unroll
-  for (int ks = 0; ks < 2; ++ks)
+  for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
     for (int dt = 0; dt < ND; ++dt) dK[ks][dt] = dV[ks][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
-  Stage<DH> st;
+  Stage<DH, NT> st;
   float sv = 0.f;
   auto load = [&](int i) {  // i-th tile of the stream: head i / T of the group, query tile t0 + i % T
     const int hh = i / T, h = hk * group + hh, q0 = (t0 + i - hh * T) * 32;
@@ -785,7 +791,7 @@ __global__ __launch_bounds__(256, DH > 96 ? 1 : 2) void rel_dkdv_kernel(const Re
     const int hh = i / T, qt = i - hh * T;
     if (REL && (qt == 0 || i == ib)) {  // the next head's bias: after the last tile of the head before has been read
       __syncthreads();
-      load_bias(eb, p, hk * group + hh, tid, 256);
+      load_bias(eb, p, hk * group + hh, tid, NT);
     }
     __syncthreads();
     if (i + 1 < ie) {
@@ -793,33 +799,36 @@ __global__ __launch_bounds__(256, DH > 96 ? 1 : 2) void rel_dkdv_kernel(const Re
       if (i + 2 < ie) load(i + 2);
     }
     const int q0 = (t0 + qt) * 32, p0 = start + q0;
-    if (!active || v.none(j0, p0)) continue;
+    if (!active || v.none<16 * KS>(j0, p0)) continue;
     const bf16_t* Qs = smem + (i & 1) * 2 * G::IMG;
     const bf16_t* Os = Qs + G::IMG;
     const float* sl = stat + (i & 1) * 64;
-    f32x4 s[2][2], dp[2][2];  // [query sub-tile][key sub-tile]: lane = key c, queries 4 g .. 4 g + 3
+    f32x4 s[2][KS], dp[2][KS];  // [query sub-tile][key sub-tile]: lane = key c, queries 4 g .. 4 g + 3
     if (REL) {
       const int d0 = j0 - p0;
-      if (d0 - 31 >= D || d0 + 31 <= -D) {
+      if (d0 - 31 >= D || d0 + 16 * KS - 1 <= -D) {
         const float f = eb[d0 > 0 ? NB - 1 : 0];
 #pragma unroll
         for (int qs = 0; qs < 2; ++qs)
 #pragma unroll
-          for (int ks = 0; ks < 2; ++ks) s[qs][ks] = f32x4{f, f, f, f};
+          for (int ks = 0; ks < KS; ++ks) s[qs][ks] = f32x4{f, f, f, f};
       } else {
         const float* e = eb + d0 + D + PAD + c - 4 * g;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           s[1][0][r] = e[-r - 16];
-          s[0][0][r] = s[1][1][r] = e[-r];
-          s[0][1][r] = e[16 - r];
+          s[0][0][r] = e[-r];
+          if constexpr (KS > 1) {
+            s[1][1][r] = s[0][0][r];
+            s[0][1][r] = e[16 - r];
+          }
         }
       }
     } else {
 #pragma unroll
       for (int qs = 0; qs < 2; ++qs)
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks) s[qs][ks] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int ks = 0; ks < KS; ++ks) s[qs][ks] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
     f32x4 nl[2], nd[2];
 #pragma unroll
@@ -830,22 +839,22 @@ __global__ __launch_bounds__(256, DH > 96 ? 1 : 2) void rel_dkdv_kernel(const Re
       frag_lds<DH>(Q, Qs + (qs * 16 + c) * G::KP, g);
       frag_lds<DH>(dO, Os + (qs * 16 + c) * G::KP, g);
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
+      for (int ks = 0; ks < KS; ++ks) {
         s[qs][ks] = frag_dot<DH>(Q, K[ks], s[qs][ks]);
         dp[qs][ks] = frag_dot<DH>(dO, V[ks], nd[qs]);
       }
     }
-    f32x4 pr[2][2];
+    f32x4 pr[2][KS];
 #pragma unroll
     for (int qs = 0; qs < 2; ++qs)
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks)
+      for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           pr[qs][ks][r] = __builtin_amdgcn_exp2f(fmaf(s[qs][ks][r], p.sc, nl[qs][r]));
           dp[qs][ks][r] *= pr[qs][ks][r];
         }
-    if (!v.full(j0, p0) || q0 + 31 >= a.nq) {
+    if (!v.full<16 * KS>(j0, p0) || q0 + 31 >= a.nq) {
       bool lone[2][4];
 #pragma unroll
       for (int qs = 0; qs < 2; ++qs)
@@ -854,7 +863,7 @@ __global__ __launch_bounds__(256, DH > 96 ? 1 : 2) void rel_dkdv_kernel(const Re
 #pragma unroll
       for (int qs = 0; qs < 2; ++qs)
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks)
+        for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const bool ok = v.seen(j0 + ks * 16 + c, p0 + qs * 16 + 4 * g + r) & (q0 + qs * 16 + 4 * g + r < a.nq);
@@ -862,9 +871,9 @@ __global__ __launch_bounds__(256, DH > 96 ? 1 : 2) void rel_dkdv_kernel(const Re
             dp[qs][ks][r] = (ok & !lone[qs][r]) ? dp[qs][ks][r] : 0.f;
           }
     }
-    bf16x8 pb[2], db[2];
+    bf16x8 pb[KS], db[KS];
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
+    for (int ks = 0; ks < KS; ++ks) {
       pb[ks] = pack8(pr[0][ks], pr[1][ks]);
       db[ks] = pack8(dp[0][ks], dp[1][ks]);
     }
@@ -873,16 +882,16 @@ __global__ __launch_bounds__(256, DH > 96 ? 1 : 2) void rel_dkdv_kernel(const Re
       const bf16x8 of = frag_tr<DH>(Os, dt, lane);
       const bf16x8 qf = frag_tr<DH>(Qs, dt, lane);
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
+      for (int ks = 0; ks < KS; ++ks) {
         dV[ks][dt] = mfma16(of, pb[ks], dV[ks][dt]);
         dK[ks][dt] = mfma16(qf, db[ks], dK[ks][dt]);
       }
     }
   }
   if (blk.slot >= 0) {
-    f32x4* out = reinterpret_cast<f32x4*>(p.dkv) + ((size_t)blk.slot * 4 + wave) * (4 * ND * 64) + lane;
+    f32x4* out = reinterpret_cast<f32x4*>(p.dkv) + ((size_t)blk.slot * 8 + wave * KS) * (2 * ND * 64) + lane;
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks)
+    for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
       for (int dt = 0; dt < ND; ++dt) {
         out[(ks * ND + dt) * 128] = dK[ks][dt];
@@ -891,7 +900,7 @@ __global__ __launch_bounds__(256, DH > 96 ? 1 : 2) void rel_dkdv_kernel(const Re
     return;
   }
 #pragma unroll
-  for (int ks = 0; ks < 2; ++ks) {
+  for (int ks = 0; ks < KS; ++ks) {
     const int j = j0 + ks * 16 + c;
     if (j >= a.nk) continue;
     bf16_t* kr = (bf16_t*)a.dk + b * a.dk_stride[0] + (long long)j * a.dk_stride[1] + hk * a.dk_stride[2] + g * 4;
@@ -910,10 +919,10 @@ __global__ __launch_bounds__(256, DH > 96 ? 1 : 2) void rel_dkdv_kernel(const Re
   }
 }
 
-// the chunks of a block, in order: a wave per accumulator fragment (wave, ks, dt, K or V) of the kernel above
+// the chunks of a block, in order: a wave per accumulator fragment (16-key sub-tile, dt, K or V) of the kernel above
 template <int DH>
 __global__ __launch_bounds__(256) void rel_join_dkdv_kernel(const RelP p) {
-  constexpr int ND = Geo<DH>::ND, FR = 4 * 4 * ND;  // fragments of a block
+  constexpr int ND = Geo<DH>::ND, FR = 8 * 2 * ND;  // fragments of a block
   const FactAttention& a = p.a;
   const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
   const int f = (blockIdx.x * 4 + (threadIdx.x >> 6)) % FR, blk = (blockIdx.x * 4 + (threadIdx.x >> 6)) / FR;
@@ -926,8 +935,8 @@ __global__ __launch_bounds__(256) void rel_join_dkdv_kernel(const RelP p) {
   const f32x4* src = reinterpret_cast<const f32x4*>(p.dkv) + ((size_t)slot * FR + f) * 64 + lane;
   f32x4 x = src[0];
   for (int i = 1; i < n; ++i) x += src[(size_t)i * FR * 64];
-  const int wave = f / (4 * ND), ks = f / (2 * ND) & 1, dt = (f >> 1) % ND, isv = f & 1;
-  const int j = kb * 128 + wave * 32 + ks * 16 + c;
+  const int dt = (f >> 1) % ND, isv = f & 1;
+  const int j = kb * 128 + f / (2 * ND) * 16 + c;
   if (j >= a.nk) return;
   const int64_t* st = isv ? a.dv_stride : a.dk_stride;
   const float k = isv ? 1.f : a.scale;
@@ -949,6 +958,7 @@ __global__ __launch_bounds__(256, 2) void rel_rows_kernel(const RelP p) {
   constexpr int BYTES = 4 * 16 * OP * 4 > 4 * G::IMG * 2 ? 4 * 16 * OP * 4 : 4 * G::IMG * 2;
   __shared__ __attribute__((aligned(16))) unsigned char smem[BYTES];
   __shared__ float ml[4][2][16];
+  extern __shared__ float tab[];  // bias of the group's heads by distance, if p.rowtab
   const FactAttention& a = p.a;
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, c = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -965,7 +975,10 @@ __global__ __launch_bounds__(256, 2) void rel_rows_kernel(const RelP p) {
   const bf16_t* kb = (const bf16_t*)a.k + b * a.k_stride[0] + hk * a.k_stride[2];
   const bf16_t* vb = (const bf16_t*)a.v + b * a.v_stride[0] + hk * a.v_stride[2];
   bf16_t* Vs = reinterpret_cast<bf16_t*>(smem) + wave * G::IMG;
-  const int D = a.rel_max_distance;
+  const int D = a.rel_max_distance, n = 2 * D + 1, hr = row / a.nq;
+  auto bias = [&](int head, int i) {  // distance i - D
+    return a.rel_table[(size_t)min(max(a.rel_map[i], 0), a.rel_buckets - 1) * a.H + head] * p.rscale;
+  };
 
   Frag<DH> K[2];
   u32x4 vr[NV];
@@ -985,21 +998,43 @@ __global__ __launch_bounds__(256, 2) void rel_rows_kernel(const RelP p) {
   for (int dt = 0; dt < ND; ++dt) O[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
   float m = -INFINITY, l = 0.f;
   if (tb + wave < te) load(tb + wave);
+  float left = 0.f, right = 0.f;
+  if (REL) {
+    left = bias(h, 0);
+    right = bias(h, n - 1);
+    // the table, where this workgroup's tiles come nearer than D to a row
+    if (p.rowtab && tb < te && tl.at(tb) * 32 - (start + a.nq - 1) < D && tl.at(te - 1) * 32 + 31 - start > -D) {
+      for (int i = tid; i < group * n; i += 256) tab[i] = bias(hk * group + i / n, i % n);
+      __syncthreads();
+    }
+  }
   for (int t = tb + wave; t < te; t += 4) {
     const int j0 = tl.at(t) * 32;
     f32x4 s[2];
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      s[ks] = frag_dot<DH>(K[ks], Q, f32x4{0.f, 0.f, 0.f, 0.f});
+    for (int ks = 0; ks < 2; ++ks) s[ks] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (REL) {
+      if (j0 + 31 - start <= -D || j0 - (start + a.nq - 1) >= D) {
+        const float f = j0 < start ? left : right;
+        s[0] = s[1] = f32x4{f, f, f, f};
+      } else {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int j = j0 + ks * 16 + 4 * g + r;
-        if (REL) {
-          const int bk = min(max(a.rel_map[min(max(j - pos, -D), D) + D], 0), a.rel_buckets - 1);
-          s[ks][r] += a.rel_table[(size_t)bk * a.H + h] * p.rscale;
-        }
-        s[ks][r] = v.seen(j, pos) ? s[ks][r] : -INFINITY;
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int i = min(max(j0 + ks * 16 + 4 * g + r - pos, -D), D) + D;
+            s[ks][r] = p.rowtab ? tab[hr * n + i] : bias(h, i);
+          }
       }
+    }
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) s[ks] = frag_dot<DH>(K[ks], Q, s[ks]);
+    // (all rows lie in the 16 positions from start on)
+    if (!(j0 + 31 < v.len && j0 + 31 - start <= v.hi && (j0 - (start + a.nq - 1) >= v.lo || j0 + 31 < v.sinks))) {
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[ks][r] = v.seen(j0 + ks * 16 + 4 * g + r, pos) ? s[ks][r] : -INFINITY;
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -1162,6 +1197,7 @@ RelP params(const FactAttention& a) {
   p.qblocks = (a.nq + 127) / 128;
   p.nwg = 0;
   p.splits = 1;
+  p.rowtab = 0;
   p.dsum = nullptr;
   p.part = nullptr;
   p.dkv = nullptr;
@@ -1196,7 +1232,9 @@ int fwd_t(const FactAttention& a, void* ws, hipStream_t s) {
   if (few_rows(a)) {
     p.splits = row_splits(a);
     p.part = (float*)ws;
-    FACT_LAUNCH((rel_rows_kernel<DH, REL>), dim3(p.splits * a.B * a.Hkv), dim3(256), 0, s, p);
+    const size_t tab = (size_t)(a.H / a.Hkv) * (2 * a.rel_max_distance + 1) * 4;
+    p.rowtab = REL && tab <= 16384;
+    FACT_LAUNCH((rel_rows_kernel<DH, REL>), dim3(p.splits * a.B * a.Hkv), dim3(256), p.rowtab ? tab : 0, s, p);
     if (p.splits > 1) FACT_LAUNCH(rel_join_kernel, dim3(a.B * a.H * a.nq), dim3(64), 0, s, p);
     return launched();
   }
@@ -1224,7 +1262,7 @@ int bwd_t(const FactAttention& a, void* ws, hipStream_t s) {
   FACT_LAUNCH((rel_dq_kernel<DH, REL>), dim3(p.nwg), dim3(256), lds1, s, p);
   if (REL) FACT_LAUNCH(rel_dtable_kernel, dim3(a.H, a.rel_buckets), dim3(256), 0, s, p);
   p.nwg = (p.sblocks * p.schunks + (p.kblocks - p.sblocks) * p.chunks) * a.B * a.Hkv;
-  FACT_LAUNCH((rel_dkdv_kernel<DH, REL>), dim3(p.nwg), dim3(256), lds2, s, p);
+  FACT_LAUNCH((rel_dkdv_kernel<DH, REL>), dim3(p.nwg), dim3(512 / key_subs<DH>()), lds2, s, p);
   const int joined = ((p.schunks > 1 ? p.sblocks : 0) + (p.chunks > 1 ? p.kblocks - p.sblocks : 0)) * a.B * a.Hkv;
   if (joined) FACT_LAUNCH(rel_join_dkdv_kernel<DH>, dim3(joined * 4 * Geo<DH>::ND), dim3(256), 0, s, p);
   return launched();
