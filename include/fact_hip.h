@@ -227,7 +227,8 @@ int fact_create_ex(const FactConfig* cfg, const FactAttnCfg* attn, int max_batch
  * Handle-free operators on caller tensors (bf16 unless stated); the engine runs the same kernels for a stack whose
  * FactAttnCfg asks for them (fact_create_ex).  No allocation, no host synchronisation and no memset nodes: every call can be
  * captured into a HIP graph.  Row-major tensors [batch][token][head][dh] given by a pointer and three element strides
- * (batch, token, head); the dh values of a head are contiguous; pointers are 16-byte aligned, strides multiples of 8.  Input
+ * (batch, token, head); the dh values of a head are contiguous; pointers are 16-byte aligned, strides multiples of 8,
+ * token strides up to 2^25.  Input
  * strides may be 0 (a broadcast input); outputs must not overlap each other or an input unless stated. */
 
 /* Attention with an optional sliding window, sinks and a learned relative position bias by buckets.

@@ -56,7 +56,7 @@ def _heads(t, name, dtype, device=None):
 
 def _addressable(t):
     s = t.stride()
-    return s[3] == 1 and not (s[0] | s[1] | s[2]) & 7 and not t.data_ptr() & 15
+    return s[3] == 1 and not (s[0] | s[1] | s[2]) & 7 and s[1] <= 1 << 25 and not t.data_ptr() & 15
 
 
 def _dest(t, name, shape, dtype, device):

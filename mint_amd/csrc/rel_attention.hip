@@ -16,6 +16,7 @@
 namespace {
 
 constexpr float LOG2E = 1.4426950408889634f;
+constexpr float THR = 6.0f;
 constexpr int PAD = 80;  // distances past +-D that a 32 x 32 tile which still touches (-D, D) can reach (62), and its folds (75)
 typedef __attribute__((address_space(3))) bf16x4 lds_bf16x4;
 
@@ -176,29 +177,51 @@ DEVINL int xcd_order(int id, int n) {
   return (x < rem ? x * (per + 1) : rem * (per + 1) + (x - rem) * per) + (id >> 3);
 }
 
+// 16 bytes at a wave-uniform base and a 32-bit byte offset of the lane (one address register; token strides are checked)
+DEVINL u32x4 load16(const bf16_t* base, unsigned off) {
+  return *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(base) + off);
+}
+
 // ---- staging of two 32-row tiles (K and V, or Q and dO) through registers into LDS -------------------------------------
+// A thread moves chunks tid, tid + NT, ...; a wave's 64 chunks lie in one image.  (Threads past the end of an uneven list repeat
+// the last chunk: no branch around a load, which would make the compiler wait for the others first.)
 template <int DH, int NT = 256>
 struct Stage {
-  static constexpr int N = (2 * 32 * Geo<DH>::CH + NT - 1) / NT;
+  static constexpr int PER = 32 * Geo<DH>::CH, N = (2 * PER + NT - 1) / NT;
   u32x4 r[N];
-  const bf16_t* src[N];
-  long long ld[N];
+  unsigned off[N];
   int row[N], dst[N];
-  DEVINL void init(const bf16_t* a, long long lda, const bf16_t* b, long long ldb, int tid) {
+  unsigned lda, ldb;  // bytes
+  unsigned second;    // bit i: chunk i of this wave lies in the second image
+  DEVINL void init(long long a, long long b, int tid) {
+    lda = (unsigned)a * 2;
+    ldb = (unsigned)b * 2;
+    second = 0;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int c = min(tid + i * NT, 2 * 32 * Geo<DH>::CH - 1);  // (the last threads of an uneven list repeat the last chunk)
-      const int im = c / (32 * Geo<DH>::CH), q = c - im * 32 * Geo<DH>::CH;
+      const int c = min(tid + i * NT, 2 * PER - 1);
+      const int im = __builtin_amdgcn_readfirstlane(c / PER), q = c - im * PER;
       row[i] = q / Geo<DH>::CH;
       const int ch = q - row[i] * Geo<DH>::CH;
-      src[i] = (im ? b : a) + ch * 8;
-      ld[i] = im ? ldb : lda;
+      second |= (unsigned)im << i;
+      off[i] = (unsigned)row[i] * (im ? ldb : lda) + ch * 16;
       dst[i] = im * Geo<DH>::IMG + row[i] * Geo<DH>::KP + ch * 8;
     }
   }
-  DEVINL void load(int row0, int last) {  // rows past `last` repeat it: finite values that the caller masks
+  // rows row0 .. row0 + 31 of a and b (wave-uniform pointers to row 0); rows past `last` repeat it: finite values, masked later
+  DEVINL void load(const bf16_t* a, const bf16_t* b, int row0, int last) {
+    a += (long long)row0 * (lda / 2);
+    b += (long long)row0 * (ldb / 2);
+    if (row0 + 31 <= last) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) r[i] = *reinterpret_cast<const u32x4*>(src[i] + (long long)min(row0 + row[i], last) * ld[i]);
+      for (int i = 0; i < N; ++i) r[i] = load16((second >> i) & 1 ? b : a, off[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const unsigned past = (unsigned)max(0, row0 + row[i] - last);
+        r[i] = load16((second >> i) & 1 ? b : a, off[i] - past * ((second >> i) & 1 ? ldb : lda));
+      }
+    }
   }
   DEVINL void store(bf16_t* lds) {
 #pragma unroll
@@ -246,8 +269,9 @@ __global__ __launch_bounds__(256, 2) void rel_fwd_kernel(const RelP p) {
     frag_load<DH>(Q[qs], (const bf16_t*)a.q + b * a.q_stride[0] + (long long)min(q0 + qs * 16 + c, a.nq - 1) * a.q_stride[1] +
                              h * a.q_stride[2], g);
   Stage<DH> st;
-  st.init((const bf16_t*)a.k + b * a.k_stride[0] + hk * a.k_stride[2], a.k_stride[1],
-          (const bf16_t*)a.v + b * a.v_stride[0] + hk * a.v_stride[2], a.v_stride[1], tid);
+  const bf16_t* kp = (const bf16_t*)a.k + b * a.k_stride[0] + hk * a.k_stride[2];
+  const bf16_t* vp = (const bf16_t*)a.v + b * a.v_stride[0] + hk * a.v_stride[2];
+  st.init(a.k_stride[1], a.v_stride[1], tid);
   pad_zero<DH>(smem, 4, tid, 256);
   if (REL) load_bias(eb, p, h, tid, 256);
   f32x4 O[2][ND];
@@ -260,16 +284,16 @@ __global__ __launch_bounds__(256, 2) void rel_fwd_kernel(const RelP p) {
     for (int dt = 0; dt < ND; ++dt) O[qs][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
   if (tl.T > 0) {
-    st.load(tl.at(0) * 32, v.len - 1);
+    st.load(kp, vp, tl.at(0) * 32, v.len - 1);
     st.store(smem);
-    if (tl.T > 1) st.load(tl.at(1) * 32, v.len - 1);
+    if (tl.T > 1) st.load(kp, vp, tl.at(1) * 32, v.len - 1);
   }
   const int D = a.rel_max_distance;
   for (int t = 0; t < tl.T; ++t) {
     __syncthreads();
     if (t + 1 < tl.T) {
       st.store(smem + ((t + 1) & 1) * 2 * G::IMG);
-      if (t + 2 < tl.T) st.load(tl.at(t + 2) * 32, v.len - 1);
+      if (t + 2 < tl.T) st.load(kp, vp, tl.at(t + 2) * 32, v.len - 1);
     }
     const int j0 = tl.at(t) * 32;
     if (!active || v.none(j0, p0)) continue;
@@ -315,27 +339,50 @@ __global__ __launch_bounds__(256, 2) void rel_fwd_kernel(const RelP p) {
           for (int r = 0; r < 4; ++r)
             s[ks][qs][r] = v.seen(j0 + ks * 16 + 4 * g + r, p0 + qs * 16 + c) ? s[ks][qs][r] : -INFINITY;
     }
+    // The reference point m of a row's exponents is raised only when a score passes it by THR powers of two: any m that keeps
+    // exp2 in range gives the same softmax, and the common path needs no lane but its own.
     bf16x8 pb[2], pl[2], pm[2];
+    float mx[2];
 #pragma unroll
     for (int qs = 0; qs < 2; ++qs) {
-      float mx = fmaxf(fmaxf(fmaxf(s[0][qs][0], s[0][qs][1]), fmaxf(s[0][qs][2], s[0][qs][3])),
-                       fmaxf(fmaxf(s[1][qs][0], s[1][qs][1]), fmaxf(s[1][qs][2], s[1][qs][3])));
-      mx = allmax4(mx) * p.sc;
-      if (__any(mx > m[qs])) {
-        const float mn = fmaxf(m[qs], mx);
-        const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[qs] - mn);
-        m[qs] = mn;
-        l[qs] *= alpha;
+      const float mu = m[qs] == -INFINITY ? 0.f : m[qs];  // -inf: the row has seen no key yet
 #pragma unroll
-        for (int dt = 0; dt < ND; ++dt) O[qs][dt] *= alpha;
+      for (int r = 0; r < 4; ++r) {
+        s[0][qs][r] = fmaf(s[0][qs][r], p.sc, -mu);
+        s[1][qs][r] = fmaf(s[1][qs][r], p.sc, -mu);
       }
-      const float mu = m[qs] == -INFINITY ? 0.f : m[qs];  // a row that has seen no key yet: every p below is 0
+      mx[qs] = fmaxf(fmaxf(fmaxf(s[0][qs][0], s[0][qs][1]), fmaxf(s[0][qs][2], s[0][qs][3])),
+                     fmaxf(fmaxf(s[1][qs][0], s[1][qs][1]), fmaxf(s[1][qs][2], s[1][qs][3])));
+    }
+    if (__any((mx[0] > THR) | (mx[1] > THR) | ((m[0] == -INFINITY) & (mx[0] > -INFINITY)) |
+              ((m[1] == -INFINITY) & (mx[1] > -INFINITY)))) {
+#pragma unroll
+      for (int qs = 0; qs < 2; ++qs) {
+        const bool first = m[qs] == -INFINITY;
+        const float top = allmax4(mx[qs]);                       // relative to m, or to 0
+        const float d = first ? (top == -INFINITY ? 0.f : top) : fmaxf(top, 0.f);
+        const float alpha = __builtin_amdgcn_exp2f(-d);          // (first: nothing has been summed)
+        m[qs] = first ? top : m[qs] + d;
+        l[qs] = first ? 0.f : l[qs] * alpha;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          s[0][qs][r] -= d;
+          s[1][qs][r] -= d;
+        }
+#pragma unroll
+        for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) O[qs][dt][r] = first ? 0.f : O[qs][dt][r] * alpha;
+      }
+    }
+#pragma unroll
+    for (int qs = 0; qs < 2; ++qs) {
       f32x4 e0, e1;
       float ls = 0.f;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        e0[r] = __builtin_amdgcn_exp2f(fmaf(s[0][qs][r], p.sc, -mu));
-        e1[r] = __builtin_amdgcn_exp2f(fmaf(s[1][qs][r], p.sc, -mu));
+        e0[r] = __builtin_amdgcn_exp2f(s[0][qs][r]);
+        e1[r] = __builtin_amdgcn_exp2f(s[1][qs][r]);
         ls += e0[r] + e1[r];
       }
       l[qs] += ls;
@@ -453,9 +500,10 @@ __global__ __launch_bounds__(256, 2) void rel_dq_kernel(const RelP p) {
   const Tiles tl = tiles_of(v, (long long)start + qb * 128, (long long)start + min(qb * 128 + 127, a.nq - 1));
 
   Stage<DH> st;
-  st.init((const bf16_t*)a.k + b * a.k_stride[0] + hk * a.k_stride[2], a.k_stride[1],
-          (const bf16_t*)a.v + b * a.v_stride[0] + hk * a.v_stride[2], a.v_stride[1], tid);
-  if (tl.T > 0) st.load(tl.at(0) * 32, v.len - 1);
+  const bf16_t* kp = (const bf16_t*)a.k + b * a.k_stride[0] + hk * a.k_stride[2];
+  const bf16_t* vp = (const bf16_t*)a.v + b * a.v_stride[0] + hk * a.v_stride[2];
+  st.init(a.k_stride[1], a.v_stride[1], tid);
+  if (tl.T > 0) st.load(kp, vp, tl.at(0) * 32, v.len - 1);
   Frag<DH> Q[2], dO[2];
   float nL[2], nD[2];
   bool live[2];  // a query of the call that sees more than one key
@@ -518,13 +566,13 @@ __global__ __launch_bounds__(256, 2) void rel_dq_kernel(const RelP p) {
   }
   if (tl.T > 0) {
     st.store(smem);
-    if (tl.T > 1) st.load(tl.at(1) * 32, v.len - 1);
+    if (tl.T > 1) st.load(kp, vp, tl.at(1) * 32, v.len - 1);
   }
   for (int t = 0; t < tl.T; ++t) {
     __syncthreads();
     if (t + 1 < tl.T) {
       st.store(smem + ((t + 1) & 1) * 2 * G::IMG);
-      if (t + 2 < tl.T) st.load(tl.at(t + 2) * 32, v.len - 1);
+      if (t + 2 < tl.T) st.load(kp, vp, tl.at(t + 2) * 32, v.len - 1);
     }
     const int j0 = tl.at(t) * 32;
     if (!active || v.none(j0, p0)) continue;
@@ -767,12 +815,12 @@ __global__ __launch_bounds__(512 / key_subs<DH>(), 2) void rel_dkdv_kernel(const
 #pragma unroll
     for (int dt = 0; dt < ND; ++dt) dK[ks][dt] = dV[ks][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
   Stage<DH, NT> st;
+  st.init(a.q_stride[1], a.dout_stride[1], tid);
   float sv = 0.f;
   auto load = [&](int i) {  // i-th tile of the stream: head i / T of the group, query tile t0 + i % T
     const int hh = i / T, h = hk * group + hh, q0 = (t0 + i - hh * T) * 32;
-    st.init((const bf16_t*)a.q + b * a.q_stride[0] + h * a.q_stride[2], a.q_stride[1],
-            (const bf16_t*)a.dout + b * a.dout_stride[0] + h * a.dout_stride[2], a.dout_stride[1], tid);
-    st.load(q0, a.nq - 1);
+    st.load((const bf16_t*)a.q + b * a.q_stride[0] + h * a.q_stride[2],
+            (const bf16_t*)a.dout + b * a.dout_stride[0] + h * a.dout_stride[2], q0, a.nq - 1);
     if (tid < 64) {
       const size_t at = ((size_t)b * a.H + h) * a.nq + min(q0 + (tid & 31), a.nq - 1);
       sv = tid < 32 ? -a.lse[at] : -p.dsum[at];
@@ -954,6 +1002,7 @@ template <int DH, bool REL>
 __global__ __launch_bounds__(256, 2) void rel_rows_kernel(const RelP p) {
   using G = Geo<DH>;
   constexpr int ND = G::ND, NV = G::CH / 2;  // 16-byte chunks of V a lane moves per 32-key tile
+  constexpr int DEPTH = DH > 96 ? 1 : 2;     // tiles in flight a wave: two of dh 128 do not fit 256 registers
   constexpr int OP = DH + 4;                 // pitch of the joined rows (floats)
   constexpr int BYTES = 4 * 16 * OP * 4 > 4 * G::IMG * 2 ? 4 * 16 * OP * 4 : 4 * G::IMG * 2;
   __shared__ __attribute__((aligned(16))) unsigned char smem[BYTES];
@@ -962,8 +1011,9 @@ __global__ __launch_bounds__(256, 2) void rel_rows_kernel(const RelP p) {
   const FactAttention& a = p.a;
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, c = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int split = blockIdx.x % p.splits, bh = blockIdx.x / p.splits;
-  const int b = bh / a.Hkv, hk = bh - b * a.Hkv, group = a.H / a.Hkv, R = group * a.nq;
+  // key heads of one range of tokens beside each other on one XCD: their rows share cache lines
+    const int id = p.splits > 1 ? (int)blockIdx.x : xcd_order(blockIdx.x, p.nwg), bs = id / a.Hkv, hk = id - bs * a.Hkv, b = bs / p.splits, split = bs - b * p.splits;
+  const int group = a.H / a.Hkv, R = group * a.nq;
   const Vis v = vis_of(a, b);
   const int start = start_of(a, b);
   const Tiles tl = tiles_of(v, start, (long long)start + a.nq - 1);
@@ -980,24 +1030,38 @@ __global__ __launch_bounds__(256, 2) void rel_rows_kernel(const RelP p) {
     return a.rel_table[(size_t)min(max(a.rel_map[i], 0), a.rel_buckets - 1) * a.H + head] * p.rscale;
   };
 
-  Frag<DH> K[2];
-  u32x4 vr[NV];
-  auto load = [&](int t) {
-    const int j0 = tl.at(t) * 32;
+  struct Tile {  // one 32-key tile in flight: K as fragments, V as rows
+    Frag<DH> K[2];
+    u32x4 vr[NV];
+  } tile[DEPTH];
+  const unsigned ldk = (unsigned)a.k_stride[1] * 2, ldv = (unsigned)a.v_stride[1] * 2;
+  auto load = [&](Tile& x, int t) {
+    const int j0 = tl.at(t) * 32, cut = j0 + 31 - (v.len - 1);  // > 0: rows past the last repeat it
+    const bf16_t* k0 = kb + (long long)j0 * a.k_stride[1];
+    const bf16_t* v0 = vb + (long long)j0 * a.v_stride[1];
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks)
-      frag_load<DH>(K[ks], kb + (long long)min(j0 + ks * 16 + c, v.len - 1) * a.k_stride[1], g);
+    for (int ks = 0; ks < 2; ++ks) {
+      const unsigned r = cut > 0 ? min(ks * 16 + c, 31 - cut) : ks * 16 + c;
+#pragma unroll
+      for (int kd = 0; kd < G::KD; ++kd) {
+        x.K[ks].f[kd] = zero_bf16x8();
+        if (kd * 32 + 32 <= DH || kd * 32 + g * 8 < DH)
+          x.K[ks].f[kd] = __builtin_bit_cast(bf16x8, load16(k0, r * ldk + kd * 64 + g * 16));
+      }
+    }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int q = lane + i * 64, r = q / G::CH, ch = q - r * G::CH;
-      vr[i] = *reinterpret_cast<const u32x4*>(vb + (long long)min(j0 + r, v.len - 1) * a.v_stride[1] + ch * 8);
+      x.vr[i] = load16(v0, (unsigned)(cut > 0 ? min(r, 31 - cut) : r) * ldv + ch * 16);
     }
   };
   f32x4 O[ND];
 #pragma unroll
   for (int dt = 0; dt < ND; ++dt) O[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
   float m = -INFINITY, l = 0.f;
-  if (tb + wave < te) load(tb + wave);
+#pragma unroll
+  for (int i = 0; i < DEPTH; ++i)
+    if (tb + wave + 4 * i < te) load(tile[i], tb + wave + 4 * i);
   float left = 0.f, right = 0.f;
   if (REL) {
     left = bias(h, 0);
@@ -1008,7 +1072,7 @@ __global__ __launch_bounds__(256, 2) void rel_rows_kernel(const RelP p) {
       __syncthreads();
     }
   }
-  for (int t = tb + wave; t < te; t += 4) {
+  auto step = [&](Tile& x, int t) {
     const int j0 = tl.at(t) * 32;
     f32x4 s[2];
 #pragma unroll
@@ -1028,7 +1092,7 @@ __global__ __launch_bounds__(256, 2) void rel_rows_kernel(const RelP p) {
       }
     }
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks) s[ks] = frag_dot<DH>(K[ks], Q, s[ks]);
+    for (int ks = 0; ks < 2; ++ks) s[ks] = frag_dot<DH>(x.K[ks], Q, s[ks]);
     // (all rows lie in the 16 positions from start on)
     if (!(j0 + 31 < v.len && j0 + 31 - start <= v.hi && (j0 - (start + a.nq - 1) >= v.lo || j0 + 31 < v.sinks))) {
 #pragma unroll
@@ -1039,9 +1103,9 @@ __global__ __launch_bounds__(256, 2) void rel_rows_kernel(const RelP p) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int q = lane + i * 64, r = q / G::CH, ch = q - r * G::CH;
-      *reinterpret_cast<u32x4*>(Vs + r * G::KP + ch * 8) = vr[i];
+      *reinterpret_cast<u32x4*>(Vs + r * G::KP + ch * 8) = x.vr[i];
     }
-    if (t + 4 < te) load(t + 4);
+    if (t + 4 * DEPTH < te) load(x, t + 4 * DEPTH);
     float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
                      fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
     mx = allmax4(mx) * p.sc;
@@ -1072,6 +1136,11 @@ __global__ __launch_bounds__(256, 2) void rel_rows_kernel(const RelP p) {
       }
     }
     __builtin_amdgcn_wave_barrier();
+  };
+  for (int t = tb + wave; t < te; t += 4 * DEPTH) {
+#pragma unroll
+    for (int i = 0; i < DEPTH; ++i)
+      if (t + 4 * i < te) step(tile[i], t + 4 * i);
   }
   l = allsum4(l);
   __syncthreads();
@@ -1097,7 +1166,7 @@ __global__ __launch_bounds__(256, 2) void rel_rows_kernel(const RelP p) {
       o += *reinterpret_cast<const f32x4*>(Oj + (w * 16 + r) * OP + d) * f;
     }
     if (p.splits > 1) {
-      float* out = p.part + ((size_t)blockIdx.x * R + r) * (DH + 4);
+      float* out = p.part + (((size_t)(b * a.Hkv + hk) * p.splits + split) * R + r) * (DH + 4);
       if (d == 0) {
         out[0] = M;
         out[1] = lt;
@@ -1183,7 +1252,10 @@ long long span(const FactAttention& a) {
 // splits of the few-row kernel: enough workgroups to fill 256 CUs twice, at least 8 tiles (2 a wave) each
 int row_splits(const FactAttention& a) {
   const long long tiles = (span(a) + 31) / 32, wgs = (long long)a.B * a.Hkv;
-  long long s = std::min((512 + wgs - 1) / wgs, tiles / 8);
+#ifndef ROWT
+#define ROWT 512
+#endif
+  long long s = std::min((ROWT + wgs - 1) / wgs, tiles / 8);
   return (int)std::max(1ll, std::min(s, 256ll));
 }
 
@@ -1232,9 +1304,10 @@ int fwd_t(const FactAttention& a, void* ws, hipStream_t s) {
   if (few_rows(a)) {
     p.splits = row_splits(a);
     p.part = (float*)ws;
+    p.nwg = p.splits * a.B * a.Hkv;
     const size_t tab = (size_t)(a.H / a.Hkv) * (2 * a.rel_max_distance + 1) * 4;
     p.rowtab = REL && tab <= 16384;
-    FACT_LAUNCH((rel_rows_kernel<DH, REL>), dim3(p.splits * a.B * a.Hkv), dim3(256), p.rowtab ? tab : 0, s, p);
+    FACT_LAUNCH((rel_rows_kernel<DH, REL>), dim3(p.nwg), dim3(256), p.rowtab ? tab : 0, s, p);
     if (p.splits > 1) FACT_LAUNCH(rel_join_kernel, dim3(a.B * a.H * a.nq), dim3(64), 0, s, p);
     return launched();
   }
@@ -1310,6 +1383,8 @@ int rel_attention_check(const FactAttention& a, bool backward, const char** why)
   for (int i = 0; i < (backward ? 8 : 4); ++i) {
     if (!t[i].p) return bad(-1, "null tensor");
     if ((uintptr_t)t[i].p & 15) return bad(-1, "tensors must be 16-byte aligned");
+    // (tiles of 32 rows are addressed with 32-bit byte offsets)
+    if (t[i].st[1] < 0 || t[i].st[1] > 1 << 25) return bad(-1, "token strides must be 0..2^25 elements");
     for (int k = 0; k < 3; ++k) {
       if (t[i].st[k] & 7) return bad(-1, "strides must be multiples of 8 elements");
       const int n[3] = {a.B, i == 1 || i == 2 || i == 6 || i == 7 ? a.nk : a.nq, i == 1 || i == 2 || i == 6 || i == 7 ? a.Hkv : a.H};

@@ -63,6 +63,7 @@ def test_struct_sizes_match_the_header(lib, tmp_path):
     (dict(scale=math.inf), -1, "scale"), (dict(scale=1e-9), -1, "scale"), (dict(sinks=-1), -1, "sinks"),
     (dict(q=None), -1, "null"), (dict(v=4096 + 8), -1, "aligned"), (dict(out_lo=4096 + 2), -1, "aligned"),
     (dict(k_stride=(24 * 128, 132, 64)), -1, "multiples of 8"), (dict(dq_stride=(8 * 256, 0, 64)), -1, "broadcast"),
+    (dict(v_stride=(1 << 40, (1 << 25) + 8, 64)), -1, "2^25"), (dict(q_stride=(1 << 40, -64, 64)), -1, "2^25"),
     (dict(dk_stride=(0, 128, 64)), -1, "broadcast"), (dict(lse=None), -1, "lse"),
     (dict(BIAS, rel_map=None), -1, "rel_map"), (dict(BIAS, rel_buckets=0), -1, "rel_buckets"),
     (dict(BIAS, rel_buckets=257), -1, "rel_buckets"), (dict(BIAS, rel_max_distance=0), -1, "rel_max_distance"),

@@ -278,20 +278,26 @@ def test_strides_packed_views_broadcast_and_unaligned_inputs():
     assert torch.equal(dst[:, :, 0], want[0]) and torch.equal(dst[:, :, 2], want[2])
 
 
-def test_long_cache_offsets_past_32_bits():
-    """Element offsets beyond 2^31 in one sequence: 2 heads x 128 x 9 M tokens would not fit a small box, so the token stride
-    carries them - 40 keys, 2^26 elements apart."""
-    stride = 1 << 26
-    big = torch.empty(40 * stride + 4096, dtype=torch.bfloat16, device=DEV)
+@pytest.mark.parametrize("stride", [1 << 24, 1 << 25, 1 << 26])
+def test_offsets_past_32_bits(stride):
+    """Element offsets beyond 2^31 in one sequence, carried by the token stride (the widest is copied by the call)."""
+    n = 200 if stride < 1 << 25 else 100 if stride < 1 << 26 else 40
+    big = torch.empty((n - 1) * stride + 4096, dtype=torch.bfloat16, device=DEV)
     gen = torch.Generator().manual_seed(6)
-    src = _rand(gen, 2, 40, 2, 64)
-    k = big.as_strided((1, 40, 2, 64), (40 * stride, stride, 64, 1))
-    v = big.as_strided((1, 40, 2, 64), (40 * stride, stride, 64, 1), 2048)
+    src = _rand(gen, 2, n, 2, 64)
+    k = big.as_strided((1, n, 2, 64), (n * stride, stride, 64, 1))
+    v = big.as_strided((1, n, 2, 64), (n * stride, stride, 64, 1), 2048)
     k.copy_(src[:1])
     v.copy_(src[1:])
     for nq in (1, 40):
         q = _rand(gen, 1, nq, 2, 64)
         assert torch.equal(A.attention(q, k, v), A.attention(q, src[:1], src[1:]))
+    do = _rand(gen, 1, n, 2, 64)
+    grads = []
+    for x, y in ((k, v), (src[:1], src[1:])):
+        o, saved = A.attention(x, x, y, training=True)
+        grads.append((o,) + A.attention_backward(do, x, x, y, o, saved))
+    assert all(torch.equal(x, y) for x, y in zip(*grads))
 
 
 def test_results_repeat_exactly():
