@@ -185,8 +185,9 @@ DEVINL u32x4 load16(const bf16_t* base, unsigned off) {
 // ---- staging of two 32-row tiles (K and V, or Q and dO) through registers into LDS -------------------------------------
 // A thread moves chunks tid, tid + NT, ...; a wave's 64 chunks lie in one image.  (Threads past the end of an uneven list repeat
 // the last chunk: no branch around a load, which would make the compiler wait for the others first.)
-template <int DH, int NT = 256>
+template <int DH>
 struct Stage {
+  static constexpr int NT = 256;
   static constexpr int PER = 32 * Geo<DH>::CH, N = (2 * PER + NT - 1) / NT;
   u32x4 r[N];
   unsigned off[N];
@@ -427,34 +428,62 @@ __global__ __launch_bounds__(256, 2) void rel_fwd_kernel(const RelP p) {
   }
 }
 
-// Sums of a 16 x 16 sub-tile of dS along its diagonals.  Lane (g, c) holds distances base + 4 g + r - c, r = 0 .. 3: moving each
-// partial sum one lane on before the next row is added collects a diagonal in one lane without touching memory:
-//   w (lane c): distance base + 4 g + 3 - c;  the three diagonals that leave the 16 lanes come back in lanes 0 .. 2 of the rotated
-// chain, `up`: distance base - 16 + 4 g + 3 - c.  Key tiles are visited in ascending order, so `up` joins the w of the
-// sub-tile before it and a sub-tile costs one LDS add (12 adds a 32 x 32 tile without the folds: 88 us for dQ at B 16, H 10,
-// n 360, dh 80, of which 45 were the adds).
-template <int CTRL>
-DEVINL float dpp_add(float x, float y) {  // x + y moved by CTRL inside rows of 16 lanes, zeros from outside
-  return x + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, y), CTRL, 0xf, 0xf, true));
+// Sums of dS along its diagonals, without atomics.  Of a 16 x 16 sub-tile at base distance d, lane (g, c) holds distances
+// d + 4 g + r - c, r = 0 .. 3.
+//   * Moving each partial sum one lane on before the next row is added collects a diagonal in one lane: w, lane c, distance
+//     d + 4 g + 3 - c.  The three diagonals that leave the 16 lanes come back in lanes 0 .. 2 of the rotated chain: `up`, the same
+//     lanes of the sub-tile at d - 16.
+//   * The four rows of lanes are 4 distances apart: rows 2 and 3 join rows 0 and 1 moved by 8 lanes, row 1 joins row 0 moved by 4;
+//     what leaves on that side belongs to the sub-tile at d + 16.
+// Key tiles are visited in ascending order, so a distance is complete after its two neighbours, and row 0 stores 16 of them at a
+// time, each once per 32 queries.  At B 8, H 12, n 1440, dh 128 dQ takes 735 us with an LDS add per value, 300 with one per
+// folded row (its four rows meet in the same words), 177 without any sums and 214 with this.
+template <int CTRL, int BANKS = 0xf>
+DEVINL float moved(float y) {  // y moved inside rows of 16 lanes; zero from outside and in lanes of other banks of 4
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, y), CTRL, 0xf, BANKS, true));
 }
 DEVINL void fold_diagonals(f32x4 v, float& w, float& up) {
   constexpr int SHR1 = 0x111, ROR1 = 0x121;
-  w = dpp_add<SHR1>(v[3], dpp_add<SHR1>(v[2], dpp_add<SHR1>(v[1], v[0])));
-  up = dpp_add<ROR1>(v[3], dpp_add<ROR1>(v[2], dpp_add<ROR1>(v[1], v[0]))) - w;
+  w = v[3] + moved<SHR1>(v[2] + moved<SHR1>(v[1] + moved<SHR1>(v[0])));
+  up = (v[3] + moved<ROR1>(v[2] + moved<ROR1>(v[1] + moved<ROR1>(v[0])))) - w;
 }
 struct Diagonals {
-  float* bins;   // this wave's sums by distance, at distance 3 + 4 g - c of a sub-tile's base 0
-  f32x4 next;    // sub-tile at base `at` + 16 that the next key tile adds to
-  float w;       // sub-tile at base `at`, without its `up`
+  float* bins;         // this wave's sums by distance, at distance 3 - c
+  int g;
+  f32x4 next;          // sub-tile at base `at` + 16 that the next key tile adds to
+  float w;             // sub-tile at base `at`, without its `up`
+  float over1, over2;  // what rows 2, 3 and row 1 of the sub-tile before left for this one
   int at;
   bool open;
-  DEVINL void add(int base, float x) { atomicAdd(bins + base, x); }
+  DEVINL float join(float x) {
+    constexpr int ROR8 = 0x128, ROR12 = 0x12C;
+    const unsigned u = __builtin_bit_cast(unsigned, x);
+    const auto hi = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    const unsigned h1 = hi[1];
+    const float r = __builtin_bit_cast(float, h1);
+    const float v = x + moved<ROR8, 0x3>(r) + over1;
+    over1 = moved<ROR8, 0xc>(r);
+    const unsigned q = __builtin_bit_cast(unsigned, v);
+    const auto lo = __builtin_amdgcn_permlane16_swap(q, q, false, false);
+    const unsigned l1 = lo[1];
+    const float s = __builtin_bit_cast(float, l1);
+    const float z = v + moved<ROR12, 0x7>(s) + over2;
+    over2 = moved<ROR12, 0x8>(s);
+    return z;
+  }
+  DEVINL void put(int base, float z) {
+    if (g == 0) bins[base] = z;
+  }
+  DEVINL void add(int base, float z) {  // where runs of tiles begin and end, a distance can have been stored already
+    if (g == 0) atomicAdd(bins + base, z);
+  }
   DEVINL void close() {
     if (!open) return;
     float w2, up;
     fold_diagonals(next, w2, up);
-    add(at, w + up);
-    add(at + 16, w2);
+    add(at, join(w + up));
+    add(at + 16, join(w2));
+    add(at + 32, join(0.f));
     open = false;
   }
   // the sub-tiles at bases d0 - 16, d0, d0 + 16
@@ -465,9 +494,14 @@ struct Diagonals {
     if (on) a += next;
     fold_diagonals(a, wa, ua);
     fold_diagonals(b, wb, ub);
-    if (on) add(d0 - 32, w + ua);
-    else add(d0 - 32, ua);
-    add(d0 - 16, wa + ub);
+    if (on) {
+      put(d0 - 32, join(w + ua));
+      put(d0 - 16, join(wa + ub));
+    } else {  // (`ua` reaches into the 16 distances stored before it)
+      over1 = over2 = 0.f;
+      put(d0 - 16, join(wa + ub));
+      atomicAdd(bins + d0 - 32 + 4 * g, ua);
+    }
     w = wb;
     next = c;
     at = d0;
@@ -555,7 +589,9 @@ __global__ __launch_bounds__(256, 2) void rel_dq_kernel(const RelP p) {
     for (int dt = 0; dt < ND; ++dt) dQ[qs][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
   float farl = 0.f, farr = 0.f;
   Diagonals diag;
-  diag.bins = bins + D + PAD + 4 * g + 3 - c;
+  diag.bins = bins + D + PAD + 3 - c;
+  diag.g = g;
+  diag.over1 = diag.over2 = 0.f;
   diag.open = false;
   diag.next = f32x4{0.f, 0.f, 0.f, 0.f};
   diag.w = 0.f;
@@ -738,7 +774,7 @@ __global__ __launch_bounds__(256) void rel_dtable_kernel(const RelP p) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// backward dK / dV: workgroup = 128 keys of one key head, 4 waves x 32 keys; the query tiles of every head that reads them
+// backward dK / dV: workgroup = 128 (64) keys of one key head, 4 waves x 32 (16); the query tiles of every head that reads them
 // are streamed (heads of a group one after another).  A block's stream is cut into `chunks` workgroups where there are too few
 // blocks to fill the chip or a block holds sinks, which all later queries see: their fp32 sums go through the workspace and
 // rel_join_dkdv_kernel adds them in order.
@@ -769,16 +805,19 @@ DEVINL KBlock kblock_of(const RelP& p, int id) {
   return k;
 }
 
-// KS 16-key sub-tiles a wave.  Two (4 waves) let every Q and dO fragment feed two products; dK, dV, K and V of 32 keys do not fit
-// 256 registers at dh 128 (the accumulators then travel through the other half of the register file, 320 moves a tile), so there
-// a wave has one and the workgroup 8 waves.
+// KS 16-key sub-tiles a wave.  Two let every Q and dO fragment feed two products; dK, dV, K and V of 32 keys do not fit 256
+// registers at dh 128 (the accumulators then travel through the other half of the register file, 320 moves a tile: 577 us at
+// B 8, H 12, n 1440), so there a wave has one.
 template <int DH>
 constexpr int key_subs() { return DH > 96 ? 1 : 2; }
+template <int DH>
+constexpr int block_keys() { return 64 * key_subs<DH>(); }
+int block_keys(int dh) { return dh > 96 ? 64 : 128; }
 
 template <int DH, bool REL>
-__global__ __launch_bounds__(512 / key_subs<DH>(), 2) void rel_dkdv_kernel(const RelP p) {
+__global__ __launch_bounds__(256, 2) void rel_dkdv_kernel(const RelP p) {
   using G = Geo<DH>;
-  constexpr int ND = G::ND, KS = key_subs<DH>(), NT = 512 / KS;
+  constexpr int ND = G::ND, KS = key_subs<DH>(), BK = block_keys<DH>();
   extern __shared__ __attribute__((aligned(16))) bf16_t smem[];
   const FactAttention& a = p.a;
   const int D = a.rel_max_distance, NB = 2 * (D + PAD) + 1;
@@ -791,10 +830,10 @@ __global__ __launch_bounds__(512 / key_subs<DH>(), 2) void rel_dkdv_kernel(const
   const int kb = blk.kb, b = blk.bh / a.Hkv, hk = blk.bh - b * a.Hkv;
   const Vis v = vis_of(a, b);
   const int start = start_of(a, b);
-  const int j0 = kb * 128 + wave * 16 * KS;
+  const int j0 = kb * BK + wave * 16 * KS;
   const bool active = j0 < v.len;
   // query rows that see any key of the block: positions [ka - hi, ke - lo], or all later ones if it holds a sink
-  const long long ka = kb * 128, ke = min(kb * 128 + 127, v.len - 1);
+  const long long ka = kb * BK, ke = min(kb * BK + BK - 1, v.len - 1);
   long long qa = v.hi == INT_MAX ? 0 : max(0ll, ka - v.hi - start);
   long long qe = (v.lo == INT_MIN || ka < v.sinks) ? a.nq - 1 : min((long long)a.nq - 1, ke - v.lo - start);
   if (ka >= v.len) qe = -1;
@@ -808,13 +847,13 @@ __global__ __launch_bounds__(512 / key_subs<DH>(), 2) void rel_dkdv_kernel(const
     frag_load<DH>(K[ks], (const bf16_t*)a.k + b * a.k_stride[0] + j * a.k_stride[1] + hk * a.k_stride[2], g);
     frag_load<DH>(V[ks], (const bf16_t*)a.v + b * a.v_stride[0] + j * a.v_stride[1] + hk * a.v_stride[2], g);
   }
-  pad_zero<DH>(smem, 4, tid, NT);
+  pad_zero<DH>(smem, 4, tid, 256);
   f32x4 dK[KS][ND], dV[KS][ND];
 #pragma unroll
   for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
     for (int dt = 0; dt < ND; ++dt) dK[ks][dt] = dV[ks][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
-  Stage<DH, NT> st;
+  Stage<DH> st;
   st.init(a.q_stride[1], a.dout_stride[1], tid);
   float sv = 0.f;
   auto load = [&](int i) {  // i-th tile of the stream: head i / T of the group, query tile t0 + i % T
@@ -835,11 +874,15 @@ __global__ __launch_bounds__(512 / key_subs<DH>(), 2) void rel_dkdv_kernel(const
     store(ib & 1);
     if (ib + 1 < ie) load(ib + 1);
   }
+  int hh = ib < ie ? ib / T : 0, qt = ib - hh * T - 1;
   for (int i = ib; i < ie; ++i) {
-    const int hh = i / T, qt = i - hh * T;
+    if (++qt == T) {
+      qt = 0;
+      ++hh;
+    }
     if (REL && (qt == 0 || i == ib)) {  // the next head's bias: after the last tile of the head before has been read
       __syncthreads();
-      load_bias(eb, p, hk * group + hh, tid, NT);
+      load_bias(eb, p, hk * group + hh, tid, 256);
     }
     __syncthreads();
     if (i + 1 < ie) {
@@ -937,7 +980,7 @@ __global__ __launch_bounds__(512 / key_subs<DH>(), 2) void rel_dkdv_kernel(const
     }
   }
   if (blk.slot >= 0) {
-    f32x4* out = reinterpret_cast<f32x4*>(p.dkv) + ((size_t)blk.slot * 8 + wave * KS) * (2 * ND * 64) + lane;
+    f32x4* out = reinterpret_cast<f32x4*>(p.dkv) + ((size_t)blk.slot * (BK / 16) + wave * KS) * (2 * ND * 64) + lane;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
@@ -970,7 +1013,7 @@ __global__ __launch_bounds__(512 / key_subs<DH>(), 2) void rel_dkdv_kernel(const
 // the chunks of a block, in order: a wave per accumulator fragment (16-key sub-tile, dt, K or V) of the kernel above
 template <int DH>
 __global__ __launch_bounds__(256) void rel_join_dkdv_kernel(const RelP p) {
-  constexpr int ND = Geo<DH>::ND, FR = 8 * 2 * ND;  // fragments of a block
+  constexpr int ND = Geo<DH>::ND, BK = block_keys<DH>(), FR = BK / 16 * 2 * ND;  // fragments of a block
   const FactAttention& a = p.a;
   const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
   const int f = (blockIdx.x * 4 + (threadIdx.x >> 6)) % FR, blk = (blockIdx.x * 4 + (threadIdx.x >> 6)) / FR;
@@ -984,7 +1027,7 @@ __global__ __launch_bounds__(256) void rel_join_dkdv_kernel(const RelP p) {
   f32x4 x = src[0];
   for (int i = 1; i < n; ++i) x += src[(size_t)i * FR * 64];
   const int dt = (f >> 1) % ND, isv = f & 1;
-  const int j = kb * 128 + f / (2 * ND) * 16 + c;
+  const int j = kb * BK + f / (2 * ND) * 16 + c;
   if (j >= a.nk) return;
   const int64_t* st = isv ? a.dv_stride : a.dk_stride;
   const float k = isv ? 1.f : a.scale;
@@ -1274,15 +1317,16 @@ RelP params(const FactAttention& a) {
   p.part = nullptr;
   p.dkv = nullptr;
   // dK / dV: streams of the blocks as long as lengths and positions allow (they are on the device), cut so that the grid fills
-  // 256 CUs twice but no piece is shorter than 4 tiles
+  // 256 CUs twice (three times with blocks of 64 keys) but no piece is shorter than 4 tiles
   const long long group = a.H / a.Hkv, all = ((long long)a.nq + 31) / 32 * group;
-  p.kblocks = (a.nk + 127) / 128;
-  p.sblocks = a.window_left < 0 ? 0 : (std::min(a.sinks, a.nk) + 127) / 128;
+  const int bk = block_keys(a.dh);
+  p.kblocks = (a.nk + bk - 1) / bk;
+  p.sblocks = a.window_left < 0 ? 0 : (std::min(a.sinks, a.nk) + bk - 1) / bk;
   long long seen = a.nq;
   if (a.window_left >= 0 && a.window_right >= 0)
-    seen = std::min<long long>(seen, 128ll + a.window_left + a.window_right + 62);
+    seen = std::min<long long>(seen, (long long)bk + a.window_left + a.window_right + 62);
   const long long t = (seen + 31) / 32 * group, blocks = (long long)a.B * a.Hkv * p.kblocks;
-  p.chunks = (int)std::max(1ll, std::min((512 + blocks / 2) / blocks, t / 4));
+  p.chunks = (int)std::max(1ll, std::min(((bk < 128 ? 768 : 512) + blocks / 2) / blocks, t / 4));
   const long long piece = std::max(8ll, (t + p.chunks - 1) / p.chunks);
   p.schunks = (int)std::max<long long>(p.chunks, std::min(all / piece, 64ll));
   return p;
@@ -1291,7 +1335,7 @@ RelP params(const FactAttention& a) {
 size_t dkv_chunks(const RelP& p) {
   return (p.schunks > 1 ? (size_t)p.sblocks * p.schunks : 0) + (p.chunks > 1 ? (size_t)(p.kblocks - p.sblocks) * p.chunks : 0);
 }
-size_t dkv_bytes(const RelP& p) { return dkv_chunks(p) * p.a.B * p.a.Hkv * 128 * 2 * p.a.dh * 4; }
+size_t dkv_bytes(const RelP& p) { return dkv_chunks(p) * p.a.B * p.a.Hkv * block_keys(p.a.dh) * 2 * p.a.dh * 4; }
 
 // the dQ kernel's partial bias gradients
 size_t part_bytes(const FactAttention& a) {
@@ -1335,9 +1379,9 @@ int bwd_t(const FactAttention& a, void* ws, hipStream_t s) {
   FACT_LAUNCH((rel_dq_kernel<DH, REL>), dim3(p.nwg), dim3(256), lds1, s, p);
   if (REL) FACT_LAUNCH(rel_dtable_kernel, dim3(a.H, a.rel_buckets), dim3(256), 0, s, p);
   p.nwg = (p.sblocks * p.schunks + (p.kblocks - p.sblocks) * p.chunks) * a.B * a.Hkv;
-  FACT_LAUNCH((rel_dkdv_kernel<DH, REL>), dim3(p.nwg), dim3(512 / key_subs<DH>()), lds2, s, p);
+  FACT_LAUNCH((rel_dkdv_kernel<DH, REL>), dim3(p.nwg), dim3(256), lds2, s, p);
   const int joined = ((p.schunks > 1 ? p.sblocks : 0) + (p.chunks > 1 ? p.kblocks - p.sblocks : 0)) * a.B * a.Hkv;
-  if (joined) FACT_LAUNCH(rel_join_dkdv_kernel<DH>, dim3(joined * 4 * Geo<DH>::ND), dim3(256), 0, s, p);
+  if (joined) FACT_LAUNCH(rel_join_dkdv_kernel<DH>, dim3(joined * (block_keys<DH>() / 32) * Geo<DH>::ND), dim3(256), 0, s, p);
   return launched();
 }
 
@@ -1368,7 +1412,7 @@ int rel_attention_check(const FactAttention& a, bool backward, const char** why)
   if (a.dh != 32 && a.dh != 64 && a.dh != 80 && a.dh != 96 && a.dh != 128)
     return bad(-3, "unsupported head dim (supported: 32, 64, 80, 96, 128)");
   if ((long long)a.B * a.H > INT_MAX / 256 || ((long long)a.nq + 127) / 128 * a.B * a.H > INT_MAX / 4 ||
-      ((long long)a.nk + 127) / 128 * a.B * a.Hkv > INT_MAX / 512)
+      ((long long)a.nk + 63) / 64 * a.B * a.Hkv > INT_MAX / 512)
     return bad(-1, "too many heads and blocks for one launch");
   if (!(a.scale >= 5.9604645e-8f) || !(a.scale <= 3.0e38f)) return bad(-1, "scale must be finite and at least 2^-24");
   if (a.sinks < 0) return bad(-1, "sinks must not be negative");
