@@ -29,7 +29,7 @@ struct RelP {
   int rowtab;     // few rows: the bias of the group's heads fits the workgroup's memory
   int kblocks, sblocks, chunks, schunks;  // dK / dV: 128-key blocks, the first of them with sinks, workgroups of a block
   float* dkv;     // partial dK, dV of blocks with several workgroups
-  float* dsum;    // [B][H][nq] rowsum(dO . O)
+  float* dsum;    // [B][H][nq] -rowsum(dO . O)
   float* part;    // per-workgroup bias gradients [B * H * qblocks][2 D + 1] / partial rows of the few-row kernel
 };
 
@@ -38,9 +38,27 @@ struct Geo {
   static constexpr int ND = DH / 16;        // 16-wide head-dim tiles
   static constexpr int KD = (DH + 31) / 32; // 32-deep contraction steps over the head dim
   static constexpr int CH = DH / 8;         // 16-byte chunks of a row
-  static constexpr int KP = KD * 32 + 8;    // LDS row pitch (elements): 16 consecutive rows start in different banks
-  static constexpr int IMG = 32 * KP;       // one 32-row tile
+  static constexpr int PC = KD * 4;         // chunks of a row in LDS
+  static constexpr int IMG = 32 * PC * 8;   // one 32-row tile (elements)
 };
+// LDS tiles have no gaps (they are filled 64 chunks at a time); a row's chunks are permuted instead.  In units of 16 bytes, modulo
+// the 16 that all banks hold, the 16 rows of a fragment read start PC apart; what is left to tell apart are rows with the same
+// PC r mod 16, and the chunk's low bits do that.  8 rows of a transposed read, two chunks of each, differ in the other bits.
+template <int DH>
+struct Swizzle {
+  static constexpr int FREE = Geo<DH>::PC == 16 ? 0 : Geo<DH>::PC == 8 ? 1 : 2;  // rows' low bits that PC r tells apart
+  static constexpr int MASK = (16 >> FREE) - 1;
+};
+template <int DH>
+DEVINL int place(int row, int ch) {  // element of chunk ch of a row
+  constexpr int FREE = Swizzle<DH>::FREE, MASK = Swizzle<DH>::MASK;
+  const int sw = ((row & 7) >> FREE << 1 | (row >> 3 & 1)) & MASK;
+  return (row * Geo<DH>::PC + (ch & ~MASK) + ((ch & MASK) ^ sw)) * 8;
+}
+template <int DH>
+DEVINL int further(int at, int chunks) {  // place<DH>(row, ch + chunks) from place<DH>(row, ch); no bit is in both ch and chunks
+  return (at ^ ((chunks & Swizzle<DH>::MASK) * 8)) + (chunks & ~Swizzle<DH>::MASK) * 8;
+}
 
 // one operand fragment set over the head dim: rows of 16 tokens
 template <int DH>
@@ -55,10 +73,21 @@ DEVINL void frag_load(Frag<DH>& r, const bf16_t* row, int g) {  // `row`: this l
     if (kd * 32 + 32 <= DH || kd * 32 + g * 8 < DH) r.f[kd] = *reinterpret_cast<const bf16x8*>(row + kd * 32 + g * 8);
   }
 }
+// where a lane's fragments begin in an LDS tile: by rows (row c, chunk g), and through the transpose read
 template <int DH>
-DEVINL void frag_lds(Frag<DH>& r, const bf16_t* row, int g) {  // an LDS row: its padding columns are zero
+struct Lane {
+  int rows, tr;
+  DEVINL void init(int lane) {
+    const int g = lane >> 4, s = lane & 15;
+    rows = place<DH>(s, g);
+    tr = place<DH>(g * 4 + (s >> 2), s >> 1 & 1) + (s & 1) * 4;
+  }
+};
+template <int DH>
+DEVINL void frag_lds(Frag<DH>& r, const bf16_t* tile, int sub, int rows) {  // row 16 sub + c
 #pragma unroll
-  for (int kd = 0; kd < Geo<DH>::KD; ++kd) r.f[kd] = *reinterpret_cast<const bf16x8*>(row + kd * 32 + g * 8);
+  for (int kd = 0; kd < Geo<DH>::KD; ++kd)
+    r.f[kd] = *reinterpret_cast<const bf16x8*>(tile + sub * (Geo<DH>::IMG / 2) + further<DH>(rows, kd * 4));
 }
 template <int DH>
 DEVINL f32x4 frag_dot(const Frag<DH>& a, const Frag<DH>& b, f32x4 c) {
@@ -66,13 +95,15 @@ DEVINL f32x4 frag_dot(const Frag<DH>& a, const Frag<DH>& b, f32x4 c) {
   for (int kd = 0; kd < Geo<DH>::KD; ++kd) c = mfma16(a.f[kd], b.f[kd], c);
   return c;
 }
-// zeros into the padding columns of `tiles` LDS tiles, once per workgroup
+// zeros into the padding columns of two LDS tiles, once per workgroup
 template <int DH>
-DEVINL void pad_zero(bf16_t* lds, int tiles, int tid, int nthr) {
-  if constexpr (DH % 32 != 0) {
-    constexpr int PC = (Geo<DH>::KD * 32 - DH) / 8;
-    for (int i = tid; i < tiles * 32 * PC; i += nthr)
-      *reinterpret_cast<u32x4*>(lds + (i / PC) * Geo<DH>::KP + DH + (i % PC) * 8) = u32x4{0u, 0u, 0u, 0u};
+DEVINL void pad_zero(bf16_t* lds, int tid) {
+  using G = Geo<DH>;
+  if constexpr (G::PC != G::CH) {
+    for (int i = tid; i < 64 * (G::PC - G::CH); i += 256) {
+      const int r = i / (G::PC - G::CH);
+      *reinterpret_cast<u32x4*>(lds + r / 32 * G::IMG + place<DH>(r % 32, G::CH + i % (G::PC - G::CH))) = u32x4{0u, 0u, 0u, 0u};
+    }
   }
 }
 
@@ -82,11 +113,10 @@ DEVINL bf16x8 pack8(f32x4 a, f32x4 b) {
 }
 // A operand [16 dims of tile dt][32 tokens] of a row-major LDS tile, token slots as in the header comment
 template <int DH>
-DEVINL bf16x8 frag_tr(const bf16_t* t, int dt, int lane) {
-  const int g = lane >> 4, s = lane & 15;
-  const bf16_t* p = t + (g * 4 + (s >> 2)) * Geo<DH>::KP + dt * 16 + (s & 3) * 4;
+DEVINL bf16x8 frag_tr(const bf16_t* t, int dt, int tr) {
+  const bf16_t* p = t + further<DH>(tr, dt * 2);
   const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)p);
-  const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(p + 16 * Geo<DH>::KP));
+  const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(p + Geo<DH>::IMG / 2));
   return cat4(lo, hi);
 }
 
@@ -182,53 +212,58 @@ DEVINL u32x4 load16(const bf16_t* base, unsigned off) {
   return *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(base) + off);
 }
 
-// ---- staging of two 32-row tiles (K and V, or Q and dO) through registers into LDS -------------------------------------
-// A thread moves chunks tid, tid + NT, ...; a wave's 64 chunks lie in one image.  (Threads past the end of an uneven list repeat
-// the last chunk: no branch around a load, which would make the compiler wait for the others first.)
+// ---- staging of two 32-row tiles (K and V, or Q and dO) into LDS --------------------------------------------------------
+// Loads that write LDS themselves, 16 bytes a lane and 64 consecutive places of a tile an instruction: no registers hold what is
+// in flight.  Each wave waits for its own before the barrier (__syncthreads alone does not).  The two buffers of a kernel are two objects, each named by half of the
+// unrolled loop: of one array with a computed half the compiler would wait for the loads in flight before each read.
+typedef __attribute__((address_space(3))) void lds_void;
+typedef __attribute__((address_space(1))) const void glb_void;
 template <int DH>
 struct Stage {
-  static constexpr int NT = 256;
-  static constexpr int PER = 32 * Geo<DH>::CH, N = (2 * PER + NT - 1) / NT;
-  u32x4 r[N];
+  using G = Geo<DH>;
+  static constexpr int PER = 32 * G::PC / 64, N = PER / 2;  // instructions of a tile; of both tiles and one of the 4 waves
   unsigned off[N];
-  int row[N], dst[N];
   unsigned lda, ldb;  // bytes
-  unsigned second;    // bit i: chunk i of this wave lies in the second image
-  DEVINL void init(long long a, long long b, int tid) {
+  int wave, lane;
+  DEVINL int tile(int i) const { return i * 4 + wave < PER ? i * 4 + wave : i * 4 + wave - PER; }
+  DEVINL int row(int i) const { return (tile(i) * 64 + lane) / G::PC; }
+  DEVINL int chunk(int i) const {  // (the permutation is its own inverse)
+    const int n = tile(i) * 64 + lane, r = n / G::PC;
+    return place<DH>(r, n - r * G::PC) / 8 - r * G::PC;
+  }
+  DEVINL void init(long long a, long long b, int w, int l) {
     lda = (unsigned)a * 2;
     ldb = (unsigned)b * 2;
-    second = 0;
+    wave = w;
+    lane = l;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int c = min(tid + i * NT, 2 * PER - 1);
-      const int im = __builtin_amdgcn_readfirstlane(c / PER), q = c - im * PER;
-      row[i] = q / Geo<DH>::CH;
-      const int ch = q - row[i] * Geo<DH>::CH;
-      second |= (unsigned)im << i;
-      off[i] = (unsigned)row[i] * (im ? ldb : lda) + ch * 16;
-      dst[i] = im * Geo<DH>::IMG + row[i] * Geo<DH>::KP + ch * 8;
-    }
+    for (int i = 0; i < N; ++i) off[i] = (unsigned)row(i) * (i * 4 + wave < PER ? lda : ldb) + chunk(i) * 16;
   }
   // rows row0 .. row0 + 31 of a and b (wave-uniform pointers to row 0); rows past `last` repeat it: finite values, masked later
-  DEVINL void load(const bf16_t* a, const bf16_t* b, int row0, int last) {
+  DEVINL void load(bf16_t* lds, const bf16_t* a, const bf16_t* b, int row0, int last) const {
     a += (long long)row0 * (lda / 2);
     b += (long long)row0 * (ldb / 2);
-    if (row0 + 31 <= last) {
+    const int in = last - row0;
+    if (in >= 31) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) r[i] = load16((second >> i) & 1 ? b : a, off[i]);
+      for (int i = 0; i < N; ++i) one(lds, a, b, i, off[i]);
     } else {
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const unsigned past = (unsigned)max(0, row0 + row[i] - last);
-        r[i] = load16((second >> i) & 1 ? b : a, off[i] - past * ((second >> i) & 1 ? ldb : lda));
-      }
+      for (int i = 0; i < N; ++i) one(lds, a, b, i, off[i] - (unsigned)max(0, row(i) - in) * (i * 4 + wave < PER ? lda : ldb));
     }
   }
-  DEVINL void store(bf16_t* lds) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) *reinterpret_cast<u32x4*>(lds + dst[i]) = r[i];
+  DEVINL void one(bf16_t* lds, const bf16_t* a, const bf16_t* b, int i, unsigned o) const {
+    const int k = i * 4 + wave;
+    const char* src = reinterpret_cast<const char*>(k < PER ? a : b);
+    if (G::PC == G::CH || chunk(i) < G::CH)
+      __builtin_amdgcn_global_load_lds((glb_void*)(src + o), (lds_void*)(lds + k * 512), 16, 0, 0);
   }
 };
+
+DEVINL void staged() {
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+  __syncthreads();
+}
 
 // bias of head h for distances -(D + PAD) .. D + PAD, divided by scale
 DEVINL void load_bias(float* eb, const RelP& p, int h, int tid, int nthr) {
@@ -250,8 +285,8 @@ template <int DH, bool REL, bool EXACT>
 __global__ __launch_bounds__(256, 2) void rel_fwd_kernel(const RelP p) {
   using G = Geo<DH>;
   constexpr int ND = G::ND;
-  extern __shared__ __attribute__((aligned(16))) bf16_t smem[];
-  float* eb = reinterpret_cast<float*>(smem + 4 * G::IMG);
+  __shared__ __attribute__((aligned(16))) bf16_t buf0[2 * G::IMG], buf1[2 * G::IMG];
+  extern __shared__ float eb[];
   const FactAttention& a = p.a;
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, c = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -269,11 +304,15 @@ __global__ __launch_bounds__(256, 2) void rel_fwd_kernel(const RelP p) {
   for (int qs = 0; qs < 2; ++qs)
     frag_load<DH>(Q[qs], (const bf16_t*)a.q + b * a.q_stride[0] + (long long)min(q0 + qs * 16 + c, a.nq - 1) * a.q_stride[1] +
                              h * a.q_stride[2], g);
+  Lane<DH> at;
+  at.init(lane);
   Stage<DH> st;
   const bf16_t* kp = (const bf16_t*)a.k + b * a.k_stride[0] + hk * a.k_stride[2];
   const bf16_t* vp = (const bf16_t*)a.v + b * a.v_stride[0] + hk * a.v_stride[2];
-  st.init(a.k_stride[1], a.v_stride[1], tid);
-  pad_zero<DH>(smem, 4, tid, 256);
+  st.init(a.k_stride[1], a.v_stride[1], wave, lane);
+  pad_zero<DH>(buf0, tid);
+  pad_zero<DH>(buf1, tid);
+  if (tl.T > 0) st.load(buf0, kp, vp, tl.at(0) * 32, v.len - 1);
   if (REL) load_bias(eb, p, h, tid, 256);
   f32x4 O[2][ND];
   float m[2], l[2];
@@ -284,24 +323,13 @@ __global__ __launch_bounds__(256, 2) void rel_fwd_kernel(const RelP p) {
 #pragma unroll
     for (int dt = 0; dt < ND; ++dt) O[qs][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  if (tl.T > 0) {
-    st.load(kp, vp, tl.at(0) * 32, v.len - 1);
-    st.store(smem);
-    if (tl.T > 1) st.load(kp, vp, tl.at(1) * 32, v.len - 1);
-  }
   const int D = a.rel_max_distance;
-  for (int t = 0; t < tl.T; ++t) {
-    __syncthreads();
-    if (t + 1 < tl.T) {
-      st.store(smem + ((t + 1) & 1) * 2 * G::IMG);
-      if (t + 2 < tl.T) st.load(kp, vp, tl.at(t + 2) * 32, v.len - 1);
-    }
-    const int j0 = tl.at(t) * 32;
-    if (!active || v.none(j0, p0)) continue;
-    const bf16_t* Ks = smem + (t & 1) * 2 * G::IMG;
+  auto step = [&](int t, const bf16_t* Ks, bf16_t* other) __attribute__((always_inline)) {
     const bf16_t* Vs = Ks + G::IMG;
+    const int j0 = tl.at(t) * 32;
+    const bool skip = !active || v.none(j0, p0);
     f32x4 s[2][2];  // [key sub-tile][query sub-tile]
-    if (REL) {
+    if (REL && !skip) {
       const int d0 = j0 - p0;  // distance of the tile's first key and the wave's first query
       if (d0 - 31 >= D || d0 + 31 <= -D) {
         const float f = eb[d0 > 0 ? 2 * (D + PAD) : 0];
@@ -324,10 +352,12 @@ __global__ __launch_bounds__(256, 2) void rel_fwd_kernel(const RelP p) {
 #pragma unroll
         for (int qs = 0; qs < 2; ++qs) s[ks][qs] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
+    if (t + 1 < tl.T) st.load(other, kp, vp, tl.at(t + 1) * 32, v.len - 1);  // (after the reads of the bias: they would wait for it)
+    if (skip) return;
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
       Frag<DH> K;
-      frag_lds<DH>(K, Ks + (ks * 16 + c) * G::KP, g);
+      frag_lds<DH>(K, Ks, ks, at.rows);
 #pragma unroll
       for (int qs = 0; qs < 2; ++qs) s[ks][qs] = frag_dot<DH>(K, Q[qs], s[ks][qs]);
     }
@@ -392,7 +422,7 @@ __global__ __launch_bounds__(256, 2) void rel_fwd_kernel(const RelP p) {
     }
 #pragma unroll
     for (int dt = 0; dt < ND; ++dt) {
-      const bf16x8 vf = frag_tr<DH>(Vs, dt, lane);
+      const bf16x8 vf = frag_tr<DH>(Vs, dt, at.tr);
 #pragma unroll
       for (int qs = 0; qs < 2; ++qs) {
         O[qs][dt] = mfma16(vf, pb[qs], O[qs][dt]);
@@ -402,6 +432,14 @@ __global__ __launch_bounds__(256, 2) void rel_fwd_kernel(const RelP p) {
         }
       }
     }
+  };
+  for (int t = 0; t < tl.T;) {
+    staged();
+    step(t, buf0, buf1);
+    if (++t == tl.T) break;
+    staged();
+    step(t, buf1, buf0);
+    ++t;
   }
   if (!active) return;
 #pragma unroll
@@ -517,10 +555,10 @@ template <int DH, bool REL>
 __global__ __launch_bounds__(256, 2) void rel_dq_kernel(const RelP p) {
   using G = Geo<DH>;
   constexpr int ND = G::ND;
-  extern __shared__ __attribute__((aligned(16))) bf16_t smem[];
+  __shared__ __attribute__((aligned(16))) bf16_t buf0[2 * G::IMG], buf1[2 * G::IMG];
+  extern __shared__ float eb[];
   const FactAttention& a = p.a;
   const int D = a.rel_max_distance, NB = 2 * (D + PAD) + 1;
-  float* eb = reinterpret_cast<float*>(smem + 4 * G::IMG);
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, c = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   float* bins = eb + NB * (1 + wave);  // this wave's bias gradient by distance: its own, so sums have one order
@@ -533,11 +571,15 @@ __global__ __launch_bounds__(256, 2) void rel_dq_kernel(const RelP p) {
   const bool active = q0 < a.nq;
   const Tiles tl = tiles_of(v, (long long)start + qb * 128, (long long)start + min(qb * 128 + 127, a.nq - 1));
 
+  Lane<DH> at;
+  at.init(lane);
   Stage<DH> st;
   const bf16_t* kp = (const bf16_t*)a.k + b * a.k_stride[0] + hk * a.k_stride[2];
   const bf16_t* vp = (const bf16_t*)a.v + b * a.v_stride[0] + hk * a.v_stride[2];
-  st.init(a.k_stride[1], a.v_stride[1], tid);
-  if (tl.T > 0) st.load(kp, vp, tl.at(0) * 32, v.len - 1);
+  st.init(a.k_stride[1], a.v_stride[1], wave, lane);
+  pad_zero<DH>(buf0, tid);
+  pad_zero<DH>(buf1, tid);
+  if (tl.T > 0) st.load(buf0, kp, vp, tl.at(0) * 32, v.len - 1);
   Frag<DH> Q[2], dO[2];
   float nL[2], nD[2];
   bool live[2];  // a query of the call that sees more than one key
@@ -579,9 +621,8 @@ __global__ __launch_bounds__(256, 2) void rel_dq_kernel(const RelP p) {
       for (int kd = 0; kd < G::KD; ++kd)
         dO[qs].f[kd] = __builtin_bit_cast(bf16x8, __builtin_bit_cast(u32x4, dO[qs].f[kd]) ^ 0x80008000u);
     }
-    if (active && g == 0) p.dsum[at] = part;  // for the dK / dV kernel (repeated rows write the same value)
+    if (active && g == 0) p.dsum[at] = -part;  // for the dK / dV kernel (repeated rows write the same value)
   }
-  pad_zero<DH>(smem, 4, tid, 256);
   f32x4 dQ[2][ND];
 #pragma unroll
   for (int qs = 0; qs < 2; ++qs)
@@ -600,24 +641,15 @@ __global__ __launch_bounds__(256, 2) void rel_dq_kernel(const RelP p) {
     load_bias(eb, p, h, tid, 256);
     for (int i = lane; i < NB; i += 64) bins[i] = 0.f;
   }
-  if (tl.T > 0) {
-    st.store(smem);
-    if (tl.T > 1) st.load(kp, vp, tl.at(1) * 32, v.len - 1);
-  }
-  for (int t = 0; t < tl.T; ++t) {
-    __syncthreads();
-    if (t + 1 < tl.T) {
-      st.store(smem + ((t + 1) & 1) * 2 * G::IMG);
-      if (t + 2 < tl.T) st.load(kp, vp, tl.at(t + 2) * 32, v.len - 1);
-    }
-    const int j0 = tl.at(t) * 32;
-    if (!active || v.none(j0, p0)) continue;
-    const bf16_t* Ks = smem + (t & 1) * 2 * G::IMG;
+  auto step = [&](int t, const bf16_t* Ks, bf16_t* other) __attribute__((always_inline)) {
     const bf16_t* Vs = Ks + G::IMG;
+    const int j0 = tl.at(t) * 32;
+    const bool skip = !active || v.none(j0, p0);
+    if (REL && DH > 96) asm("" : "+v"(at.tr));  // 8 offsets made from it each tile: kept, they do not fit 256 registers
     f32x4 s[2][2], dp[2][2];
     const int d0 = j0 - p0;
     const bool left = REL && d0 + 31 <= -D, right = REL && d0 - 31 >= D;
-    if (REL) {
+    if (REL && !skip) {
       if (left || right) {
         const float f = eb[right ? NB - 1 : 0];
 #pragma unroll
@@ -639,11 +671,13 @@ __global__ __launch_bounds__(256, 2) void rel_dq_kernel(const RelP p) {
 #pragma unroll
         for (int qs = 0; qs < 2; ++qs) s[ks][qs] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
+    if (t + 1 < tl.T) st.load(other, kp, vp, tl.at(t + 1) * 32, v.len - 1);  // (after the reads of the bias: they would wait for it)
+    if (skip) return;
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
       Frag<DH> K, V;
-      frag_lds<DH>(K, Ks + (ks * 16 + c) * G::KP, g);
-      frag_lds<DH>(V, Vs + (ks * 16 + c) * G::KP, g);
+      frag_lds<DH>(K, Ks, ks, at.rows);
+      frag_lds<DH>(V, Vs, ks, at.rows);
 #pragma unroll
       for (int qs = 0; qs < 2; ++qs) {
         dp[ks][qs] = f32x4{nD[qs], nD[qs], nD[qs], nD[qs]};
@@ -668,6 +702,15 @@ __global__ __launch_bounds__(256, 2) void rel_dq_kernel(const RelP p) {
           for (int r = 0; r < 4; ++r)
             ds[ks][qs][r] = (v.seen(j0 + ks * 16 + 4 * g + r, p0 + qs * 16 + c) & live[qs]) ? ds[ks][qs][r] : 0.f;
     }
+    bf16x8 dsb[2];
+#pragma unroll
+    for (int qs = 0; qs < 2; ++qs) dsb[qs] = pack8(ds[0][qs], ds[1][qs]);
+#pragma unroll
+    for (int dt = 0; dt < ND; ++dt) {
+      const bf16x8 kf = frag_tr<DH>(Ks, dt, at.tr);
+#pragma unroll
+      for (int qs = 0; qs < 2; ++qs) dQ[qs][dt] = mfma16(kf, dsb[qs], dQ[qs][dt]);
+    }
     if (REL) {
       if (left || right) {
         float x = 0.f;
@@ -679,15 +722,14 @@ __global__ __launch_bounds__(256, 2) void rel_dq_kernel(const RelP p) {
         diag.tile(d0, -ds[0][1], ds[0][0] - ds[1][1], ds[1][0]);
       }
     }
-    bf16x8 dsb[2];
-#pragma unroll
-    for (int qs = 0; qs < 2; ++qs) dsb[qs] = pack8(ds[0][qs], ds[1][qs]);
-#pragma unroll
-    for (int dt = 0; dt < ND; ++dt) {
-      const bf16x8 kf = frag_tr<DH>(Ks, dt, lane);
-#pragma unroll
-      for (int qs = 0; qs < 2; ++qs) dQ[qs][dt] = mfma16(kf, dsb[qs], dQ[qs][dt]);
-    }
+  };
+  for (int t = 0; t < tl.T;) {
+    staged();
+    step(t, buf0, buf1);
+    if (++t == tl.T) break;
+    staged();
+    step(t, buf1, buf0);
+    ++t;
   }
   if (active) {
 #pragma unroll
@@ -815,14 +857,13 @@ constexpr int block_keys() { return 64 * key_subs<DH>(); }
 int block_keys(int dh) { return dh > 96 ? 64 : 128; }
 
 template <int DH, bool REL>
-__global__ __launch_bounds__(256, 2) void rel_dkdv_kernel(const RelP p) {
+__global__ __launch_bounds__(256, DH > 96 ? 3 : 2) void rel_dkdv_kernel(const RelP p) {
   using G = Geo<DH>;
   constexpr int ND = G::ND, KS = key_subs<DH>(), BK = block_keys<DH>();
-  extern __shared__ __attribute__((aligned(16))) bf16_t smem[];
+  __shared__ __attribute__((aligned(16))) bf16_t buf0[2 * G::IMG + 128], buf1[2 * G::IMG + 128];  // Q, dO, fp32 L and -D
+  extern __shared__ float eb[];
   const FactAttention& a = p.a;
   const int D = a.rel_max_distance, NB = 2 * (D + PAD) + 1;
-  float* stat = reinterpret_cast<float*>(smem + 4 * G::IMG);  // [2][64]: -L, -D of the tile's queries
-  float* eb = stat + 128;
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, c = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int group = a.H / a.Hkv;
@@ -847,55 +888,42 @@ __global__ __launch_bounds__(256, 2) void rel_dkdv_kernel(const RelP p) {
     frag_load<DH>(K[ks], (const bf16_t*)a.k + b * a.k_stride[0] + j * a.k_stride[1] + hk * a.k_stride[2], g);
     frag_load<DH>(V[ks], (const bf16_t*)a.v + b * a.v_stride[0] + j * a.v_stride[1] + hk * a.v_stride[2], g);
   }
-  pad_zero<DH>(smem, 4, tid, 256);
+  pad_zero<DH>(buf0, tid);
+  pad_zero<DH>(buf1, tid);
   f32x4 dK[KS][ND], dV[KS][ND];
 #pragma unroll
   for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
     for (int dt = 0; dt < ND; ++dt) dK[ks][dt] = dV[ks][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  Lane<DH> at;
+  at.init(lane);
   Stage<DH> st;
-  st.init(a.q_stride[1], a.dout_stride[1], tid);
-  float sv = 0.f;
-  auto load = [&](int i) {  // i-th tile of the stream: head i / T of the group, query tile t0 + i % T
-    const int hh = i / T, h = hk * group + hh, q0 = (t0 + i - hh * T) * 32;
-    st.load((const bf16_t*)a.q + b * a.q_stride[0] + h * a.q_stride[2],
+  st.init(a.q_stride[1], a.dout_stride[1], wave, lane);
+  auto load = [&](int hh, int qt, bf16_t* buf) __attribute__((always_inline)) {  // head hh of the group, its query tile t0 + qt
+    const int h = hk * group + hh, q0 = (t0 + qt) * 32;
+    st.load(buf, (const bf16_t*)a.q + b * a.q_stride[0] + h * a.q_stride[2],
             (const bf16_t*)a.dout + b * a.dout_stride[0] + h * a.dout_stride[2], q0, a.nq - 1);
-    if (tid < 64) {
-      const size_t at = ((size_t)b * a.H + h) * a.nq + min(q0 + (tid & 31), a.nq - 1);
-      sv = tid < 32 ? -a.lse[at] : -p.dsum[at];
+    if (wave == 0) {
+      const size_t at = ((size_t)b * a.H + h) * a.nq + min(q0 + (lane & 31), a.nq - 1);
+      __builtin_amdgcn_global_load_lds((glb_void*)((lane < 32 ? a.lse : p.dsum) + at), (lds_void*)(buf + 2 * G::IMG), 4, 0, 0);
     }
   };
-  auto store = [&](int buf) {
-    st.store(smem + buf * 2 * G::IMG);
-    if (tid < 64) stat[buf * 64 + tid] = sv;
-  };
-  if (ib < ie) {
-    load(ib);
-    store(ib & 1);
-    if (ib + 1 < ie) load(ib + 1);
-  }
-  int hh = ib < ie ? ib / T : 0, qt = ib - hh * T - 1;
-  for (int i = ib; i < ie; ++i) {
-    if (++qt == T) {
-      qt = 0;
-      ++hh;
-    }
+  int hh = ib < ie ? ib / T : 0, qt = ib - hh * T;
+  if (ib < ie) load(hh, qt, buf0);
+  auto step = [&](int i, const bf16_t* Qs, bf16_t* other) __attribute__((always_inline)) {
     if (REL && (qt == 0 || i == ib)) {  // the next head's bias: after the last tile of the head before has been read
       __syncthreads();
       load_bias(eb, p, hk * group + hh, tid, 256);
     }
-    __syncthreads();
-    if (i + 1 < ie) {
-      store((i + 1) & 1);
-      if (i + 2 < ie) load(i + 2);
-    }
-    const int q0 = (t0 + qt) * 32, p0 = start + q0;
-    if (!active || v.none<16 * KS>(j0, p0)) continue;
-    const bf16_t* Qs = smem + (i & 1) * 2 * G::IMG;
+    staged();
     const bf16_t* Os = Qs + G::IMG;
-    const float* sl = stat + (i & 1) * 64;
+    const float* sl = reinterpret_cast<const float*>(Qs + 2 * G::IMG);
+    const int q0 = (t0 + qt) * 32, p0 = start + q0;
+    if (DH > 96) asm("" : "+v"(at.tr));  // offsets made from them each tile: kept, they do not fit the registers of 3 waves
+    if (REL && DH > 96) asm("" : "+v"(at.rows));
+    const bool skip = !active || v.none<16 * KS>(j0, p0);
     f32x4 s[2][KS], dp[2][KS];  // [query sub-tile][key sub-tile]: lane = key c, queries 4 g .. 4 g + 3
-    if (REL) {
+    if (REL && !skip) {
       const int d0 = j0 - p0;
       if (d0 - 31 >= D || d0 + 16 * KS - 1 <= -D) {
         const float f = eb[d0 > 0 ? NB - 1 : 0];
@@ -921,14 +949,20 @@ __global__ __launch_bounds__(256, 2) void rel_dkdv_kernel(const RelP p) {
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) s[qs][ks] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    f32x4 nl[2], nd[2];
+    if (++qt == T) {
+      qt = 0;
+      ++hh;
+    }
+    if (i + 1 < ie) load(hh, qt, other);  // (after the reads of the bias: they would wait for it)
+    if (skip) return;
+    f32x4 L[2], nd[2];
 #pragma unroll
     for (int qs = 0; qs < 2; ++qs) {
-      nl[qs] = *reinterpret_cast<const f32x4*>(sl + qs * 16 + g * 4);
+      L[qs] = *reinterpret_cast<const f32x4*>(sl + qs * 16 + g * 4);
       nd[qs] = *reinterpret_cast<const f32x4*>(sl + 32 + qs * 16 + g * 4);
       Frag<DH> Q, dO;
-      frag_lds<DH>(Q, Qs + (qs * 16 + c) * G::KP, g);
-      frag_lds<DH>(dO, Os + (qs * 16 + c) * G::KP, g);
+      frag_lds<DH>(Q, Qs, qs, at.rows);
+      frag_lds<DH>(dO, Os, qs, at.rows);
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         s[qs][ks] = frag_dot<DH>(Q, K[ks], s[qs][ks]);
@@ -942,7 +976,7 @@ __global__ __launch_bounds__(256, 2) void rel_dkdv_kernel(const RelP p) {
       for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          pr[qs][ks][r] = __builtin_amdgcn_exp2f(fmaf(s[qs][ks][r], p.sc, nl[qs][r]));
+          pr[qs][ks][r] = __builtin_amdgcn_exp2f(fmaf(s[qs][ks][r], p.sc, -L[qs][r]));
           dp[qs][ks][r] *= pr[qs][ks][r];
         }
     if (!v.full<16 * KS>(j0, p0) || q0 + 31 >= a.nq) {
@@ -970,14 +1004,20 @@ __global__ __launch_bounds__(256, 2) void rel_dkdv_kernel(const RelP p) {
     }
 #pragma unroll
     for (int dt = 0; dt < ND; ++dt) {
-      const bf16x8 of = frag_tr<DH>(Os, dt, lane);
-      const bf16x8 qf = frag_tr<DH>(Qs, dt, lane);
+      const bf16x8 of = frag_tr<DH>(Os, dt, at.tr);
+      const bf16x8 qf = frag_tr<DH>(Qs, dt, at.tr);
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         dV[ks][dt] = mfma16(of, pb[ks], dV[ks][dt]);
         dK[ks][dt] = mfma16(qf, db[ks], dK[ks][dt]);
       }
     }
+  };
+  for (int i = ib; i < ie;) {
+    step(i, buf0, buf1);
+    if (++i == ie) break;
+    step(i, buf1, buf0);
+    ++i;
   }
   if (blk.slot >= 0) {
     f32x4* out = reinterpret_cast<f32x4*>(p.dkv) + ((size_t)blk.slot * (BK / 16) + wave * KS) * (2 * ND * 64) + lane;
@@ -1055,7 +1095,8 @@ __global__ __launch_bounds__(256, 2) void rel_rows_kernel(const RelP p) {
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, c = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   // key heads of one range of tokens beside each other on one XCD: their rows share cache lines
-    const int id = p.splits > 1 ? (int)blockIdx.x : xcd_order(blockIdx.x, p.nwg), bs = id / a.Hkv, hk = id - bs * a.Hkv, b = bs / p.splits, split = bs - b * p.splits;
+  const int id = p.splits > 1 ? (int)blockIdx.x : xcd_order(blockIdx.x, p.nwg);
+  const int bs = id / a.Hkv, hk = id - bs * a.Hkv, b = bs / p.splits, split = bs - b * p.splits;
   const int group = a.H / a.Hkv, R = group * a.nq;
   const Vis v = vis_of(a, b);
   const int start = start_of(a, b);
@@ -1068,6 +1109,8 @@ __global__ __launch_bounds__(256, 2) void rel_rows_kernel(const RelP p) {
   const bf16_t* kb = (const bf16_t*)a.k + b * a.k_stride[0] + hk * a.k_stride[2];
   const bf16_t* vb = (const bf16_t*)a.v + b * a.v_stride[0] + hk * a.v_stride[2];
   bf16_t* Vs = reinterpret_cast<bf16_t*>(smem) + wave * G::IMG;
+  Lane<DH> at;
+  at.init(lane);
   const int D = a.rel_max_distance, n = 2 * D + 1, hr = row / a.nq;
   auto bias = [&](int head, int i) {  // distance i - D
     return a.rel_table[(size_t)min(max(a.rel_map[i], 0), a.rel_buckets - 1) * a.H + head] * p.rscale;
@@ -1146,7 +1189,7 @@ __global__ __launch_bounds__(256, 2) void rel_rows_kernel(const RelP p) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int q = lane + i * 64, r = q / G::CH, ch = q - r * G::CH;
-      *reinterpret_cast<u32x4*>(Vs + r * G::KP + ch * 8) = x.vr[i];
+      *reinterpret_cast<u32x4*>(Vs + place<DH>(r, ch)) = x.vr[i];
     }
     if (t + 4 * DEPTH < te) load(x, t + 4 * DEPTH);
     float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
@@ -1171,7 +1214,7 @@ __global__ __launch_bounds__(256, 2) void rel_rows_kernel(const RelP p) {
     __builtin_amdgcn_wave_barrier();  // the tile below was written by this wave alone: its LDS accesses stay in order
 #pragma unroll
     for (int dt = 0; dt < ND; ++dt) {
-      const bf16x8 vf = frag_tr<DH>(Vs, dt, lane);
+      const bf16x8 vf = frag_tr<DH>(Vs, dt, at.tr);
       O[dt] = mfma16(vf, pb, O[dt] * alpha);
       if (a.out_lo) {
         O[dt] = mfma16(vf, pm, O[dt]);
@@ -1275,12 +1318,12 @@ __global__ __launch_bounds__(256) void zero_rows_kernel(bf16_t* x, int n, int t0
 // ---- host ------------------------------------------------------------------------------------------------------------
 int launched() { return hipGetLastError() == hipSuccess ? 0 : -100; }
 
-// dynamic LDS above 64 KiB has to be allowed once per kernel and device
+// more than 64 KiB of LDS has to be allowed once per kernel and device
 template <typename K>
-int allow_lds(K kernel, size_t bytes) {
-  if (bytes <= 65536) return 0;
+int allow_lds(K kernel, size_t dynamic, size_t fixed) {
+  if (dynamic + fixed <= 65536) return 0;
   return hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
-                             160 * 1024) == hipSuccess ? 0 : -101;
+                             (int)dynamic) == hipSuccess ? 0 : -101;
 }
 
 bool few_rows(const FactAttention& a) { return (long long)a.nq * (a.H / a.Hkv) <= 16; }
@@ -1295,10 +1338,7 @@ long long span(const FactAttention& a) {
 // splits of the few-row kernel: enough workgroups to fill 256 CUs twice, at least 8 tiles (2 a wave) each
 int row_splits(const FactAttention& a) {
   const long long tiles = (span(a) + 31) / 32, wgs = (long long)a.B * a.Hkv;
-#ifndef ROWT
-#define ROWT 512
-#endif
-  long long s = std::min((ROWT + wgs - 1) / wgs, tiles / 8);
+  long long s = std::min((512 + wgs - 1) / wgs, tiles / 8);
   return (int)std::max(1ll, std::min(s, 256ll));
 }
 
@@ -1356,9 +1396,8 @@ int fwd_t(const FactAttention& a, void* ws, hipStream_t s) {
     return launched();
   }
   p.nwg = p.qblocks * a.B * a.H;
-  const size_t lds = 4 * Geo<DH>::IMG * 2 + (REL ? (2 * (a.rel_max_distance + PAD) + 1) * 4 : 0);
+  const size_t lds = REL ? (2 * (a.rel_max_distance + PAD) + 1) * 4 : 0;
   auto go = [&](auto kernel) {
-    if (int rc = allow_lds(kernel, lds)) return rc;
     FACT_LAUNCH(kernel, dim3(p.nwg), dim3(256), lds, s, p);
     return launched();
   };
@@ -1373,9 +1412,8 @@ int bwd_t(const FactAttention& a, void* ws, hipStream_t s) {
   p.part = (float*)((char*)ws + up16((size_t)a.B * a.H * a.nq * 4));
   p.dkv = (float*)((char*)p.part + part_bytes(a));
   p.nwg = p.qblocks * a.B * a.H;
-  const size_t lds1 = 4 * Geo<DH>::IMG * 2 + 5 * nb * 4, lds2 = 4 * Geo<DH>::IMG * 2 + 512 + nb * 4;
-  if (int rc = allow_lds(rel_dq_kernel<DH, REL>, lds1)) return rc;
-  if (int rc = allow_lds(rel_dkdv_kernel<DH, REL>, lds2)) return rc;
+  const size_t lds1 = 5 * nb * 4, lds2 = nb * 4;
+  if (int rc = allow_lds(rel_dq_kernel<DH, REL>, lds1, 4 * Geo<DH>::IMG * 2)) return rc;
   FACT_LAUNCH((rel_dq_kernel<DH, REL>), dim3(p.nwg), dim3(256), lds1, s, p);
   if (REL) FACT_LAUNCH(rel_dtable_kernel, dim3(a.H, a.rel_buckets), dim3(256), 0, s, p);
   p.nwg = (p.sblocks * p.schunks + (p.kblocks - p.sblocks) * p.chunks) * a.B * a.Hkv;
