@@ -27,7 +27,7 @@ struct RelP {
   int qblocks, nwg;
   int splits;
   int rowtab;     // few rows: the bias of the group's heads fits the workgroup's memory
-  int kblocks, sblocks, chunks, schunks;  // dK / dV: 128-key blocks, the first of them with sinks, workgroups of a block
+  int kblocks, sblocks, chunks, schunks;  // dK / dV: blocks of keys, the first of them with sinks, workgroups of a block
   float* dkv;     // partial dK, dV of blocks with several workgroups
   float* dsum;    // [B][H][nq] -rowsum(dO . O)
   float* part;    // per-workgroup bias gradients [B * H * qblocks][2 D + 1] / partial rows of the few-row kernel
@@ -816,8 +816,8 @@ __global__ __launch_bounds__(256) void rel_dtable_kernel(const RelP p) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// backward dK / dV: workgroup = 128 (64) keys of one key head, 4 waves x 32 (16); the query tiles of every head that reads them
-// are streamed (heads of a group one after another).  A block's stream is cut into `chunks` workgroups where there are too few
+// backward dK / dV: workgroup = 64 keys of one key head, 4 waves x 16; the query tiles of every head that reads them are
+// streamed (heads of a group one after another).  A block's stream is cut into `chunks` workgroups where there are too few
 // blocks to fill the chip or a block holds sinks, which all later queries see: their fp32 sums go through the workspace and
 // rel_join_dkdv_kernel adds them in order.
 // ---------------------------------------------------------------------------------------------------------------------
@@ -847,19 +847,16 @@ DEVINL KBlock kblock_of(const RelP& p, int id) {
   return k;
 }
 
-// KS 16-key sub-tiles a wave.  Two let every Q and dO fragment feed two products; dK, dV, K and V of 32 keys do not fit 256
-// registers at dh 128 (the accumulators then travel through the other half of the register file, 320 moves a tile: 577 us at
-// B 8, H 12, n 1440), so there a wave has one.
-template <int DH>
-constexpr int key_subs() { return DH > 96 ? 1 : 2; }
-template <int DH>
-constexpr int block_keys() { return 64 * key_subs<DH>(); }
-int block_keys(int dh) { return dh > 96 ? 64 : 128; }
-
+// A wave has 16 keys and its four sums fit the registers of 4 (dh 96 and 128: 3) workgroups a CU.  With 32 keys a wave every Q
+// and dO fragment feeds two products, but two workgroups a CU are left: dh 64, B 2, H 12 on 4 key heads, n 2047, window 256 takes
+// 45.8 us instead of 29.8; B 4, H 12, n 1440, window 257: 57 instead of 38; B 8, H 12, n 1440, all keys: 186 instead of 176
+// (dh 80: 222 and 214, dh 32: 115 and 132, where nothing else gains).
+constexpr int BLOCK_KEYS = 64;
+constexpr int dkdv_slots(int dh) { return dh < 96 ? 4 : 3; }  // workgroups of a CU
 template <int DH, bool REL>
-__global__ __launch_bounds__(256, DH > 96 ? 3 : 2) void rel_dkdv_kernel(const RelP p) {
+__global__ __launch_bounds__(256, dkdv_slots(DH)) void rel_dkdv_kernel(const RelP p) {
   using G = Geo<DH>;
-  constexpr int ND = G::ND, KS = key_subs<DH>(), BK = block_keys<DH>();
+  constexpr int ND = G::ND;
   __shared__ __attribute__((aligned(16))) bf16_t buf0[2 * G::IMG + 128], buf1[2 * G::IMG + 128];  // Q, dO, fp32 L and -D
   extern __shared__ float eb[];
   const FactAttention& a = p.a;
@@ -871,30 +868,27 @@ __global__ __launch_bounds__(256, DH > 96 ? 3 : 2) void rel_dkdv_kernel(const Re
   const int kb = blk.kb, b = blk.bh / a.Hkv, hk = blk.bh - b * a.Hkv;
   const Vis v = vis_of(a, b);
   const int start = start_of(a, b);
-  const int j0 = kb * BK + wave * 16 * KS;
+  const int j0 = kb * BLOCK_KEYS + wave * 16;
   const bool active = j0 < v.len;
   // query rows that see any key of the block: positions [ka - hi, ke - lo], or all later ones if it holds a sink
-  const long long ka = kb * BK, ke = min(kb * BK + BK - 1, v.len - 1);
+  const long long ka = kb * BLOCK_KEYS, ke = min(kb * BLOCK_KEYS + BLOCK_KEYS - 1, v.len - 1);
   long long qa = v.hi == INT_MAX ? 0 : max(0ll, ka - v.hi - start);
   long long qe = (v.lo == INT_MIN || ka < v.sinks) ? a.nq - 1 : min((long long)a.nq - 1, ke - v.lo - start);
   if (ka >= v.len) qe = -1;
   const int t0 = (int)(min(qa, 1ll << 30) >> 5), T = qe >= qa ? (int)(qe >> 5) - t0 + 1 : 0, TT = T * group;
   const int per = (TT + blk.chunks - 1) / blk.chunks, ib = min(TT, blk.chunk * per), ie = min(TT, ib + per);
 
-  Frag<DH> K[KS], V[KS];
-#pragma unroll
-  for (int ks = 0; ks < KS; ++ks) {
-    const long long j = max(0, min(j0 + ks * 16 + c, v.len - 1));
-    frag_load<DH>(K[ks], (const bf16_t*)a.k + b * a.k_stride[0] + j * a.k_stride[1] + hk * a.k_stride[2], g);
-    frag_load<DH>(V[ks], (const bf16_t*)a.v + b * a.v_stride[0] + j * a.v_stride[1] + hk * a.v_stride[2], g);
+  Frag<DH> K, V;
+  {
+    const long long j = max(0, min(j0 + c, v.len - 1));
+    frag_load<DH>(K, (const bf16_t*)a.k + b * a.k_stride[0] + j * a.k_stride[1] + hk * a.k_stride[2], g);
+    frag_load<DH>(V, (const bf16_t*)a.v + b * a.v_stride[0] + j * a.v_stride[1] + hk * a.v_stride[2], g);
   }
   pad_zero<DH>(buf0, tid);
   pad_zero<DH>(buf1, tid);
-  f32x4 dK[KS][ND], dV[KS][ND];
+  f32x4 dK[ND], dV[ND];
 #pragma unroll
-  for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-    for (int dt = 0; dt < ND; ++dt) dK[ks][dt] = dV[ks][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int dt = 0; dt < ND; ++dt) dK[dt] = dV[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
   Lane<DH> at;
   at.init(lane);
   Stage<DH> st;
@@ -904,8 +898,10 @@ __global__ __launch_bounds__(256, DH > 96 ? 3 : 2) void rel_dkdv_kernel(const Re
     st.load(buf, (const bf16_t*)a.q + b * a.q_stride[0] + h * a.q_stride[2],
             (const bf16_t*)a.dout + b * a.dout_stride[0] + h * a.dout_stride[2], q0, a.nq - 1);
     if (wave == 0) {
-      const size_t at = ((size_t)b * a.H + h) * a.nq + min(q0 + (lane & 31), a.nq - 1);
-      __builtin_amdgcn_global_load_lds((glb_void*)((lane < 32 ? a.lse : p.dsum) + at), (lds_void*)(buf + 2 * G::IMG), 4, 0, 0);
+      int l = lane;
+      asm("" : "+v"(l));  // (the addresses are made here, not kept)
+      const size_t row = ((size_t)b * a.H + h) * a.nq + min(q0 + (l & 31), a.nq - 1);
+      __builtin_amdgcn_global_load_lds((glb_void*)((l < 32 ? a.lse : p.dsum) + row), (lds_void*)(buf + 2 * G::IMG), 4, 0, 0);
     }
   };
   int hh = ib < ie ? ib / T : 0, qt = ib - hh * T;
@@ -921,33 +917,24 @@ __global__ __launch_bounds__(256, DH > 96 ? 3 : 2) void rel_dkdv_kernel(const Re
     const int q0 = (t0 + qt) * 32, p0 = start + q0;
     if (DH > 96) asm("" : "+v"(at.tr));  // offsets made from them each tile: kept, they do not fit the registers of 3 waves
     if (REL && DH > 96) asm("" : "+v"(at.rows));
-    const bool skip = !active || v.none<16 * KS>(j0, p0);
-    f32x4 s[2][KS], dp[2][KS];  // [query sub-tile][key sub-tile]: lane = key c, queries 4 g .. 4 g + 3
+    const bool skip = !active || v.none<16>(j0, p0);
+    if (DH >= 80) asm("" : "+v"(at.tr), "+v"(at.rows));  // offsets made from them each tile: kept, they do not fit the registers
+    f32x4 s[2], dp[2];  // query sub-tiles: lane = key c, queries 4 g .. 4 g + 3
     if (REL && !skip) {
       const int d0 = j0 - p0;
-      if (d0 - 31 >= D || d0 + 16 * KS - 1 <= -D) {
+      if (d0 - 31 >= D || d0 + 15 <= -D) {
         const float f = eb[d0 > 0 ? NB - 1 : 0];
-#pragma unroll
-        for (int qs = 0; qs < 2; ++qs)
-#pragma unroll
-          for (int ks = 0; ks < KS; ++ks) s[qs][ks] = f32x4{f, f, f, f};
+        s[0] = s[1] = f32x4{f, f, f, f};
       } else {
         const float* e = eb + d0 + D + PAD + c - 4 * g;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          s[1][0][r] = e[-r - 16];
-          s[0][0][r] = e[-r];
-          if constexpr (KS > 1) {
-            s[1][1][r] = s[0][0][r];
-            s[0][1][r] = e[16 - r];
-          }
+          s[0][r] = e[-r];
+          s[1][r] = e[-r - 16];
         }
       }
     } else {
-#pragma unroll
-      for (int qs = 0; qs < 2; ++qs)
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) s[qs][ks] = f32x4{0.f, 0.f, 0.f, 0.f};
+      s[0] = s[1] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
     if (++qt == T) {
       qt = 0;
@@ -955,62 +942,40 @@ __global__ __launch_bounds__(256, DH > 96 ? 3 : 2) void rel_dkdv_kernel(const Re
     }
     if (i + 1 < ie) load(hh, qt, other);  // (after the reads of the bias: they would wait for it)
     if (skip) return;
-    f32x4 L[2], nd[2];
+    f32x4 L[2], pr[2];
 #pragma unroll
     for (int qs = 0; qs < 2; ++qs) {
       L[qs] = *reinterpret_cast<const f32x4*>(sl + qs * 16 + g * 4);
-      nd[qs] = *reinterpret_cast<const f32x4*>(sl + 32 + qs * 16 + g * 4);
+      dp[qs] = *reinterpret_cast<const f32x4*>(sl + 32 + qs * 16 + g * 4);
       Frag<DH> Q, dO;
       frag_lds<DH>(Q, Qs, qs, at.rows);
       frag_lds<DH>(dO, Os, qs, at.rows);
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        s[qs][ks] = frag_dot<DH>(Q, K[ks], s[qs][ks]);
-        dp[qs][ks] = frag_dot<DH>(dO, V[ks], nd[qs]);
-      }
+      s[qs] = frag_dot<DH>(Q, K, s[qs]);
+      dp[qs] = frag_dot<DH>(dO, V, dp[qs]);
     }
-    f32x4 pr[2][KS];
 #pragma unroll
     for (int qs = 0; qs < 2; ++qs)
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
+      for (int r = 0; r < 4; ++r) {
+        pr[qs][r] = __builtin_amdgcn_exp2f(fmaf(s[qs][r], p.sc, -L[qs][r]));
+        dp[qs][r] *= pr[qs][r];
+      }
+    if (!v.full<16>(j0, p0) || q0 + 31 >= a.nq) {
+#pragma unroll
+      for (int qs = 0; qs < 2; ++qs)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          pr[qs][ks][r] = __builtin_amdgcn_exp2f(fmaf(s[qs][ks][r], p.sc, -L[qs][r]));
-          dp[qs][ks][r] *= pr[qs][ks][r];
+          const int q = qs * 16 + 4 * g + r;
+          const bool ok = v.seen(j0 + c, p0 + q) & (q0 + q < a.nq);
+          pr[qs][r] = ok ? pr[qs][r] : 0.f;
+          dp[qs][r] = (ok & !v.lone(p0 + q)) ? dp[qs][r] : 0.f;
         }
-    if (!v.full<16 * KS>(j0, p0) || q0 + 31 >= a.nq) {
-      bool lone[2][4];
-#pragma unroll
-      for (int qs = 0; qs < 2; ++qs)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) lone[qs][r] = v.lone(p0 + qs * 16 + 4 * g + r);
-#pragma unroll
-      for (int qs = 0; qs < 2; ++qs)
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const bool ok = v.seen(j0 + ks * 16 + c, p0 + qs * 16 + 4 * g + r) & (q0 + qs * 16 + 4 * g + r < a.nq);
-            pr[qs][ks][r] = ok ? pr[qs][ks][r] : 0.f;
-            dp[qs][ks][r] = (ok & !lone[qs][r]) ? dp[qs][ks][r] : 0.f;
-          }
     }
-    bf16x8 pb[KS], db[KS];
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      pb[ks] = pack8(pr[0][ks], pr[1][ks]);
-      db[ks] = pack8(dp[0][ks], dp[1][ks]);
-    }
+    const bf16x8 pb = pack8(pr[0], pr[1]), db = pack8(dp[0], dp[1]);
 #pragma unroll
     for (int dt = 0; dt < ND; ++dt) {
-      const bf16x8 of = frag_tr<DH>(Os, dt, at.tr);
-      const bf16x8 qf = frag_tr<DH>(Qs, dt, at.tr);
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        dV[ks][dt] = mfma16(of, pb[ks], dV[ks][dt]);
-        dK[ks][dt] = mfma16(qf, db[ks], dK[ks][dt]);
-      }
+      dV[dt] = mfma16(frag_tr<DH>(Os, dt, at.tr), pb, dV[dt]);
+      dK[dt] = mfma16(frag_tr<DH>(Qs, dt, at.tr), db, dK[dt]);
     }
   };
   for (int i = ib; i < ie;) {
@@ -1020,40 +985,35 @@ __global__ __launch_bounds__(256, DH > 96 ? 3 : 2) void rel_dkdv_kernel(const Re
     ++i;
   }
   if (blk.slot >= 0) {
-    f32x4* out = reinterpret_cast<f32x4*>(p.dkv) + ((size_t)blk.slot * (BK / 16) + wave * KS) * (2 * ND * 64) + lane;
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-      for (int dt = 0; dt < ND; ++dt) {
-        out[(ks * ND + dt) * 128] = dK[ks][dt];
-        out[(ks * ND + dt) * 128 + 64] = dV[ks][dt];
-      }
-    return;
-  }
-#pragma unroll
-  for (int ks = 0; ks < KS; ++ks) {
-    const int j = j0 + ks * 16 + c;
-    if (j >= a.nk) continue;
-    bf16_t* kr = (bf16_t*)a.dk + b * a.dk_stride[0] + (long long)j * a.dk_stride[1] + hk * a.dk_stride[2] + g * 4;
-    bf16_t* vr = (bf16_t*)a.dv + b * a.dv_stride[0] + (long long)j * a.dv_stride[1] + hk * a.dv_stride[2] + g * 4;
+    f32x4* out = reinterpret_cast<f32x4*>(p.dkv) + ((size_t)blk.slot * (BLOCK_KEYS / 16) + wave) * (2 * ND * 64) + lane;
 #pragma unroll
     for (int dt = 0; dt < ND; ++dt) {
-      bf16x4 x, y;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        x[r] = (bf16_t)(dK[ks][dt][r] * a.scale);
-        y[r] = (bf16_t)dV[ks][dt][r];
-      }
-      *reinterpret_cast<bf16x4*>(kr + dt * 16) = x;
-      *reinterpret_cast<bf16x4*>(vr + dt * 16) = y;
+      out[dt * 128] = dK[dt];
+      out[dt * 128 + 64] = dV[dt];
     }
+    return;
+  }
+  const int j = j0 + c;
+  if (j >= a.nk) return;
+  bf16_t* kr = (bf16_t*)a.dk + b * a.dk_stride[0] + (long long)j * a.dk_stride[1] + hk * a.dk_stride[2] + g * 4;
+  bf16_t* vr = (bf16_t*)a.dv + b * a.dv_stride[0] + (long long)j * a.dv_stride[1] + hk * a.dv_stride[2] + g * 4;
+#pragma unroll
+  for (int dt = 0; dt < ND; ++dt) {
+    bf16x4 x, y;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      x[r] = (bf16_t)(dK[dt][r] * a.scale);
+      y[r] = (bf16_t)dV[dt][r];
+    }
+    *reinterpret_cast<bf16x4*>(kr + dt * 16) = x;
+    *reinterpret_cast<bf16x4*>(vr + dt * 16) = y;
   }
 }
 
 // the chunks of a block, in order: a wave per accumulator fragment (16-key sub-tile, dt, K or V) of the kernel above
 template <int DH>
 __global__ __launch_bounds__(256) void rel_join_dkdv_kernel(const RelP p) {
-  constexpr int ND = Geo<DH>::ND, BK = block_keys<DH>(), FR = BK / 16 * 2 * ND;  // fragments of a block
+  constexpr int ND = Geo<DH>::ND, FR = BLOCK_KEYS / 16 * 2 * ND;  // fragments of a block
   const FactAttention& a = p.a;
   const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
   const int f = (blockIdx.x * 4 + (threadIdx.x >> 6)) % FR, blk = (blockIdx.x * 4 + (threadIdx.x >> 6)) / FR;
@@ -1067,7 +1027,7 @@ __global__ __launch_bounds__(256) void rel_join_dkdv_kernel(const RelP p) {
   f32x4 x = src[0];
   for (int i = 1; i < n; ++i) x += src[(size_t)i * FR * 64];
   const int dt = (f >> 1) % ND, isv = f & 1;
-  const int j = kb * BK + f / (2 * ND) * 16 + c;
+  const int j = kb * BLOCK_KEYS + f / (2 * ND) * 16 + c;
   if (j >= a.nk) return;
   const int64_t* st = isv ? a.dv_stride : a.dk_stride;
   const float k = isv ? 1.f : a.scale;
@@ -1356,17 +1316,16 @@ RelP params(const FactAttention& a) {
   p.dsum = nullptr;
   p.part = nullptr;
   p.dkv = nullptr;
-  // dK / dV: streams of the blocks as long as lengths and positions allow (they are on the device), cut so that the grid fills
-  // 256 CUs twice (three times with blocks of 64 keys) but no piece is shorter than 4 tiles
+  // dK / dV: streams of the blocks as long as lengths and positions allow (they are on the device), cut so that the chip
+  // is filled but no piece is shorter than 4 tiles
   const long long group = a.H / a.Hkv, all = ((long long)a.nq + 31) / 32 * group;
-  const int bk = block_keys(a.dh);
-  p.kblocks = (a.nk + bk - 1) / bk;
-  p.sblocks = a.window_left < 0 ? 0 : (std::min(a.sinks, a.nk) + bk - 1) / bk;
+  p.kblocks = (a.nk + BLOCK_KEYS - 1) / BLOCK_KEYS;
+  p.sblocks = a.window_left < 0 ? 0 : (std::min(a.sinks, a.nk) + BLOCK_KEYS - 1) / BLOCK_KEYS;
   long long seen = a.nq;
   if (a.window_left >= 0 && a.window_right >= 0)
-    seen = std::min<long long>(seen, (long long)bk + a.window_left + a.window_right + 62);
+    seen = std::min<long long>(seen, (long long)BLOCK_KEYS + a.window_left + a.window_right + 62);
   const long long t = (seen + 31) / 32 * group, blocks = (long long)a.B * a.Hkv * p.kblocks;
-  p.chunks = (int)std::max(1ll, std::min(((bk < 128 ? 768 : 512) + blocks / 2) / blocks, t / 4));
+  p.chunks = (int)std::max(1ll, std::min((768 + blocks / 2) / blocks, t / 4));
   const long long piece = std::max(8ll, (t + p.chunks - 1) / p.chunks);
   p.schunks = (int)std::max<long long>(p.chunks, std::min(all / piece, 64ll));
   return p;
@@ -1375,7 +1334,7 @@ RelP params(const FactAttention& a) {
 size_t dkv_chunks(const RelP& p) {
   return (p.schunks > 1 ? (size_t)p.sblocks * p.schunks : 0) + (p.chunks > 1 ? (size_t)(p.kblocks - p.sblocks) * p.chunks : 0);
 }
-size_t dkv_bytes(const RelP& p) { return dkv_chunks(p) * p.a.B * p.a.Hkv * block_keys(p.a.dh) * 2 * p.a.dh * 4; }
+size_t dkv_bytes(const RelP& p) { return dkv_chunks(p) * p.a.B * p.a.Hkv * BLOCK_KEYS * 2 * p.a.dh * 4; }
 
 // the dQ kernel's partial bias gradients
 size_t part_bytes(const FactAttention& a) {
@@ -1419,7 +1378,7 @@ int bwd_t(const FactAttention& a, void* ws, hipStream_t s) {
   p.nwg = (p.sblocks * p.schunks + (p.kblocks - p.sblocks) * p.chunks) * a.B * a.Hkv;
   FACT_LAUNCH((rel_dkdv_kernel<DH, REL>), dim3(p.nwg), dim3(256), lds2, s, p);
   const int joined = ((p.schunks > 1 ? p.sblocks : 0) + (p.chunks > 1 ? p.kblocks - p.sblocks : 0)) * a.B * a.Hkv;
-  if (joined) FACT_LAUNCH(rel_join_dkdv_kernel<DH>, dim3(joined * (block_keys<DH>() / 32) * Geo<DH>::ND), dim3(256), 0, s, p);
+  if (joined) FACT_LAUNCH(rel_join_dkdv_kernel<DH>, dim3(joined * (BLOCK_KEYS / 32) * Geo<DH>::ND), dim3(256), 0, s, p);
   return launched();
 }
 
