@@ -16,8 +16,9 @@
 namespace {
 
 constexpr float LOG2E = 1.4426950408889634f;
+constexpr int BLOCK_ROWS = 64;  // queries of a workgroup, 16 a wave
 constexpr float THR = 6.0f;
-constexpr int PAD = 80;  // distances past +-D that a 32 x 32 tile which still touches (-D, D) can reach (62), and its folds (75)
+constexpr int PAD = 48;  // distances past +-D that a 32 x 16 tile which still touches (-D, D) can reach
 typedef __attribute__((address_space(3))) bf16x4 lds_bf16x4;
 
 struct RelP {
@@ -30,7 +31,7 @@ struct RelP {
   int kblocks, sblocks, chunks, schunks;  // dK / dV: blocks of keys, the first of them with sinks, workgroups of a block
   float* dkv;     // partial dK, dV of blocks with several workgroups
   float* dsum;    // [B][H][nq] -rowsum(dO . O)
-  float* part;    // per-workgroup bias gradients [B * H * qblocks][2 D + 1] / partial rows of the few-row kernel
+  float* part;    // per-workgroup bias gradients [H][B][qblocks][2 D + 1] / partial rows of the few-row kernel
 };
 
 template <int DH>
@@ -159,14 +160,14 @@ struct Vis {
     const long long low = lo == INT_MIN ? 0 : max(0ll, (long long)p + lo), sk = min((long long)sinks, top);
     return max(0ll, top - max(low, sk)) + max(0ll, sk) == 1;
   }
-  // keys j0 .. j0 + W - 1 against positions p0 .. p0 + 31
-  template <int W = 32>
+  // keys j0 .. j0 + W - 1 against positions p0 .. p0 + R - 1
+  template <int W = 32, int R = 32>
   DEVINL bool none(int j0, int p0) const {
-    return j0 >= len || j0 - (p0 + 31) > hi || (j0 + W - 1 - p0 < lo && j0 >= sinks);
+    return j0 >= len || j0 - (p0 + R - 1) > hi || (j0 + W - 1 - p0 < lo && j0 >= sinks);
   }
-  template <int W = 32>
+  template <int W = 32, int R = 32>
   DEVINL bool full(int j0, int p0) const {
-    return j0 + W - 1 < len && j0 + W - 1 - p0 <= hi && (j0 - (p0 + 31) >= lo || j0 + W - 1 < sinks);
+    return j0 + W - 1 < len && j0 + W - 1 - p0 <= hi && (j0 - (p0 + R - 1) >= lo || j0 + W - 1 < sinks);
   }
 };
 // Lengths are below 2^30 (checked) and first positions clamped to +-(2^30 - 64), so no key - position overflows.
@@ -276,7 +277,7 @@ DEVINL void load_bias(float* eb, const RelP& p, int h, int tid, int nthr) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// forward: workgroup = 128 queries of one head, 4 waves x 32 queries; 32-key tiles double-buffered in LDS
+// forward: workgroup = 64 queries of one head, 4 waves x 16; 32-key tiles double-buffered in LDS
 // ---------------------------------------------------------------------------------------------------------------------
 // EXACT (a.out_lo given): the probabilities enter P V as a sum of three bf16 values, 24 bits, and the output's rounding residual
 // is kept in fp32.  The backward takes D = rowsum(dO . O) from them: from the rounded P and O it is off by 1e-3 of itself, which
@@ -295,15 +296,12 @@ __global__ __launch_bounds__(256, 2) void rel_fwd_kernel(const RelP p) {
   const int b = bh / a.H, h = bh - b * a.H, hk = h / (a.H / a.Hkv);
   const Vis v = vis_of(a, b);
   const int start = start_of(a, b);
-  const int q0 = qb * 128 + wave * 32, p0 = start + q0;
+  const int q0 = qb * BLOCK_ROWS + wave * 16, p0 = start + q0;
   const bool active = q0 < a.nq;
-  const Tiles tl = tiles_of(v, (long long)start + qb * 128, (long long)start + min(qb * 128 + 127, a.nq - 1));
+  const Tiles tl = tiles_of(v, (long long)start + qb * BLOCK_ROWS, (long long)start + min(qb * BLOCK_ROWS + BLOCK_ROWS - 1, a.nq - 1));
 
-  Frag<DH> Q[2];
-#pragma unroll
-  for (int qs = 0; qs < 2; ++qs)
-    frag_load<DH>(Q[qs], (const bf16_t*)a.q + b * a.q_stride[0] + (long long)min(q0 + qs * 16 + c, a.nq - 1) * a.q_stride[1] +
-                             h * a.q_stride[2], g);
+  Frag<DH> Q;
+  frag_load<DH>(Q, (const bf16_t*)a.q + b * a.q_stride[0] + (long long)min(q0 + c, a.nq - 1) * a.q_stride[1] + h * a.q_stride[2], g);
   Lane<DH> at;
   at.init(lane);
   Stage<DH> st;
@@ -314,43 +312,31 @@ __global__ __launch_bounds__(256, 2) void rel_fwd_kernel(const RelP p) {
   pad_zero<DH>(buf1, tid);
   if (tl.T > 0) st.load(buf0, kp, vp, tl.at(0) * 32, v.len - 1);
   if (REL) load_bias(eb, p, h, tid, 256);
-  f32x4 O[2][ND];
-  float m[2], l[2];
+  f32x4 O[ND];
+  float m = -INFINITY, l = 0.f;
 #pragma unroll
-  for (int qs = 0; qs < 2; ++qs) {
-    m[qs] = -INFINITY;
-    l[qs] = 0.f;
-#pragma unroll
-    for (int dt = 0; dt < ND; ++dt) O[qs][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
+  for (int dt = 0; dt < ND; ++dt) O[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
   const int D = a.rel_max_distance;
   auto step = [&](int t, const bf16_t* Ks, bf16_t* other) __attribute__((always_inline)) {
     const bf16_t* Vs = Ks + G::IMG;
     const int j0 = tl.at(t) * 32;
-    const bool skip = !active || v.none(j0, p0);
-    f32x4 s[2][2];  // [key sub-tile][query sub-tile]
+    const bool skip = !active || v.none<32, 16>(j0, p0);
+    f32x4 s[2];  // key sub-tiles
     if (REL && !skip) {
       const int d0 = j0 - p0;  // distance of the tile's first key and the wave's first query
-      if (d0 - 31 >= D || d0 + 31 <= -D) {
+      if (d0 - 15 >= D || d0 + 31 <= -D) {
         const float f = eb[d0 > 0 ? 2 * (D + PAD) : 0];
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-          for (int qs = 0; qs < 2; ++qs) s[ks][qs] = f32x4{f, f, f, f};
+        s[0] = s[1] = f32x4{f, f, f, f};
       } else {
         const float* e = eb + d0 + D + PAD + 4 * g - c;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          s[0][1][r] = e[r - 16];
-          s[0][0][r] = s[1][1][r] = e[r];
-          s[1][0][r] = e[r + 16];
+          s[0][r] = e[r];
+          s[1][r] = e[r + 16];
         }
       }
     } else {
-#pragma unroll
-      for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-        for (int qs = 0; qs < 2; ++qs) s[ks][qs] = f32x4{0.f, 0.f, 0.f, 0.f};
+      s[0] = s[1] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
     if (t + 1 < tl.T) st.load(other, kp, vp, tl.at(t + 1) * 32, v.len - 1);  // (after the reads of the bias: they would wait for it)
     if (skip) return;
@@ -358,78 +344,60 @@ __global__ __launch_bounds__(256, 2) void rel_fwd_kernel(const RelP p) {
     for (int ks = 0; ks < 2; ++ks) {
       Frag<DH> K;
       frag_lds<DH>(K, Ks, ks, at.rows);
-#pragma unroll
-      for (int qs = 0; qs < 2; ++qs) s[ks][qs] = frag_dot<DH>(K, Q[qs], s[ks][qs]);
+      s[ks] = frag_dot<DH>(K, Q, s[ks]);
     }
-    if (!v.full(j0, p0)) {
+    if (!v.full<32, 16>(j0, p0)) {
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
-        for (int qs = 0; qs < 2; ++qs)
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            s[ks][qs][r] = v.seen(j0 + ks * 16 + 4 * g + r, p0 + qs * 16 + c) ? s[ks][qs][r] : -INFINITY;
+        for (int r = 0; r < 4; ++r) s[ks][r] = v.seen(j0 + ks * 16 + 4 * g + r, p0 + c) ? s[ks][r] : -INFINITY;
     }
     // The reference point m of a row's exponents is raised only when a score passes it by THR powers of two: any m that keeps
     // exp2 in range gives the same softmax, and the common path needs no lane but its own.
-    bf16x8 pb[2], pl[2], pm[2];
-    float mx[2];
+    const float mu = m == -INFINITY ? 0.f : m;  // -inf: the row has seen no key yet
 #pragma unroll
-    for (int qs = 0; qs < 2; ++qs) {
-      const float mu = m[qs] == -INFINITY ? 0.f : m[qs];  // -inf: the row has seen no key yet
+    for (int r = 0; r < 4; ++r) {
+      s[0][r] = fmaf(s[0][r], p.sc, -mu);
+      s[1][r] = fmaf(s[1][r], p.sc, -mu);
+    }
+    const float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
+                           fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+    if (__any((mx > THR) | ((m == -INFINITY) & (mx > -INFINITY)))) {
+      const bool first = m == -INFINITY;
+      const float top = allmax4(mx);                   // relative to m, or to 0
+      const float d = first ? (top == -INFINITY ? 0.f : top) : fmaxf(top, 0.f);
+      const float alpha = __builtin_amdgcn_exp2f(-d);  // (first: nothing has been summed)
+      m = first ? top : m + d;
+      l = first ? 0.f : l * alpha;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        s[0][qs][r] = fmaf(s[0][qs][r], p.sc, -mu);
-        s[1][qs][r] = fmaf(s[1][qs][r], p.sc, -mu);
+        s[0][r] -= d;
+        s[1][r] -= d;
       }
-      mx[qs] = fmaxf(fmaxf(fmaxf(s[0][qs][0], s[0][qs][1]), fmaxf(s[0][qs][2], s[0][qs][3])),
-                     fmaxf(fmaxf(s[1][qs][0], s[1][qs][1]), fmaxf(s[1][qs][2], s[1][qs][3])));
+#pragma unroll
+      for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) O[dt][r] = first ? 0.f : O[dt][r] * alpha;
     }
-    if (__any((mx[0] > THR) | (mx[1] > THR) | ((m[0] == -INFINITY) & (mx[0] > -INFINITY)) |
-              ((m[1] == -INFINITY) & (mx[1] > -INFINITY)))) {
+    f32x4 e0, e1;
+    float ls = 0.f;
 #pragma unroll
-      for (int qs = 0; qs < 2; ++qs) {
-        const bool first = m[qs] == -INFINITY;
-        const float top = allmax4(mx[qs]);                       // relative to m, or to 0
-        const float d = first ? (top == -INFINITY ? 0.f : top) : fmaxf(top, 0.f);
-        const float alpha = __builtin_amdgcn_exp2f(-d);          // (first: nothing has been summed)
-        m[qs] = first ? top : m[qs] + d;
-        l[qs] = first ? 0.f : l[qs] * alpha;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          s[0][qs][r] -= d;
-          s[1][qs][r] -= d;
-        }
-#pragma unroll
-        for (int dt = 0; dt < ND; ++dt)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) O[qs][dt][r] = first ? 0.f : O[qs][dt][r] * alpha;
-      }
+    for (int r = 0; r < 4; ++r) {
+      e0[r] = __builtin_amdgcn_exp2f(s[0][r]);
+      e1[r] = __builtin_amdgcn_exp2f(s[1][r]);
+      ls += e0[r] + e1[r];
     }
-#pragma unroll
-    for (int qs = 0; qs < 2; ++qs) {
-      f32x4 e0, e1;
-      float ls = 0.f;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        e0[r] = __builtin_amdgcn_exp2f(s[0][qs][r]);
-        e1[r] = __builtin_amdgcn_exp2f(s[1][qs][r]);
-        ls += e0[r] + e1[r];
-      }
-      l[qs] += ls;
-      pb[qs] = pack8(e0, e1);
-      if (EXACT) split3(e0, e1, pb[qs], pm[qs], pl[qs]);
-    }
+    l += ls;
+    const bf16x8 pb = pack8(e0, e1);
+    bf16x8 pm, pl;
+    if (EXACT) split3(e0, e1, pb, pm, pl);
 #pragma unroll
     for (int dt = 0; dt < ND; ++dt) {
       const bf16x8 vf = frag_tr<DH>(Vs, dt, at.tr);
-#pragma unroll
-      for (int qs = 0; qs < 2; ++qs) {
-        O[qs][dt] = mfma16(vf, pb[qs], O[qs][dt]);
-        if (EXACT) {
-          O[qs][dt] = mfma16(vf, pm[qs], O[qs][dt]);
-          O[qs][dt] = mfma16(vf, pl[qs], O[qs][dt]);
-        }
+      O[dt] = mfma16(vf, pb, O[dt]);
+      if (EXACT) {
+        O[dt] = mfma16(vf, pm, O[dt]);
+        O[dt] = mfma16(vf, pl, O[dt]);
       }
     }
   };
@@ -441,28 +409,24 @@ __global__ __launch_bounds__(256, 2) void rel_fwd_kernel(const RelP p) {
     step(t, buf1, buf0);
     ++t;
   }
-  if (!active) return;
+  const int q = q0 + c;
+  const float lt = allsum4(l);
+  if (q >= a.nq) return;
+  const float inv = lt == 0.f ? 0.f : 1.0f / lt;
+  if (a.lse && g == 0) a.lse[((size_t)b * a.H + h) * a.nq + q] = lt == 0.f ? INFINITY : m + __log2f(lt);
+  const long long off = b * a.out_stride[0] + (long long)q * a.out_stride[1] + h * a.out_stride[2] + g * 4;
 #pragma unroll
-  for (int qs = 0; qs < 2; ++qs) {
-    const float lt = allsum4(l[qs]);
-    const float inv = lt == 0.f ? 0.f : 1.0f / lt;
-    const int q = q0 + qs * 16 + c;
-    if (q >= a.nq) continue;
-    if (a.lse && g == 0) a.lse[((size_t)b * a.H + h) * a.nq + q] = lt == 0.f ? INFINITY : m[qs] + __log2f(lt);
-    const long long off = b * a.out_stride[0] + (long long)q * a.out_stride[1] + h * a.out_stride[2] + g * 4;
+  for (int dt = 0; dt < ND; ++dt) {
+    bf16x4 o;
+    f32x4 lo;
 #pragma unroll
-    for (int dt = 0; dt < ND; ++dt) {
-      bf16x4 o;
-      f32x4 lo;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float x = O[qs][dt][r] * inv;
-        o[r] = (bf16_t)x;
-        lo[r] = x - (float)o[r];
-      }
-      *reinterpret_cast<bf16x4*>((bf16_t*)a.out + off + dt * 16) = o;
-      if (EXACT) *reinterpret_cast<f32x4*>(a.out_lo + low_row(a, b, h, q) + g * 4 + dt * 16) = lo;
+    for (int r = 0; r < 4; ++r) {
+      const float x = O[dt][r] * inv;
+      o[r] = (bf16_t)x;
+      lo[r] = x - (float)o[r];
     }
+    *reinterpret_cast<bf16x4*>((bf16_t*)a.out + off + dt * 16) = o;
+    if (EXACT) *reinterpret_cast<f32x4*>(a.out_lo + low_row(a, b, h, q) + g * 4 + dt * 16) = lo;
   }
 }
 
@@ -474,7 +438,7 @@ __global__ __launch_bounds__(256, 2) void rel_fwd_kernel(const RelP p) {
 //   * The four rows of lanes are 4 distances apart: rows 2 and 3 join rows 0 and 1 moved by 8 lanes, row 1 joins row 0 moved by 4;
 //     what leaves on that side belongs to the sub-tile at d + 16.
 // Key tiles are visited in ascending order, so a distance is complete after its two neighbours, and row 0 stores 16 of them at a
-// time, each once per 32 queries.  At B 8, H 12, n 1440, dh 128 dQ takes 735 us with an LDS add per value, 300 with one per
+// time, each once per 16 queries.  At B 8, H 12, n 1440, dh 128 dQ takes 735 us with an LDS add per value, 300 with one per
 // folded row (its four rows meet in the same words), 177 without any sums and 214 with this.
 template <int CTRL, int BANKS = 0xf>
 DEVINL float moved(float y) {  // y moved inside rows of 16 lanes; zero from outside and in lanes of other banks of 4
@@ -486,9 +450,9 @@ DEVINL void fold_diagonals(f32x4 v, float& w, float& up) {
   up = (v[3] + moved<ROR1>(v[2] + moved<ROR1>(v[1] + moved<ROR1>(v[0])))) - w;
 }
 struct Diagonals {
-  float* bins;         // this wave's sums by distance, at distance 3 - c
-  int g;
-  f32x4 next;          // sub-tile at base `at` + 16 that the next key tile adds to
+  float* bins;         // this wave's sums by distance, 1 - D .. D - 1
+  int D, g, c;
+  float left, right;   // lane's share of the sums at -D and D
   float w;             // sub-tile at base `at`, without its `up`
   float over1, over2;  // what rows 2, 3 and row 1 of the sub-tile before left for this one
   int at;
@@ -509,50 +473,53 @@ struct Diagonals {
     over2 = moved<ROR12, 0x8>(s);
     return z;
   }
-  DEVINL void put(int base, float z) {
-    if (g == 0) bins[base] = z;
-  }
-  DEVINL void add(int base, float z) {  // where runs of tiles begin and end, a distance can have been stored already
-    if (g == 0) atomicAdd(bins + base, z);
+  // lane's sum z of distance base + 3 - c (row 0) or further rows', four on each: `fresh` where nothing was stored there before
+  DEVINL void put(int base, float z, bool fresh, bool all) {
+    const int i = base + (all ? 4 * g : 0) + 3 - c + D - 1;
+    if (all || g == 0) {
+      if ((i >= 0) & (i < 2 * D - 1)) {
+        if (fresh) bins[i] = z;
+        else atomicAdd(bins + i, z);
+      } else if (i < 0) {
+        left += z;
+      } else {
+        right += z;
+      }
+    }
   }
   DEVINL void close() {
     if (!open) return;
-    float w2, up;
-    fold_diagonals(next, w2, up);
-    add(at, join(w + up));
-    add(at + 16, join(w2));
-    add(at + 32, join(0.f));
+    put(at, join(w), false, false);  // (where runs of tiles begin and end, a distance can have been stored already)
+    put(at + 16, join(0.f), false, false);
     open = false;
   }
-  // the sub-tiles at bases d0 - 16, d0, d0 + 16
-  DEVINL void tile(int d0, f32x4 a, f32x4 b, f32x4 c) {
+  // the sub-tiles at bases d0, d0 + 16
+  DEVINL void tile(int d0, f32x4 a, f32x4 b) {
     float wa, ua, wb, ub;
-    const bool on = open && at + 32 == d0;
+    const bool on = open && at + 16 == d0;
     if (!on) close();
-    if (on) a += next;
     fold_diagonals(a, wa, ua);
     fold_diagonals(b, wb, ub);
     if (on) {
-      put(d0 - 32, join(w + ua));
-      put(d0 - 16, join(wa + ub));
+      put(d0 - 16, join(w + ua), true, false);
+      put(d0, join(wa + ub), true, false);
     } else {  // (`ua` reaches into the 16 distances stored before it)
       over1 = over2 = 0.f;
-      put(d0 - 16, join(wa + ub));
-      atomicAdd(bins + d0 - 32 + 4 * g, ua);
+      put(d0, join(wa + ub), true, false);
+      put(d0 - 16, ua, false, true);
     }
     w = wb;
-    next = c;
-    at = d0;
+    at = d0 + 16;
     open = true;
   }
 };
 
 // ---------------------------------------------------------------------------------------------------------------------
-// backward dQ and the bias gradient: workgroup = 128 queries of one head
+// backward dQ and the bias gradient: workgroup = 64 queries of one head, 16 a wave
 //   P = exp2(S c - L);  dP = V dO^T;  dS = P (dP - D), D = rowsum(dO . O);  dQ^T += K^T dS;  dbias[j - p] += dS
 // ---------------------------------------------------------------------------------------------------------------------
 template <int DH, bool REL>
-__global__ __launch_bounds__(256, 2) void rel_dq_kernel(const RelP p) {
+__global__ __launch_bounds__(256, DH > 96 ? 3 : 4) void rel_dq_kernel(const RelP p) {
   using G = Geo<DH>;
   constexpr int ND = G::ND;
   __shared__ __attribute__((aligned(16))) bf16_t buf0[2 * G::IMG], buf1[2 * G::IMG];
@@ -561,15 +528,15 @@ __global__ __launch_bounds__(256, 2) void rel_dq_kernel(const RelP p) {
   const int D = a.rel_max_distance, NB = 2 * (D + PAD) + 1;
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, c = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  float* bins = eb + NB * (1 + wave);  // this wave's bias gradient by distance: its own, so sums have one order
+  float* bins = eb + NB + (2 * D - 1) * wave;  // this wave's bias gradient by distance: its own, so sums have one order
   const int id = xcd_order(blockIdx.x, p.nwg);
   const int bh = id / p.qblocks, qb = p.qblocks - 1 - (id - bh * p.qblocks);
   const int b = bh / a.H, h = bh - b * a.H, hk = h / (a.H / a.Hkv);
   const Vis v = vis_of(a, b);
   const int start = start_of(a, b);
-  const int q0 = qb * 128 + wave * 32, p0 = start + q0;
+  const int q0 = qb * BLOCK_ROWS + wave * 16, p0 = start + q0;
   const bool active = q0 < a.nq;
-  const Tiles tl = tiles_of(v, (long long)start + qb * 128, (long long)start + min(qb * 128 + 127, a.nq - 1));
+  const Tiles tl = tiles_of(v, (long long)start + qb * BLOCK_ROWS, (long long)start + min(qb * BLOCK_ROWS + BLOCK_ROWS - 1, a.nq - 1));
 
   Lane<DH> at;
   at.init(lane);
@@ -580,146 +547,116 @@ __global__ __launch_bounds__(256, 2) void rel_dq_kernel(const RelP p) {
   pad_zero<DH>(buf0, tid);
   pad_zero<DH>(buf1, tid);
   if (tl.T > 0) st.load(buf0, kp, vp, tl.at(0) * 32, v.len - 1);
-  Frag<DH> Q[2], dO[2];
-  float nL[2], nD[2];
-  bool live[2];  // a query of the call that sees more than one key
+  const int q = min(q0 + c, a.nq - 1);
+  const bool live = (q0 + c < a.nq) & !v.lone(start + q);  // a query of the call that sees more than one key
+  Frag<DH> Q, dO;
+  frag_load<DH>(Q, (const bf16_t*)a.q + b * a.q_stride[0] + (long long)q * a.q_stride[1] + h * a.q_stride[2], g);
+  frag_load<DH>(dO, (const bf16_t*)a.dout + b * a.dout_stride[0] + (long long)q * a.dout_stride[1] + h * a.dout_stride[2], g);
+  float part = 0.f;
+  {
+    Frag<DH> f;
+    frag_load<DH>(f, (const bf16_t*)a.out + b * a.out_stride[0] + (long long)q * a.out_stride[1] + h * a.out_stride[2], g);
 #pragma unroll
-  for (int qs = 0; qs < 2; ++qs) {
-    const int q = min(q0 + qs * 16 + c, a.nq - 1);
-    live[qs] = (q0 + qs * 16 + c < a.nq) & !v.lone(start + q);
-    frag_load<DH>(Q[qs], (const bf16_t*)a.q + b * a.q_stride[0] + (long long)q * a.q_stride[1] + h * a.q_stride[2], g);
-    frag_load<DH>(dO[qs], (const bf16_t*)a.dout + b * a.dout_stride[0] + (long long)q * a.dout_stride[1] + h * a.dout_stride[2], g);
-    const long long off = b * a.out_stride[0] + (long long)q * a.out_stride[1] + h * a.out_stride[2];
-    float part = 0.f;
-    {
-      Frag<DH> f;
-      frag_load<DH>(f, (const bf16_t*)a.out + off, g);
+    for (int kd = 0; kd < G::KD; ++kd)
 #pragma unroll
-      for (int kd = 0; kd < G::KD; ++kd)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) part += (float)dO[qs].f[kd][j] * (float)f.f[kd][j];
-      if (a.out_lo) {
-        const float* lo = a.out_lo + low_row(a, b, h, q);
-#pragma unroll
-        for (int kd = 0; kd < G::KD; ++kd)
-          if (kd * 32 + 32 <= DH || kd * 32 + g * 8 < DH) {
-            const f32x4 x = *reinterpret_cast<const f32x4*>(lo + kd * 32 + g * 8);
-            const f32x4 y = *reinterpret_cast<const f32x4*>(lo + kd * 32 + g * 8 + 4);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) part += (float)dO[qs].f[kd][j] * x[j] + (float)dO[qs].f[kd][4 + j] * y[j];
-          }
-      }
-    }
-    part = allsum4(part);
-    const size_t at = ((size_t)b * a.H + h) * a.nq + q;
-    nL[qs] = -a.lse[at];
-    nD[qs] = qs ? part : -part;
-    // The second sub-tile of queries is carried with its sign turned over (dS, hence dQ): the matrix pipe adds with a rounding
-    // that leans down by 0.02 of a last place, which the millions of dS behind one table entry add up to 3.5e-6 of its gradient.
-    if (qs) {
+      for (int j = 0; j < 8; ++j) part += (float)dO.f[kd][j] * (float)f.f[kd][j];
+    if (a.out_lo) {
+      const float* lo = a.out_lo + low_row(a, b, h, q);
 #pragma unroll
       for (int kd = 0; kd < G::KD; ++kd)
-        dO[qs].f[kd] = __builtin_bit_cast(bf16x8, __builtin_bit_cast(u32x4, dO[qs].f[kd]) ^ 0x80008000u);
+        if (kd * 32 + 32 <= DH || kd * 32 + g * 8 < DH) {
+          const f32x4 x = *reinterpret_cast<const f32x4*>(lo + kd * 32 + g * 8);
+          const f32x4 y = *reinterpret_cast<const f32x4*>(lo + kd * 32 + g * 8 + 4);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) part += (float)dO.f[kd][j] * x[j] + (float)dO.f[kd][4 + j] * y[j];
+        }
     }
-    if (active && g == 0) p.dsum[at] = -part;  // for the dK / dV kernel (repeated rows write the same value)
   }
-  f32x4 dQ[2][ND];
+  part = allsum4(part);
+  const size_t row = ((size_t)b * a.H + h) * a.nq + q;
+  const float nL = -a.lse[row];
+  if (active && g == 0) p.dsum[row] = -part;  // for the dK / dV kernel (repeated rows write the same value)
+  // Every second wave carries its queries with the sign turned over (dS, hence dQ): the matrix pipe adds with a rounding that
+  // leans down by 0.02 of a last place, which the millions of dS behind one table entry add up to 3.5e-6 of its gradient.
+  const bool turned = wave & 1;
+  const float nD = turned ? part : -part;
+  if (turned) {
 #pragma unroll
-  for (int qs = 0; qs < 2; ++qs)
+    for (int kd = 0; kd < G::KD; ++kd) dO.f[kd] = __builtin_bit_cast(bf16x8, __builtin_bit_cast(u32x4, dO.f[kd]) ^ 0x80008000u);
+  }
+  f32x4 dQ[ND];
 #pragma unroll
-    for (int dt = 0; dt < ND; ++dt) dQ[qs][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float farl = 0.f, farr = 0.f;
+  for (int dt = 0; dt < ND; ++dt) dQ[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
   Diagonals diag;
-  diag.bins = bins + D + PAD + 3 - c;
+  diag.bins = bins;
+  diag.D = D;
   diag.g = g;
+  diag.c = c;
+  diag.left = diag.right = 0.f;
   diag.over1 = diag.over2 = 0.f;
   diag.open = false;
-  diag.next = f32x4{0.f, 0.f, 0.f, 0.f};
   diag.w = 0.f;
   diag.at = 0;
   if (REL) {
     load_bias(eb, p, h, tid, 256);
-    for (int i = lane; i < NB; i += 64) bins[i] = 0.f;
+    for (int i = lane; i < 2 * D - 1; i += 64) bins[i] = 0.f;
   }
   auto step = [&](int t, const bf16_t* Ks, bf16_t* other) __attribute__((always_inline)) {
     const bf16_t* Vs = Ks + G::IMG;
     const int j0 = tl.at(t) * 32;
-    const bool skip = !active || v.none(j0, p0);
-    if (REL && DH > 96) asm("" : "+v"(at.tr));  // 8 offsets made from it each tile: kept, they do not fit 256 registers
-    f32x4 s[2][2], dp[2][2];
+    const bool skip = !active || v.none<32, 16>(j0, p0);
+    f32x4 s[2], dp[2];
     const int d0 = j0 - p0;
-    const bool left = REL && d0 + 31 <= -D, right = REL && d0 - 31 >= D;
+    const bool left = REL && d0 + 31 <= -D, right = REL && d0 - 15 >= D;
     if (REL && !skip) {
       if (left || right) {
         const float f = eb[right ? NB - 1 : 0];
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-          for (int qs = 0; qs < 2; ++qs) s[ks][qs] = f32x4{f, f, f, f};
+        s[0] = s[1] = f32x4{f, f, f, f};
       } else {
         const float* e = eb + d0 + D + PAD + 4 * g - c;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          s[0][1][r] = e[r - 16];
-          s[0][0][r] = s[1][1][r] = e[r];
-          s[1][0][r] = e[r + 16];
+          s[0][r] = e[r];
+          s[1][r] = e[r + 16];
         }
       }
     } else {
-#pragma unroll
-      for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-        for (int qs = 0; qs < 2; ++qs) s[ks][qs] = f32x4{0.f, 0.f, 0.f, 0.f};
+      s[0] = s[1] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
     if (t + 1 < tl.T) st.load(other, kp, vp, tl.at(t + 1) * 32, v.len - 1);  // (after the reads of the bias: they would wait for it)
     if (skip) return;
+    f32x4 ds[2];
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
       Frag<DH> K, V;
       frag_lds<DH>(K, Ks, ks, at.rows);
       frag_lds<DH>(V, Vs, ks, at.rows);
-#pragma unroll
-      for (int qs = 0; qs < 2; ++qs) {
-        dp[ks][qs] = f32x4{nD[qs], nD[qs], nD[qs], nD[qs]};
-        s[ks][qs] = frag_dot<DH>(K, Q[qs], s[ks][qs]);
-        dp[ks][qs] = frag_dot<DH>(V, dO[qs], dp[ks][qs]);
-      }
+      dp[ks] = f32x4{nD, nD, nD, nD};
+      s[ks] = frag_dot<DH>(K, Q, s[ks]);
+      dp[ks] = frag_dot<DH>(V, dO, dp[ks]);
     }
-    f32x4 ds[2][2];
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
-      for (int qs = 0; qs < 2; ++qs)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          ds[ks][qs][r] = __builtin_amdgcn_exp2f(fmaf(s[ks][qs][r], p.sc, nL[qs])) * dp[ks][qs][r];
-    if (!v.full(j0, p0) || q0 + 31 >= a.nq) {  // (queries past the last repeat it: kept out of the bias gradient)
+      for (int r = 0; r < 4; ++r) ds[ks][r] = __builtin_amdgcn_exp2f(fmaf(s[ks][r], p.sc, nL)) * dp[ks][r];
+    if (!v.full<32, 16>(j0, p0) || q0 + 15 >= a.nq) {  // (queries past the last repeat it: kept out of the bias gradient)
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
-        for (int qs = 0; qs < 2; ++qs)
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            ds[ks][qs][r] = (v.seen(j0 + ks * 16 + 4 * g + r, p0 + qs * 16 + c) & live[qs]) ? ds[ks][qs][r] : 0.f;
+        for (int r = 0; r < 4; ++r) ds[ks][r] = (v.seen(j0 + ks * 16 + 4 * g + r, p0 + c) & live) ? ds[ks][r] : 0.f;
     }
-    bf16x8 dsb[2];
+    const bf16x8 dsb = pack8(ds[0], ds[1]);
 #pragma unroll
-    for (int qs = 0; qs < 2; ++qs) dsb[qs] = pack8(ds[0][qs], ds[1][qs]);
-#pragma unroll
-    for (int dt = 0; dt < ND; ++dt) {
-      const bf16x8 kf = frag_tr<DH>(Ks, dt, at.tr);
-#pragma unroll
-      for (int qs = 0; qs < 2; ++qs) dQ[qs][dt] = mfma16(kf, dsb[qs], dQ[qs][dt]);
-    }
+    for (int dt = 0; dt < ND; ++dt) dQ[dt] = mfma16(frag_tr<DH>(Ks, dt, at.tr), dsb, dQ[dt]);
     if (REL) {
       if (left || right) {
         float x = 0.f;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) x += (ds[0][0][r] - ds[1][1][r]) + (ds[1][0][r] - ds[0][1][r]);
-        if (left) farl += x;
-        else farr += x;
+        for (int r = 0; r < 4; ++r) x += ds[0][r] + ds[1][r];
+        if (left) diag.left += x;
+        else diag.right += x;
       } else {
-        diag.tile(d0, -ds[0][1], ds[0][0] - ds[1][1], ds[1][0]);
+        diag.tile(d0, ds[0], ds[1]);
       }
     }
   };
@@ -731,47 +668,27 @@ __global__ __launch_bounds__(256, 2) void rel_dq_kernel(const RelP p) {
     step(t, buf1, buf0);
     ++t;
   }
-  if (active) {
+  if (q0 + c < a.nq) {
+    bf16_t* out = (bf16_t*)a.dq + b * a.dq_stride[0] + (long long)q * a.dq_stride[1] + h * a.dq_stride[2] + g * 4;
 #pragma unroll
-    for (int qs = 0; qs < 2; ++qs) {
-      const int q = q0 + qs * 16 + c;
-      if (q >= a.nq) continue;
-      bf16_t* row = (bf16_t*)a.dq + b * a.dq_stride[0] + (long long)q * a.dq_stride[1] + h * a.dq_stride[2] + g * 4;
+    for (int dt = 0; dt < ND; ++dt) {
+      bf16x4 o;
 #pragma unroll
-      for (int dt = 0; dt < ND; ++dt) {
-        bf16x4 o;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) o[r] = (bf16_t)(dQ[qs][dt][r] * (qs ? -a.scale : a.scale));
-        *reinterpret_cast<bf16x4*>(row + dt * 16) = o;
-      }
+      for (int r = 0; r < 4; ++r) o[r] = (bf16_t)(dQ[dt][r] * (turned ? -a.scale : a.scale));
+      *reinterpret_cast<bf16x4*>(out + dt * 16) = o;
     }
   }
   if (REL) {
     diag.close();
-    farl = wave_sum(farl);
-    farr = wave_sum(farr);
-    if (lane == 0) {
-      bins[PAD] += farl;
-      bins[NB - 1 - PAD] += farr;
-    }
+    const float far[2] = {wave_sum(diag.left), wave_sum(diag.right)};
     __syncthreads();
-    float* out = p.part + (size_t)id * (2 * D + 1);
-    float* b0 = eb + NB;
-    for (int i = tid; i < 2 * D + 1; i += 256) {
-      const int k = i + PAD;
-      float x = (b0[k] + b0[NB + k]) + (b0[2 * NB + k] + b0[3 * NB + k]);
-      if (i > 0 && i < 2 * D) out[i] = x;
-    }
-    // the two ends take the PAD distances beyond them as well
-    if (wave < 2) {
-      float x = 0.f;
-      for (int i = lane; i <= PAD; i += 64) {
-        const int k = wave ? NB - 1 - PAD + i : i;
-        x += (b0[k] + b0[NB + k]) + (b0[2 * NB + k] + b0[3 * NB + k]);
-      }
-      x = wave_sum(x);
-      if (lane == 0) out[wave ? 2 * D : 0] = x;
-    }
+    if (lane == 0) eb[wave] = far[0], eb[4 + wave] = far[1];  // (the table is not read any more)
+    __syncthreads();
+    float* out = p.part + (((size_t)h * a.B + b) * p.qblocks + qb) * (2 * D + 1);
+    const float* b0 = eb + NB;
+    const int n = 2 * D - 1;
+    for (int i = tid; i < n; i += 256) out[1 + i] = (b0[i] + b0[2 * n + i]) - (b0[n + i] + b0[3 * n + i]);
+    if (tid < 2) out[tid * 2 * D] = (eb[4 * tid] + eb[4 * tid + 2]) - (eb[4 * tid + 1] + eb[4 * tid + 3]);
   }
 }
 
@@ -797,13 +714,18 @@ __global__ __launch_bounds__(256) void rel_dtable_kernel(const RelP p) {
     if (in) list[at + __popcll(m & ((1ull << lane) - 1))] = (short)i;
     __syncthreads();
   }
-  const int rows = a.B * p.qblocks;
-  const float* part = p.part + (size_t)h * p.qblocks * n;
+  // 8 groups of 32 threads, every 8th row each: four rows' loads are under way at once
+  const int rows = a.B * p.qblocks, first = tid >> 5;
+  const float* part = p.part + (size_t)h * rows * n;
   float x = 0.f;
-#pragma unroll 4
-  for (int i = tid; i < rows * total; i += 256) {
-    const int r = i / total, b = r / p.qblocks;
-    x += part[((size_t)b * a.H * p.qblocks + (r - b * p.qblocks)) * n + list[i - r * total]];
+  for (int i = tid & 31; i < total; i += 32) {
+    const float* col = part + list[i];
+    int r = first;
+    for (; r + 24 < rows; r += 32) {
+      const float y0 = col[(size_t)r * n], y1 = col[(size_t)(r + 8) * n], y2 = col[(size_t)(r + 16) * n], y3 = col[(size_t)(r + 24) * n];
+      x += (y0 + y1) + (y2 + y3);
+    }
+    for (; r < rows; r += 8) x += col[(size_t)r * n];
   }
   x = wave_sum(x);
   if (lane == 0) red[wave] = x;
@@ -918,7 +840,8 @@ __global__ __launch_bounds__(256, dkdv_slots(DH)) void rel_dkdv_kernel(const Rel
     if (DH > 96) asm("" : "+v"(at.tr));  // offsets made from them each tile: kept, they do not fit the registers of 3 waves
     if (REL && DH > 96) asm("" : "+v"(at.rows));
     const bool skip = !active || v.none<16>(j0, p0);
-    if (DH >= 80) asm("" : "+v"(at.tr), "+v"(at.rows));  // offsets made from them each tile: kept, they do not fit the registers
+    if (DH >= 80) asm("" : "+v"(at.tr));  // offsets made from them each tile: kept, they do not fit the registers
+    if (DH >= 80 && (REL || DH < 96)) asm("" : "+v"(at.rows));
     f32x4 s[2], dp[2];  // query sub-tiles: lane = key c, queries 4 g .. 4 g + 3
     if (REL && !skip) {
       const int d0 = j0 - p0;
@@ -1309,7 +1232,7 @@ RelP params(const FactAttention& a) {
   p.a = a;
   p.sc = a.scale * LOG2E;
   p.rscale = 1.0f / a.scale;
-  p.qblocks = (a.nq + 127) / 128;
+  p.qblocks = (a.nq + BLOCK_ROWS - 1) / BLOCK_ROWS;
   p.nwg = 0;
   p.splits = 1;
   p.rowtab = 0;
@@ -1338,7 +1261,7 @@ size_t dkv_bytes(const RelP& p) { return dkv_chunks(p) * p.a.B * p.a.Hkv * BLOCK
 
 // the dQ kernel's partial bias gradients
 size_t part_bytes(const FactAttention& a) {
-  return a.rel_table ? up16((size_t)a.B * a.H * ((a.nq + 127) / 128) * (2 * a.rel_max_distance + 1) * 4) : 0;
+  return a.rel_table ? up16((size_t)a.B * a.H * ((a.nq + BLOCK_ROWS - 1) / BLOCK_ROWS) * (2 * a.rel_max_distance + 1) * 4) : 0;
 }
 
 template <int DH, bool REL>
@@ -1371,7 +1294,7 @@ int bwd_t(const FactAttention& a, void* ws, hipStream_t s) {
   p.part = (float*)((char*)ws + up16((size_t)a.B * a.H * a.nq * 4));
   p.dkv = (float*)((char*)p.part + part_bytes(a));
   p.nwg = p.qblocks * a.B * a.H;
-  const size_t lds1 = 5 * nb * 4, lds2 = nb * 4;
+  const size_t lds1 = (nb + (REL ? 4 * (2 * a.rel_max_distance - 1) : 0)) * 4, lds2 = nb * 4;
   if (int rc = allow_lds(rel_dq_kernel<DH, REL>, lds1, 4 * Geo<DH>::IMG * 2)) return rc;
   FACT_LAUNCH((rel_dq_kernel<DH, REL>), dim3(p.nwg), dim3(256), lds1, s, p);
   if (REL) FACT_LAUNCH(rel_dtable_kernel, dim3(a.H, a.rel_buckets), dim3(256), 0, s, p);
@@ -1408,7 +1331,7 @@ int rel_attention_check(const FactAttention& a, bool backward, const char** why)
   if (a.H % a.Hkv) return bad(-1, "H must be a multiple of Hkv");
   if (a.dh != 32 && a.dh != 64 && a.dh != 80 && a.dh != 96 && a.dh != 128)
     return bad(-3, "unsupported head dim (supported: 32, 64, 80, 96, 128)");
-  if ((long long)a.B * a.H > INT_MAX / 256 || ((long long)a.nq + 127) / 128 * a.B * a.H > INT_MAX / 4 ||
+  if ((long long)a.B * a.H > INT_MAX / 256 || ((long long)a.nq + 63) / 64 * a.B * a.H > INT_MAX / 4 ||
       ((long long)a.nk + 63) / 64 * a.B * a.Hkv > INT_MAX / 512)
     return bad(-1, "too many heads and blocks for one launch");
   if (!(a.scale >= 5.9604645e-8f) || !(a.scale <= 3.0e38f)) return bad(-1, "scale must be finite and at least 2^-24");
