@@ -1159,35 +1159,45 @@ __global__ __launch_bounds__(256, 2) void rel_rows_kernel(const RelP p) {
   }
 }
 
-// join the splits of the few-row kernel: one wave per row, 2 dims a lane
-__global__ __launch_bounds__(64) void rel_join_kernel(const RelP p) {
+// join the splits of the few-row kernel: a workgroup per row, every 4th split a wave, 2 dims a lane
+__global__ __launch_bounds__(256) void rel_join_kernel(const RelP p) {
   const FactAttention& a = p.a;
-  const int group = a.H / a.Hkv, R = group * a.nq, lane = threadIdx.x;
+  const int group = a.H / a.Hkv, R = group * a.nq, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int bh = blockIdx.x / R, r = blockIdx.x - bh * R, b = bh / a.Hkv, hk = bh - b * a.Hkv;
-  const size_t pitch = a.dh + 4;
+  const size_t pitch = a.dh + 4, step = (size_t)R * pitch;
   const float* src = p.part + ((size_t)bh * p.splits * R + r) * pitch;
-  float M = -INFINITY;
-  for (int s = lane; s < p.splits; s += 64) M = fmaxf(M, src[(size_t)s * R * pitch]);
-  M = wave_max(M);
-  const float mu = M == -INFINITY ? 0.f : M;
-  float lt = 0.f, o0 = 0.f, o1 = 0.f;
+  __shared__ float red[2][4], f[256];
+  __shared__ f32x2 o[4][64];
+  const float m = tid < p.splits ? src[tid * step] : -INFINITY, l = tid < p.splits ? src[tid * step + 1] : 0.f;  // splits <= 256
   const int d = min(lane * 2, a.dh - 2);
-  for (int s = 0; s < p.splits; ++s) {
-    const float* x = src + (size_t)s * R * pitch;
-    const float f = __builtin_amdgcn_exp2f(x[0] - mu);
-    lt += x[1] * f;
-    const f32x2 o = *reinterpret_cast<const f32x2*>(x + 4 + d);
-    o0 += o[0] * f;
-    o1 += o[1] * f;
+  float M = wave_max(m);
+  if (lane == 0) red[0][wave] = M;
+  __syncthreads();
+  M = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+  f[tid] = __builtin_amdgcn_exp2f(m - (M == -INFINITY ? 0.f : M));
+  const float lw = wave_sum(l * f[tid]);
+  if (lane == 0) red[1][wave] = lw;
+  __syncthreads();
+  f32x2 x = {0.f, 0.f};
+#pragma unroll 4
+  for (int s = wave; s < p.splits; s += 4) {
+    const f32x2 y = *reinterpret_cast<const f32x2*>(src + s * step + 4 + d);
+    x[0] = fmaf(y[0], f[s], x[0]);
+    x[1] = fmaf(y[1], f[s], x[1]);
   }
+  o[wave][lane] = x;
+  __syncthreads();
+  if (wave) return;
+  const float lt = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
   const int h = hk * group + r / a.nq, q = r - (r / a.nq) * a.nq;
   const float inv = lt == 0.f ? 0.f : 1.0f / lt;
   if (a.lse && lane == 0) a.lse[((size_t)b * a.H + h) * a.nq + q] = lt == 0.f ? INFINITY : M + __log2f(lt);
   if (lane * 2 >= a.dh) return;
-  const long long off = b * a.out_stride[0] + (long long)q * a.out_stride[1] + h * a.out_stride[2] + d;
-  bf16x2 x = {(bf16_t)(o0 * inv), (bf16_t)(o1 * inv)};
-  *reinterpret_cast<bf16x2*>((bf16_t*)a.out + off) = x;
-  if (a.out_lo) *reinterpret_cast<f32x2*>(a.out_lo + low_row(a, b, h, q) + d) = f32x2{o0 * inv - (float)x[0], o1 * inv - (float)x[1]};
+  const float o0 = ((o[0][lane][0] + o[1][lane][0]) + (o[2][lane][0] + o[3][lane][0])) * inv;
+  const float o1 = ((o[0][lane][1] + o[1][lane][1]) + (o[2][lane][1] + o[3][lane][1])) * inv;
+  const bf16x2 y = {(bf16_t)o0, (bf16_t)o1};
+  *reinterpret_cast<bf16x2*>((bf16_t*)a.out + b * a.out_stride[0] + (long long)q * a.out_stride[1] + h * a.out_stride[2] + d) = y;
+  if (a.out_lo) *reinterpret_cast<f32x2*>(a.out_lo + low_row(a, b, h, q) + d) = f32x2{o0 - (float)y[0], o1 - (float)y[1]};
 }
 
 __global__ __launch_bounds__(256) void zero_rows_kernel(bf16_t* x, int n, int t0, int ld, int chunks, long long total) {
@@ -1221,7 +1231,7 @@ long long span(const FactAttention& a) {
 // splits of the few-row kernel: enough workgroups to fill 256 CUs twice, at least 8 tiles (2 a wave) each
 int row_splits(const FactAttention& a) {
   const long long tiles = (span(a) + 31) / 32, wgs = (long long)a.B * a.Hkv;
-  long long s = std::min((512 + wgs - 1) / wgs, tiles / 8);
+  long long s = std::min((1536 + wgs - 1) / wgs, tiles / 8);
   return (int)std::max(1ll, std::min(s, 256ll));
 }
 
@@ -1274,7 +1284,7 @@ int fwd_t(const FactAttention& a, void* ws, hipStream_t s) {
     const size_t tab = (size_t)(a.H / a.Hkv) * (2 * a.rel_max_distance + 1) * 4;
     p.rowtab = REL && tab <= 16384;
     FACT_LAUNCH((rel_rows_kernel<DH, REL>), dim3(p.nwg), dim3(256), p.rowtab ? tab : 0, s, p);
-    if (p.splits > 1) FACT_LAUNCH(rel_join_kernel, dim3(a.B * a.H * a.nq), dim3(64), 0, s, p);
+    if (p.splits > 1) FACT_LAUNCH(rel_join_kernel, dim3(a.B * a.H * a.nq), dim3(256), 0, s, p);
     return launched();
   }
   p.nwg = p.qblocks * a.B * a.H;
