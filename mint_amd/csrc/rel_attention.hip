@@ -42,9 +42,12 @@ struct Geo {
   static constexpr int PC = KD * 4;         // chunks of a row in LDS
   static constexpr int IMG = 32 * PC * 8;   // one 32-row tile (elements)
 };
-// LDS tiles have no gaps (they are filled 64 chunks at a time); a row's chunks are permuted instead.  In units of 16 bytes, modulo
-// the 16 that all banks hold, the 16 rows of a fragment read start PC apart; what is left to tell apart are rows with the same
-// PC r mod 16, and the chunk's low bits do that.  8 rows of a transposed read, two chunks of each, differ in the other bits.
+// LDS tiles have no gaps (they are filled 64 chunks at a time); a row's chunks are permuted instead.  A cycle serves 16 chunks of
+// 16 bytes, one of each place modulo 16, and rows start PC apart, so rows with the same PC r mod 16 are told apart by `sw`:
+//   * a transposed read takes 8 consecutive rows at once, two chunks of each: u differs between them;
+//   * a fragment read takes rows 0 .. 3 and 12 .. 15 of one chunk with rows 4 .. 11 of its neighbour: the chunks that either set of
+//     rows moves to are whole pairs (u alike, v 0 and 1).
+// With u from row & 7 alone the second kind of read took twice the cycles, 30 % of all the LDS was busy.
 template <int DH>
 struct Swizzle {
   static constexpr int FREE = Geo<DH>::PC == 16 ? 0 : Geo<DH>::PC == 8 ? 1 : 2;  // rows' low bits that PC r tells apart
@@ -53,7 +56,7 @@ struct Swizzle {
 template <int DH>
 DEVINL int place(int row, int ch) {  // element of chunk ch of a row
   constexpr int FREE = Swizzle<DH>::FREE, MASK = Swizzle<DH>::MASK;
-  const int sw = ((row & 7) >> FREE << 1 | (row >> 3 & 1)) & MASK;
+  const int v = row >> 3 & 1, u = (row & 7) >> FREE ^ v << (2 - FREE), sw = u << 1 | v;
   return (row * Geo<DH>::PC + (ch & ~MASK) + ((ch & MASK) ^ sw)) * 8;
 }
 template <int DH>
