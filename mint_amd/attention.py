@@ -193,7 +193,9 @@ def attention(q, k, v, scale=None, window=None, sinks=0, rel_table=None, rel_map
     Query row i of sequence b stands at position q_start[b] + i (0 + i without q_start) and sees the keys j with j < kv_len[b],
     j <= position + window[1] and (j >= position - window[0] or j < sinks); a negative window side is open.  rel_table
     [buckets, H] fp32 adds rel_table[rel_map[clip(j - position)]][h] to scale * q . k.  A row that sees no key gives zeros.
-    Keys and values at and after kv_len are never read.  Returns out [B, nq, H, dh], with `training` (out, AttentionSaved)."""
+    What stands at keys and values that no row of their sequence sees (from kv_len on, behind the window, in a cache's free places)
+    reaches no result.  `out` may be q, and must not overlap k or v.  Returns out [B, nq, H, dh], with `training`
+    (out, AttentionSaved)."""
     options = _options(scale, window, sinks)
     held = (q, k, v, rel_table, rel_map, kv_len, q_start)
     key = _key("attention", held + (out,), options + (bool(training),))
@@ -240,7 +242,7 @@ def attention_backward(dout, q, k, v, out, saved, scale=None, window=None, sinks
                        q_start=None, dq=None, dk=None, dv=None):
     """Gradients of attention(..., training=True) for dout [B, nq, H, dh]: (dq, dk, dv), with a relative bias also the fp32
     gradient of rel_table.  `out` and `saved` are what the forward returned; dq, dk, dv may be given (views of one packed
-    gradient, for instance)."""
+    gradient, for instance; they must not overlap the inputs)."""
     _need(isinstance(saved, AttentionSaved), "saved must be what attention(training=True) returned")
     options = _options(scale, window, sinks)
     held = (q, k, v, rel_table, rel_map, kv_len, q_start)

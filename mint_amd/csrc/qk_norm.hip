@@ -346,7 +346,10 @@ int run(const FactQkNorm& a, bool backward, void* ws, hipStream_t s) {
 int qk_norm_check(const FactQkNorm& a, bool backward, const char** why) {
   auto bad = [&](int rc, const char* w) { *why = w; return rc; };
   if (a.B <= 0 || a.n <= 0 || a.H <= 0 || a.Hkv <= 0) return bad(-1, "B, n, H and Hkv must be positive");
-  if ((long long)a.H + a.Hkv > 65536 || (long long)a.B * a.n > (1ll << 32) || (long long)a.B * a.n * ((std::max(a.H, a.Hkv) + 7) / 8) > INT_MAX) return bad(-1, "too many tokens or heads");
+  // (pieces have at least 8 heads and workgroups 4 pieces; a launch has fewer than 2^32 threads, 256 a workgroup)
+  if ((long long)a.H + a.Hkv > 65536 || (long long)a.B * a.n > 1 << 26 ||
+      (long long)a.B * a.n * ((a.H + 7) / 8 + (a.Hkv + 7) / 8) > (1 << 26) - 8)
+    return bad(-1, "too many tokens or heads");
   if (a.dh < 8 || a.dh > 128 || a.dh % 8) return bad(-3, "unsupported head dim (a multiple of 8 up to 128)");
   if (a.rotary_dim < 0 || a.rotary_dim > a.dh || a.rotary_dim % 8) return bad(-1, "rotary_dim must be a multiple of 8 up to dh");
   if (a.dtype != 0 && a.dtype != 1) return bad(-1, "dtype must be 0 (bf16) or 1 (fp32)");

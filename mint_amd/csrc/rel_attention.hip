@@ -188,7 +188,15 @@ DEVINL int start_of(const FactAttention& a, int b) {
 // the 32-key tiles that positions pa .. pb can see: tiles 0 .. ns - 1 (sinks), then t0 .. t0 + (T - ns) - 1
 struct Tiles {
   int ns, t0, T;
+  int first, last, sinks;  // keys that any of them sees: first .. last, and up to last those below sinks
   DEVINL int at(int t) const { return t < ns ? t : t - ns + t0; }
+  // Rows of a tile that none of them sees are not read, as what is there may be no number, which a probability of zero does not
+  // cancel: another row of the tile is taken instead, and masked.
+  DEVINL bool whole(int row0) const { return (row0 >= first || row0 + 31 < sinks) && row0 + 31 <= last; }
+  DEVINL int row(int row0, int r) const {
+    const int j = min(row0 + r, last);
+    return (j < first && j >= sinks ? (row0 < sinks ? row0 : first) : j) - row0;
+  }
 };
 DEVINL Tiles tiles_of(const Vis& v, long long pa, long long pb) {
   const long long hi = min((long long)v.len, v.hi == INT_MAX ? (long long)v.len : pb + v.hi + 1);
@@ -198,6 +206,9 @@ DEVINL Tiles tiles_of(const Vis& v, long long pa, long long pb) {
   t.ns = hi > 0 ? (int)((min(hi, (long long)v.sinks) + 31) >> 5) : 0;
   t.t0 = max(t.ns, (int)(min(lo, 1ll << 30) >> 5));
   t.T = t.ns + (lo < hi ? max(0, t1 - t.t0) : 0);
+  t.first = (int)min(lo, 1ll << 30);
+  t.last = (int)hi - 1;
+  t.sinks = v.sinks;
   return t;
 }
 
@@ -218,8 +229,10 @@ DEVINL u32x4 load16(const bf16_t* base, unsigned off) {
 
 // ---- staging of two 32-row tiles (K and V, or Q and dO) into LDS --------------------------------------------------------
 // Loads that write LDS themselves, 16 bytes a lane and 64 consecutive places of a tile an instruction: no registers hold what is
-// in flight.  Each wave waits for its own before the barrier (__syncthreads alone does not).  The two buffers of a kernel are two objects, each named by half of the
-// unrolled loop: of one array with a computed half the compiler would wait for the loads in flight before each read.
+// in flight.  Each wave waits for its own before the barrier (__syncthreads alone does not).  The two buffers of a kernel are two
+// objects, each named by half of the unrolled loop: of one array with a computed half the compiler would wait for the loads in
+// flight before each read.  At B 8, H 12, n 1440, dh 128 with a bias dK/dV takes 350 us with them and 427 staged through registers;
+// a third buffer, with two tiles in flight, costs the workgroups it leaves no LDS for (354 instead of 263, forward 172 and 162).
 typedef __attribute__((address_space(3))) void lds_void;
 typedef __attribute__((address_space(1))) const void glb_void;
 template <int DH>
@@ -243,17 +256,17 @@ struct Stage {
 #pragma unroll
     for (int i = 0; i < N; ++i) off[i] = (unsigned)row(i) * (i * 4 + wave < PER ? lda : ldb) + chunk(i) * 16;
   }
-  // rows row0 .. row0 + 31 of a and b (wave-uniform pointers to row 0); rows past `last` repeat it: finite values, masked later
-  DEVINL void load(bf16_t* lds, const bf16_t* a, const bf16_t* b, int row0, int last) const {
+  // rows row0 .. row0 + 31 of a and b (wave-uniform pointers to row 0)
+  DEVINL void load(bf16_t* lds, const bf16_t* a, const bf16_t* b, int row0, const Tiles& t) const {
     a += (long long)row0 * (lda / 2);
     b += (long long)row0 * (ldb / 2);
-    const int in = last - row0;
-    if (in >= 31) {
+    if (t.whole(row0)) {
 #pragma unroll
       for (int i = 0; i < N; ++i) one(lds, a, b, i, off[i]);
     } else {
 #pragma unroll
-      for (int i = 0; i < N; ++i) one(lds, a, b, i, off[i] - (unsigned)max(0, row(i) - in) * (i * 4 + wave < PER ? lda : ldb));
+      for (int i = 0; i < N; ++i)
+        one(lds, a, b, i, off[i] + (unsigned)(t.row(row0, row(i)) - row(i)) * (i * 4 + wave < PER ? lda : ldb));
     }
   }
   DEVINL void one(bf16_t* lds, const bf16_t* a, const bf16_t* b, int i, unsigned o) const {
@@ -313,7 +326,7 @@ __global__ __launch_bounds__(256, 2) void rel_fwd_kernel(const RelP p) {
   st.init(a.k_stride[1], a.v_stride[1], wave, lane);
   pad_zero<DH>(buf0, tid);
   pad_zero<DH>(buf1, tid);
-  if (tl.T > 0) st.load(buf0, kp, vp, tl.at(0) * 32, v.len - 1);
+  if (tl.T > 0) st.load(buf0, kp, vp, tl.at(0) * 32, tl);
   if (REL) load_bias(eb, p, h, tid, 256);
   f32x4 O[ND];
   float m = -INFINITY, l = 0.f;
@@ -341,7 +354,7 @@ __global__ __launch_bounds__(256, 2) void rel_fwd_kernel(const RelP p) {
     } else {
       s[0] = s[1] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    if (t + 1 < tl.T) st.load(other, kp, vp, tl.at(t + 1) * 32, v.len - 1);  // (after the reads of the bias: they would wait for it)
+    if (t + 1 < tl.T) st.load(other, kp, vp, tl.at(t + 1) * 32, tl);  // (after the reads of the bias: they would wait for it)
     if (skip) return;
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
@@ -549,7 +562,7 @@ __global__ __launch_bounds__(256, DH > 96 ? 3 : 4) void rel_dq_kernel(const RelP
   st.init(a.k_stride[1], a.v_stride[1], wave, lane);
   pad_zero<DH>(buf0, tid);
   pad_zero<DH>(buf1, tid);
-  if (tl.T > 0) st.load(buf0, kp, vp, tl.at(0) * 32, v.len - 1);
+  if (tl.T > 0) st.load(buf0, kp, vp, tl.at(0) * 32, tl);
   const int q = min(q0 + c, a.nq - 1);
   const bool live = (q0 + c < a.nq) & !v.lone(start + q);  // a query of the call that sees more than one key
   Frag<DH> Q, dO;
@@ -626,7 +639,7 @@ __global__ __launch_bounds__(256, DH > 96 ? 3 : 4) void rel_dq_kernel(const RelP
     } else {
       s[0] = s[1] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    if (t + 1 < tl.T) st.load(other, kp, vp, tl.at(t + 1) * 32, v.len - 1);  // (after the reads of the bias: they would wait for it)
+    if (t + 1 < tl.T) st.load(other, kp, vp, tl.at(t + 1) * 32, tl);  // (after the reads of the bias: they would wait for it)
     if (skip) return;
     f32x4 ds[2];
 #pragma unroll
@@ -818,10 +831,11 @@ __global__ __launch_bounds__(256, dkdv_slots(DH)) void rel_dkdv_kernel(const Rel
   at.init(lane);
   Stage<DH> st;
   st.init(a.q_stride[1], a.dout_stride[1], wave, lane);
+  const Tiles all = {0, 0, 0, 0, a.nq - 1, 0};
   auto load = [&](int hh, int qt, bf16_t* buf) __attribute__((always_inline)) {  // head hh of the group, its query tile t0 + qt
     const int h = hk * group + hh, q0 = (t0 + qt) * 32;
     st.load(buf, (const bf16_t*)a.q + b * a.q_stride[0] + h * a.q_stride[2],
-            (const bf16_t*)a.dout + b * a.dout_stride[0] + h * a.dout_stride[2], q0, a.nq - 1);
+            (const bf16_t*)a.dout + b * a.dout_stride[0] + h * a.dout_stride[2], q0, all);
     if (wave == 0) {
       int l = lane;
       asm("" : "+v"(l));  // (the addresses are made here, not kept)
@@ -1008,12 +1022,13 @@ __global__ __launch_bounds__(256, 2) void rel_rows_kernel(const RelP p) {
   } tile[DEPTH];
   const unsigned ldk = (unsigned)a.k_stride[1] * 2, ldv = (unsigned)a.v_stride[1] * 2;
   auto load = [&](Tile& x, int t) {
-    const int j0 = tl.at(t) * 32, cut = j0 + 31 - (v.len - 1);  // > 0: rows past the last repeat it
+    const int j0 = tl.at(t) * 32;
+    const bool whole = tl.whole(j0);
     const bf16_t* k0 = kb + (long long)j0 * a.k_stride[1];
     const bf16_t* v0 = vb + (long long)j0 * a.v_stride[1];
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
-      const unsigned r = cut > 0 ? min(ks * 16 + c, 31 - cut) : ks * 16 + c;
+      const unsigned r = whole ? ks * 16 + c : tl.row(j0, ks * 16 + c);
 #pragma unroll
       for (int kd = 0; kd < G::KD; ++kd) {
         x.K[ks].f[kd] = zero_bf16x8();
@@ -1024,7 +1039,7 @@ __global__ __launch_bounds__(256, 2) void rel_rows_kernel(const RelP p) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int q = lane + i * 64, r = q / G::CH, ch = q - r * G::CH;
-      x.vr[i] = load16(v0, (unsigned)(cut > 0 ? min(r, 31 - cut) : r) * ldv + ch * 16);
+      x.vr[i] = load16(v0, (unsigned)(whole ? r : tl.row(j0, r)) * ldv + ch * 16);
     }
   };
   f32x4 O[ND];
@@ -1240,6 +1255,8 @@ int row_splits(const FactAttention& a) {
 
 size_t up16(size_t x) { return (x + 15) & ~(size_t)15; }
 
+constexpr long long SLOTS = 768;  // workgroups that run at once at dh 128 (more do at smaller ones; cut for 1024, they take longer)
+
 RelP params(const FactAttention& a) {
   RelP p;
   p.a = a;
@@ -1261,8 +1278,11 @@ RelP params(const FactAttention& a) {
   if (a.window_left >= 0 && a.window_right >= 0)
     seen = std::min<long long>(seen, (long long)BLOCK_KEYS + a.window_left + a.window_right + 62);
   const long long t = (seen + 31) / 32 * group, blocks = (long long)a.B * a.Hkv * p.kblocks;
-  p.chunks = (int)std::max(1ll, std::min((768 + blocks / 2) / blocks, t / 4));
-  const long long piece = std::max(8ll, (t + p.chunks - 1) / p.chunks);
+  p.chunks = (int)std::max(1ll, std::min((SLOTS + blocks / 2) / blocks, t / 4));
+  // blocks with sinks, which all later queries see: pieces as long as the other blocks', or, where there is much other work to
+  // run beside them, a quarter of a workgroup slot's share of the whole
+  const long long share = ((long long)(p.kblocks - p.sblocks) * t + p.sblocks * all) * a.B * a.Hkv / (4 * SLOTS);
+  const long long piece = std::max({8ll, (t + p.chunks - 1) / p.chunks, share});
   p.schunks = (int)std::max<long long>(p.chunks, std::min(all / piece, 64ll));
   return p;
 }
@@ -1344,8 +1364,10 @@ int rel_attention_check(const FactAttention& a, bool backward, const char** why)
   if (a.H % a.Hkv) return bad(-1, "H must be a multiple of Hkv");
   if (a.dh != 32 && a.dh != 64 && a.dh != 80 && a.dh != 96 && a.dh != 128)
     return bad(-3, "unsupported head dim (supported: 32, 64, 80, 96, 128)");
-  if ((long long)a.B * a.H > INT_MAX / 256 || ((long long)a.nq + 63) / 64 * a.B * a.H > INT_MAX / 4 ||
-      ((long long)a.nk + 63) / 64 * a.B * a.Hkv > INT_MAX / 512)
+  // (a launch has fewer than 2^32 threads, 256 a workgroup)
+  const long long most = (1 << 24) - 1, heads = (long long)a.B * a.H;
+  if (heads > most || (a.nq + 63ll) / 64 * heads > most || (few_rows(a) && a.nq * heads > most) ||
+      (backward && (a.nk + 63ll) / 64 * a.B * a.Hkv > most / 64))
     return bad(-1, "too many heads and blocks for one launch");
   if (!(a.scale >= 5.9604645e-8f) || !(a.scale <= 3.0e38f)) return bad(-1, "scale must be finite and at least 2^-24");
   if (a.sinks < 0) return bad(-1, "sinks must not be negative");
@@ -1368,6 +1390,9 @@ int rel_attention_check(const FactAttention& a, bool backward, const char** why)
       if (t[i].out && t[i].st[k] == 0 && n[k] > 1) return bad(-1, "an output must not be broadcast");
     }
   }
+  for (int i = 0; i < (backward ? 8 : 4); ++i)
+    for (int k = 0; k < i; ++k)
+      if (t[i].p == t[k].p && (t[i].out || t[k].out) && !(i == 3 && k == 0)) return bad(-1, "an output must not be another tensor");
   if ((uintptr_t)a.out_lo & 15) return bad(-1, "tensors must be 16-byte aligned");
   if (backward && !a.lse) return bad(-1, "the backward needs the forward's lse");
   if (backward && a.rel_table && !a.drel) return bad(-1, "the backward with rel_table needs drel");

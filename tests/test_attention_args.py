@@ -64,7 +64,8 @@ def test_struct_sizes_match_the_header(lib, tmp_path):
     (dict(q=None), -1, "null"), (dict(v=4096 + 8), -1, "aligned"), (dict(out_lo=4096 + 2), -1, "aligned"),
     (dict(k_stride=(24 * 128, 132, 64)), -1, "multiples of 8"), (dict(dq_stride=(8 * 256, 0, 64)), -1, "broadcast"),
     (dict(v_stride=(1 << 40, (1 << 25) + 8, 64)), -1, "2^25"), (dict(q_stride=(1 << 40, -64, 64)), -1, "2^25"),
-    (dict(dk_stride=(0, 128, 64)), -1, "broadcast"), (dict(lse=None), -1, "lse"),
+    (dict(dk_stride=(0, 128, 64)), -1, "broadcast"), (dict(dq=4096), -1, "another tensor"), (dict(dk=8 * 4096, dv=8 * 4096), -1, "another tensor"),
+    (dict(dv=6 * 4096), -1, "another tensor"), (dict(B=1 << 19, nk=64 * 64), -1, "too many"), (dict(nq=1 << 29, B=1 << 3), -1, "too many"), (dict(lse=None), -1, "lse"),
     (dict(BIAS, rel_map=None), -1, "rel_map"), (dict(BIAS, rel_buckets=0), -1, "rel_buckets"),
     (dict(BIAS, rel_buckets=257), -1, "rel_buckets"), (dict(BIAS, rel_max_distance=0), -1, "rel_max_distance"),
     (dict(BIAS, rel_max_distance=1025), -1, "rel_max_distance"), (dict(BIAS, drel=None), -1, "drel")])
@@ -93,6 +94,23 @@ def test_attention_asks_for_its_workspace(lib):
     assert lib.fact_attention_workspace(None, 0, C.byref(n)) == -1 and lib.fact_attention(None, None, 0, None) == -1
 
 
+def test_an_output_is_not_an_input(lib):
+    n = C.c_size_t(0)
+    for name in ("k", "v"):
+        a = _attention(out=getattr(_attention(), name))
+        assert lib.fact_attention_workspace(C.byref(a), 0, C.byref(n)) == -1 and "another tensor" in lib.fact_last_error().decode()
+    assert lib.fact_attention_workspace(C.byref(_attention(out=4096)), 0, C.byref(n)) == 0  # in place of q
+
+
+def test_workspace_of_blocks_with_sinks_stays_small(lib):
+    """The partial sums of the blocks that all queries see are bounded by the work that runs beside them."""
+    n = C.c_size_t(0)
+    for B, H, nq in ((1, 4, 16384), (32, 12, 16384), (4, 12, 1440), (1, 1, 1 << 20)):
+        a = _attention(B=B, H=H, Hkv=H, nq=nq, nk=nq, dh=128, window_left=255, window_right=0, sinks=4)
+        assert lib.fact_attention_workspace(C.byref(a), 1, C.byref(n)) == 0
+        assert n.value <= 4 * B * H * nq + (1 << 28), (B, H, nq, n.value)
+
+
 def _norm(**kw):
     a = L.FactQkNorm(B=2, n=8, H=4, Hkv=2, dh=64, rotary_dim=64, base=10000.0, eps=1e-6)
     for i, n in enumerate(("q", "k", "q_out", "k_out", "dq_out", "dk_out", "dq", "dk")):
@@ -108,6 +126,7 @@ def _norm(**kw):
 
 @pytest.mark.parametrize("kw,rc,word", [
     (dict(B=0), -1, "positive"), (dict(Hkv=0), -1, "positive"), (dict(n=1 << 30, B=1 << 10), -1, "too many"),
+    (dict(n=1 << 16, B=1 << 10), -1, "too many"),
     (dict(dh=132), -3, "head dim"), (dict(dh=20), -3, "head dim"), (dict(rotary_dim=72), -1, "rotary_dim"),
     (dict(rotary_dim=-8), -1, "rotary_dim"), (dict(rotary_dim=12), -1, "rotary_dim"), (dict(dtype=2), -1, "dtype"),
     (dict(eps=-1.0), -1, "eps"), (dict(eps=math.nan), -1, "eps"), (dict(base=0.0), -1, "base"), (dict(base=math.nan), -1, "base"),
@@ -170,7 +189,7 @@ def test_operator_sources_hold_nothing_that_a_graph_cannot_replay():
 
 
 def _model_cfg(**at):
-    st = lambda seq, feat: L.FactStackCfg(seq, feat, 800, 2, 10, 3072)
+    st = lambda seq, feat: L.FactStackCfg(seq, feat, 800, 2, 10, 1600)
     cfg = L.FactConfig(st(120, 225), st(240, 35), st(0, 0), 225, 1e-5)
     return cfg, (L.FactAttnCfg * 3)(L.FactAttnCfg(), L.FactAttnCfg(), L.FactAttnCfg(**at))
 

@@ -197,6 +197,32 @@ def test_ragged_batch_with_empty_sequences_and_garbage_past_the_end(bias):
     _check(q, k, v, 0.125, window=(12, 2), sinks=1, **kw)  # later rows see nothing but the sink, or nothing at all
 
 
+@pytest.mark.parametrize("nq,nk,start,window,sinks", [(1, 500, 333, (-1, 0), 0), (1, 500, 333, (40, 0), 3), (2, 70, 40, (5, 0), 0),
+                                                      (100, 400, 250, (60, 0), 4), (100, 400, 250, (-1, 0), 0), (64, 300, 100, (20, 9), 0),
+                                                      (150, 800, 500, (-1, -1), 0), (40, 500, 300, (33, 0), 70), (17, 90, -5, (3, 2), 0)])
+@pytest.mark.parametrize("bias", [False, True])
+def test_keys_that_no_query_sees_may_hold_anything(nq, nk, start, window, sinks, bias):
+    """Places of a cache that are not written yet, or have left the window: nothing of them reaches a result."""
+    gen = torch.Generator().manual_seed(nq + nk)
+    B, H, Hkv, dh = 2, 4, 2, 80
+    q, k, v = _rand(gen, B, nq, H, dh), _rand(gen, B, nk, Hkv, dh), _rand(gen, B, nk, Hkv, dh)
+    kw = dict(window=window, sinks=sinks, q_start=torch.tensor([start, start + 3], dtype=torch.int32, device=DEV))
+    if bias:
+        kw["rel_table"], kw["rel_map"] = _table(gen, H)
+    hidden = ~_seen(B, nq, nk, window, sinks, None, kw["q_start"])[0].any(1)
+    assert hidden.any() or window == (-1, -1)
+    zk, zv = (t.masked_fill(hidden[:, :, None, None], 0.0) for t in (k, v))
+    k[hidden], v[hidden] = float("nan"), float("inf")
+    do = _rand(gen, B, nq, H, dh)
+    want, ws = A.attention(q, zk, zv, training=True, **kw)
+    got, gs = A.attention(q, k, v, training=True, **kw)
+    assert torch.equal(got, want) and torch.equal(gs.lse, ws.lse)
+    for x, y in zip(A.attention_backward(do, q, k, v, got, gs, **kw), A.attention_backward(do, q, zk, zv, want, ws, **kw)):
+        assert torch.equal(x, y)
+    assert torch.equal(A.attention(q, k, v, **kw), A.attention(q, zk, zv, **kw))
+    _check(q, zk, zv, dh ** -0.5, **kw)
+
+
 def test_lengths_out_of_range_are_clamped():
     gen = torch.Generator().manual_seed(4)
     q, k, v = (_rand(gen, 3, 20, 1, 32) for _ in range(3))
@@ -266,6 +292,10 @@ def test_strides_packed_views_broadcast_and_unaligned_inputs():
     assert torch.equal(A.attention(q, wide, v), base)
     one = k[:, :, :1].expand(B, n, H, dh)  # a broadcast key head
     assert torch.equal(A.attention(q, one, v), A.attention(q, one.contiguous(), v))
+    for nq in (75, 3):  # in place of the queries
+        x = q[:, :nq].contiguous()
+        want = A.attention(x, k, v)
+        assert A.attention(x, k, v, out=x).data_ptr() == x.data_ptr() and torch.equal(x, want)
     # packed destinations; nothing around them is touched
     dst = torch.full((B, n, 3, H, dh), 7.0, dtype=torch.bfloat16, device=DEV)
     base, _ = A.attention(q.contiguous(), k.contiguous(), v.contiguous(), training=True)
