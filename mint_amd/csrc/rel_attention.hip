@@ -156,13 +156,16 @@ struct Vis {
     const int d = j - p;  // (selects, no branches: hipcc dropped one of the branchy form's stores)
     return (j < len) & (d <= hi) & ((d >= lo) | (j < sinks));
   }
+  DEVINL int count(int p) const {  // of keys that position p sees (saturating sums: hi may be the largest int, lo the smallest)
+    const int top = min(len, __builtin_elementwise_add_sat(__builtin_elementwise_add_sat(p, hi), 1));
+    const int low = max(0, __builtin_elementwise_add_sat(p, lo)), sk = min(sinks, top);
+    return max(0, top - max(low, sk)) + max(0, sk);
+  }
   // sees one key only: its softmax is 1 whatever the score, its dS exactly 0 (which P (dP - D) misses by a rounding).  Such a
   // row never lies in a tile that is full.
-  DEVINL bool lone(int p) const {
-    const long long top = min((long long)len, hi == INT_MAX ? (long long)len : (long long)p + hi + 1);
-    const long long low = lo == INT_MIN ? 0 : max(0ll, (long long)p + lo), sk = min((long long)sinks, top);
-    return max(0ll, top - max(low, sk)) + max(0ll, sk) == 1;
-  }
+  DEVINL bool lone(int p) const { return count(p) == 1; }
+  // whether one of p .. p + n - 1 may be such a row: over positions the count rises, stays and falls
+  DEVINL bool any_lone(int p, int n) const { return count(p) < 2 || count(p + n - 1) < 2; }
   // keys j0 .. j0 + W - 1 against positions p0 .. p0 + R - 1
   template <int W = 32, int R = 32>
   DEVINL bool none(int j0, int p0) const {
@@ -243,7 +246,7 @@ struct Stage {
   unsigned lda, ldb;  // bytes
   int wave, lane;
   DEVINL int tile(int i) const { return i * 4 + wave < PER ? i * 4 + wave : i * 4 + wave - PER; }
-  DEVINL int row(int i) const { return (tile(i) * 64 + lane) / G::PC; }
+  DEVINL int row(int i, int l) const { return (tile(i) * 64 + l) / G::PC; }
   DEVINL int chunk(int i) const {  // (the permutation is its own inverse)
     const int n = tile(i) * 64 + lane, r = n / G::PC;
     return place<DH>(r, n - r * G::PC) / 8 - r * G::PC;
@@ -254,7 +257,7 @@ struct Stage {
     wave = w;
     lane = l;
 #pragma unroll
-    for (int i = 0; i < N; ++i) off[i] = (unsigned)row(i) * (i * 4 + wave < PER ? lda : ldb) + chunk(i) * 16;
+    for (int i = 0; i < N; ++i) off[i] = (unsigned)row(i, l) * (i * 4 + wave < PER ? lda : ldb) + chunk(i) * 16;
   }
   // rows row0 .. row0 + 31 of a and b (wave-uniform pointers to row 0)
   DEVINL void load(bf16_t* lds, const bf16_t* a, const bf16_t* b, int row0, const Tiles& t) const {
@@ -264,9 +267,11 @@ struct Stage {
 #pragma unroll
       for (int i = 0; i < N; ++i) one(lds, a, b, i, off[i]);
     } else {
+      int l = lane;
+      asm("" : "+v"(l));  // (rows are worked out here, where they are seldom needed, and hold no registers)
 #pragma unroll
       for (int i = 0; i < N; ++i)
-        one(lds, a, b, i, off[i] + (unsigned)(t.row(row0, row(i)) - row(i)) * (i * 4 + wave < PER ? lda : ldb));
+        one(lds, a, b, i, off[i] + (unsigned)(t.row(row0, row(i, l)) - row(i, l)) * (i * 4 + wave < PER ? lda : ldb));
     }
   }
   DEVINL void one(bf16_t* lds, const bf16_t* a, const bf16_t* b, int i, unsigned o) const {
@@ -908,8 +913,14 @@ __global__ __launch_bounds__(256, dkdv_slots(DH)) void rel_dkdv_kernel(const Rel
           const int q = qs * 16 + 4 * g + r;
           const bool ok = v.seen(j0 + c, p0 + q) & (q0 + q < a.nq);
           pr[qs][r] = ok ? pr[qs][r] : 0.f;
-          dp[qs][r] = (ok & !v.lone(p0 + q)) ? dp[qs][r] : 0.f;
+          dp[qs][r] = ok ? dp[qs][r] : 0.f;
         }
+      if (v.any_lone(p0, 32)) {
+#pragma unroll
+        for (int qs = 0; qs < 2; ++qs)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) dp[qs][r] = v.lone(p0 + qs * 16 + 4 * g + r) ? 0.f : dp[qs][r];
+      }
     }
     const bf16x8 pb = pack8(pr[0], pr[1]), db = pack8(dp[0], dp[1]);
 #pragma unroll
