@@ -795,7 +795,7 @@ DEVINL KBlock kblock_of(const RelP& p, int id) {
 // 45.8 us instead of 29.8; B 4, H 12, n 1440, window 257: 57 instead of 38; B 8, H 12, n 1440, all keys: 186 instead of 176
 // (dh 80: 222 and 214, dh 32: 115 and 132, where nothing else gains).
 constexpr int BLOCK_KEYS = 64;
-constexpr int dkdv_slots(int dh) { return dh < 96 ? 4 : 3; }  // workgroups of a CU
+constexpr int dkdv_slots(int dh) { return dh <= 96 ? 4 : 3; }  // workgroups of a CU
 template <int DH, bool REL>
 __global__ __launch_bounds__(256, dkdv_slots(DH)) void rel_dkdv_kernel(const RelP p) {
   using G = Geo<DH>;
