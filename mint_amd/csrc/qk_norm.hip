@@ -3,7 +3,9 @@
 //
 // Forward   r = rsqrt(mean x^2 + eps), y = x r gamma, z = R(pos) y
 // Backward  dy = R(pos)^T dz, dgamma = sum dy x r, dx = r (gamma dy - x r mean(gamma dy x r))
-// Both read each value once and write each result once, so the rate of the copy they amount to bounds them.  A head of dh
+// Both read each value once and write each result once, so the rate of the copy they amount to bounds them: fp32, B 8, n 1440,
+// 24 heads of 128 takes 54 us forward (5.2 TB/s) and 91 + 5 backward (4.6 TB/s); bf16, B 16, n 360, 20 heads of 80, which caches
+// hold, 12 and 17.5 + 4; one token of 32 sequences 4.  A head of dh
 // values is held by dh / 8 lanes of a group of GL = 4, 8 or 16 (its row sums stay inside a 16-lane row); a lane holds 4 pairs
 // of one rotation slot, so the partner of every value is in the same lane.  A wave takes heads of one token, of the queries or
 // of the keys: the angles, reduced in double (a far position times a frequency loses whole turns in 32 bits), are computed once

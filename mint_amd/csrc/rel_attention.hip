@@ -298,7 +298,11 @@ DEVINL void load_bias(float* eb, const RelP& p, int h, int tid, int nthr) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// forward: workgroup = 64 queries of one head, 4 waves x 16; 32-key tiles double-buffered in LDS
+// forward: workgroup = 64 queries of one head, 4 waves x 16; 32-key tiles double-buffered in LDS.  One pass over the keys:
+//   m' = max(m, s);  l' = l 2^(m - m') + sum 2^(s - m');  O' = O 2^(m - m') + P V;  out = O / l
+// Bound by vector instructions (60 % of a SIMD's issue with a bias; LDS 20 %, matrix pipe below 30 %).  With 32 queries a wave each
+// K and V fragment feeds two products, but half as many waves fit, and a block's edge tiles are twice as many: B 4, H 12, n 1440,
+// dh 128, window 257 takes 40 us instead of 29, B 8, H 12, n 1440, dh 128, all keys 172 instead of 159.
 // ---------------------------------------------------------------------------------------------------------------------
 // EXACT (a.out_lo given): the probabilities enter P V as a sum of three bf16 values, 24 bits, and the output's rounding residual
 // is kept in fp32.  The backward takes D = rowsum(dO . O) from them: from the rounded P and O it is off by 1e-3 of itself, which
@@ -460,7 +464,7 @@ __global__ __launch_bounds__(256, 2) void rel_fwd_kernel(const RelP p) {
 //     what leaves on that side belongs to the sub-tile at d + 16.
 // Key tiles are visited in ascending order, so a distance is complete after its two neighbours, and row 0 stores 16 of them at a
 // time, each once per 16 queries.  At B 8, H 12, n 1440, dh 128 dQ takes 735 us with an LDS add per value, 300 with one per
-// folded row (its four rows meet in the same words), 177 without any sums and 214 with this.
+// folded row (its four rows meet in the same words), 177 without any sums and 214 with this (32 queries a wave).
 template <int CTRL, int BANKS = 0xf>
 DEVINL float moved(float y) {  // y moved inside rows of 16 lanes; zero from outside and in lanes of other banks of 4
   return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, y), CTRL, 0xf, BANKS, true));
@@ -538,6 +542,8 @@ struct Diagonals {
 // ---------------------------------------------------------------------------------------------------------------------
 // backward dQ and the bias gradient: workgroup = 64 queries of one head, 16 a wave
 //   P = exp2(S c - L);  dP = V dO^T;  dS = P (dP - D), D = rowsum(dO . O);  dQ^T += K^T dS;  dbias[j - p] += dS
+// Bound by instruction issue and the tile's dependent chain (vector 45 %, LDS 25 %, matrix pipe 25 %).  32 queries a wave: 49 us
+// instead of 38 (B 4, H 12, n 1440, dh 128, window 257), 231 instead of 237 where nothing but full tiles is left (B 8, all keys).
 // ---------------------------------------------------------------------------------------------------------------------
 template <int DH, bool REL>
 __global__ __launch_bounds__(256, DH > 96 ? 3 : 4) void rel_dq_kernel(const RelP p) {
@@ -713,7 +719,8 @@ __global__ __launch_bounds__(256, DH > 96 ? 3 : 4) void rel_dq_kernel(const RelP
   }
 }
 
-// drel[bucket][h], a workgroup each: the distances of the bucket, listed in order, over the batch and the query blocks
+// drel[bucket][h], a workgroup each: the distances of the bucket, listed in order, over the batch and the query blocks.  B 8, H 12,
+// n 1440, 64 buckets of 1025 distances: 9 MB in 15 us, as long as its largest bucket takes.
 __global__ __launch_bounds__(256) void rel_dtable_kernel(const RelP p) {
   const FactAttention& a = p.a;
   const int D = a.rel_max_distance, n = 2 * D + 1, h = blockIdx.x, bu = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -790,10 +797,10 @@ DEVINL KBlock kblock_of(const RelP& p, int id) {
   return k;
 }
 
-// A wave has 16 keys and its four sums fit the registers of 4 (dh 96 and 128: 3) workgroups a CU.  With 32 keys a wave every Q
-// and dO fragment feeds two products, but two workgroups a CU are left: dh 64, B 2, H 12 on 4 key heads, n 2047, window 256 takes
-// 45.8 us instead of 29.8; B 4, H 12, n 1440, window 257: 57 instead of 38; B 8, H 12, n 1440, all keys: 186 instead of 176
-// (dh 80: 222 and 214, dh 32: 115 and 132, where nothing else gains).
+// A wave has 16 keys and its four sums fit the registers of 4 (dh 128: 3) workgroups a CU.  With 32 keys a wave every Q and dO
+// fragment feeds two products, but two workgroups a CU are left: dh 64, B 2, H 12 on 4 key heads, n 2047, window 256 took 45.8 us
+// against 29.8; B 4, H 12, n 1440, window 257: 57 against 38; B 8, H 12, n 1440, all keys: 186 against 176 (dh 80: 222 and 214,
+// dh 32: 115 and 132, the one that lost).  What is left is latency: vector issue 40 %, LDS 27 %, matrix pipe 18 %.
 constexpr int BLOCK_KEYS = 64;
 constexpr int dkdv_slots(int dh) { return dh <= 96 ? 4 : 3; }  // workgroups of a CU
 template <int DH, bool REL>
@@ -990,7 +997,9 @@ __global__ __launch_bounds__(256) void rel_join_dkdv_kernel(const RelP p) {
 
 // ---------------------------------------------------------------------------------------------------------------------
 // few rows: all nq * group <= 16 query rows of one key head are the 16 columns of a score tile; the waves of a workgroup and
-// the splits of a head take different key tiles and are joined by their maxima and sums at the end
+// the splits of a head take different key tiles and are joined by their maxima and sums at the end.  Bound by the reads of K and V:
+// 4 sequences of 16384 .. 32767 keys, H 10, dh 80 (315 MB) take 72 us, 4.4 TB/s; a small call (B 32, H 10, 360 keys, 37 MB) 12.4 us,
+// of which a third is the chain of length, tile, score, probability, output and join.
 // ---------------------------------------------------------------------------------------------------------------------
 template <int DH, bool REL>
 __global__ __launch_bounds__(256, 2) void rel_rows_kernel(const RelP p) {
@@ -1257,7 +1266,9 @@ long long span(const FactAttention& a) {
   return std::min<long long>(a.nk, (long long)a.window_left + right + a.nq + a.sinks + 62);
 }
 
-// splits of the few-row kernel: enough workgroups to fill 256 CUs twice, at least 8 tiles (2 a wave) each
+// splits of the few-row kernel: up to 1536 workgroups - of sequences of 16384 to 32767 keys at B 4, H 10, dh 80 the rows take 72 us,
+// with 512 (as many as run at once) 77, the longest sequence's being the last - of at least 8 tiles (2 a wave) each: with half as
+// many tiles a workgroup, B 32 and 4 key heads over 1028 keys of dh 128 take 20 us instead of 17.5
 int row_splits(const FactAttention& a) {
   const long long tiles = (span(a) + 31) / 32, wgs = (long long)a.B * a.Hkv;
   long long s = std::min((1536 + wgs - 1) / wgs, tiles / 8);
