@@ -97,6 +97,7 @@ struct Stack {
   FactAttnCfg at = {};      // attention options
   int32_t* rel_map = nullptr;
   char* attn_ws = nullptr;  // forward workspace (few query rows)
+  size_t attn_bytes = 0;
   bool ext() const { return at.window > 0 || at.rel_buckets > 0; }  // runs rel_attention.hip
   float* out() { return L ? la[L - 1].x_out : x0; }
 };
@@ -167,6 +168,7 @@ struct BwScratch {
   bf16_t* dorow = nullptr;   // per-head dO rows
   float* dsum = nullptr;     // rowsum(dO o O)
   char* attn_ws = nullptr;   // workspace of the attention options' backward kernels
+  size_t attn_bytes = 0;
   float* ln_ws = nullptr;    // LayerNorm-backward per-block partial column sums (fused-kernel path)
   // buffers both the dgrad chain and the wgrad stream touch, indexed by layer parity q = layer count % 3
   bf16_t* dpre_pp[kBwBuf] = {};   // [M][ff pitch]
@@ -565,14 +567,21 @@ FactQkNorm ext_norm(FactHandle* h, const Stack& st, const LayerP& p, const Layer
   f.dgamma_accumulate = 1;
   return f;
 }
-// bytes of the largest workspace a stack's attention options ask for
+// Bytes of the largest workspace a stack's attention options ask for in any call the handle takes: up to B sequences, any number of
+// query rows.  (Not what the largest call asks for: fewer blocks are cut into more pieces.  What depends on the rows beyond growing
+// with them goes by their 32-row tiles, or by the few-row kernel's limit of 16.)
 size_t ext_ws(FactHandle* h, const Stack& st, int B, bool backward) {
   size_t need = 0;
-  if (st.ext() && st.L)
-    for (int nq = backward ? st.n : 1; nq <= st.n; nq = (nq < 32 && nq + 1 < st.n) ? nq + 1 : (nq < st.n ? st.n : st.n + 1)) {
-      FactAttention f = ext_attn(h, st, st.lp[0], st.la[0], B, nq);
-      need = std::max(need, rel_attention_ws(f, backward));
-    }
+  if (st.ext() && st.L) {
+    FactAttention f = ext_attn(h, st, st.lp[0], st.la[0], B, st.n);
+    for (f.B = 1; f.B <= B; ++f.B)
+      for (f.nq = backward ? 32 : 1; f.nq < st.n + 32 && (backward || f.nq <= 16); f.nq += backward ? 32 : 1) {
+        const int nq = f.nq;
+        f.nq = std::min(nq, st.n);
+        need = std::max(need, rel_attention_ws(f, backward));
+        f.nq = nq;
+      }
+  }
   if (st.at.qk_norm && st.L && backward) need = std::max(need, qk_norm_ws(ext_norm(h, st, st.lp[0], st.la[0], B), true));
   return need;
 }
@@ -618,7 +627,7 @@ void layout_stack_acts(FactHandle* h, Bump& b, Stack& st, int B) {
     st.la[l] = a;
   }
   if (st.at.rel_buckets > 0) st.rel_map = b.take<int32_t>((size_t)2 * st.at.rel_max_distance + 1);
-  if (st.ext()) st.attn_ws = b.take<char>(ext_ws(h, st, B, false));
+  if (st.ext()) st.attn_ws = b.take<char>(st.attn_bytes = ext_ws(h, st, B, false));
 }
 
 void layout_work(FactHandle* h, Bump& b) {
@@ -695,7 +704,7 @@ void layout_work(FactHandle* h, Bump& b) {
       size_t aw = 0;
       if (c) aw = ext_ws(h, h->motion, B, true);
       else for (const Stack* st : sts) aw = std::max(aw, ext_ws(h, *st, B, true));
-      sc.attn_ws = b.take<char>(aw);
+      sc.attn_ws = b.take<char>(sc.attn_bytes = aw);
       sc.ln_ws = b.take<float>(ln_bwd_ws_floats((int)Mx, d));
       if (c) {  // chain 1 queues its weight gradients behind its own dgrad chain: own slabs
         sc.slab = b.take<float>((size_t)6 * rups((size_t)d * (ffmax > 3 * d ? ffmax : 3 * d), 4));
@@ -1068,7 +1077,9 @@ hipStream_t side_of(FactHandle* h, hipStream_t s) { return (h->use_side && h->si
 int attn_forward(FactHandle* h, Stack& st, const LayerP& p, const LayerA& a, int B, int nq, hipStream_t s) {
   if (st.at.qk_norm) CHK(launch_qk_norm_fwd(ext_norm(h, st, p, a, B), s));
   if (st.ext()) {
-    CHK(launch_rel_attention_fwd(ext_attn(h, st, p, a, B, nq > 0 ? std::min(nq, st.n) : st.n), st.attn_ws, s));
+    const FactAttention f = ext_attn(h, st, p, a, B, nq > 0 ? std::min(nq, st.n) : st.n);
+    if (rel_attention_ws(f, false) > st.attn_bytes) return fail(-4, "attention workspace of the handle is too small");
+    CHK(launch_rel_attention_fwd(f, st.attn_ws, s));
     return 0;
   }
   AttnParams ap = attn_params(st, a, B);
@@ -1087,6 +1098,7 @@ int attn_backward(FactHandle* h, Stack& st, const LayerP& p, const LayerA& a, in
     for (int i = 0; i < 3; ++i) f.dout_stride[i] = f.q_stride[i];
     f.dq = dqkv; f.dk = dqkv + st.d; f.dv = dqkv + 2 * st.d;
     for (int64_t* t : {f.dq_stride, f.dk_stride, f.dv_stride}) { t[0] = bs; t[1] = st.qp; t[2] = st.dh; }
+    if (rel_attention_ws(f, true) > sc.attn_bytes) return fail(-4, "attention workspace of the handle is too small");
     CHK(launch_rel_attention_bwd(f, sc.attn_ws, s));
     if (rows < st.n) CHK(launch_zero_rows(dqkv, B, st.n, rows, st.qp, st.d, s));
   } else {

@@ -2,9 +2,12 @@
 position bias) against the float64 oracle with the same options: forward, every gradient, the sampler, optimizer steps,
 checkpoints.  Tolerances are those of the model tests without options (bf16 operands): forward 2e-2, loss 1e-2, per-tensor
 gradient cosine 0.99 and relative error 8e-2."""
+import ctypes
+
 import pytest
 import torch
 
+from mint_amd import _lib as L
 from mint_amd import checkpoint, model_builder
 from mint_amd.trainer import Adam, SingleTaskTrainer
 from oracle import fact_oracle as O
@@ -137,6 +140,39 @@ def test_two_streams_of_encoders_and_repeat():
         seen.append({n: g.clone() for n, g in zip(model.variable_names, model.gradients)})
     for n in seen[0]:  # (bias and split-K sums of the engine use fp32 atomics: equal up to their order)
         assert rel(seen[1][n], seen[0][n]) < 1e-3 and rel(seen[2][n], seen[0][n]) < 1e-3, n
+
+
+@pytest.mark.parametrize("name", ["all", "window", "bias"])
+def test_batches_smaller_than_the_handle(name):
+    """Fewer sequences are cut into more pieces: a handle for 24 has the workspace of every smaller batch, too."""
+    cfg, opts = {k: (dict(v, layers=1) if isinstance(v, dict) else v) for k, v in O.TINY_CFG.items()}, SETS[name]
+    cfg["motion"]["seq_len"], cfg["audio"]["seq_len"] = 256, 512
+    ask = L.FactAttention(H=4, Hkv=4, nq=768, nk=768, dh=32, window_left=-1, window_right=-1, scale=1.0)
+    for i, t in enumerate(("q", "k", "v", "out", "lse", "dout", "dq", "dk", "dv")):
+        setattr(ask, t, 4096 * (i + 1))
+        if t != "lse":
+            getattr(ask, t + "_stride")[:] = (1 << 20, 128, 32)
+    need, bytes_ = {}, ctypes.c_size_t(0)
+    for ask.B in (1, 24):
+        L.check(L.lib().fact_attention_workspace(ctypes.byref(ask), 1, ctypes.byref(bytes_)))
+        need[ask.B] = bytes_.value
+    assert need[1] > need[24]  # (what makes this more than a repetition)
+    big = _model(cfg, opts, 24)
+    for B in (1, 2, 5, 11, 24):
+        one = _model(cfg, opts, B)
+        gb = gpu_batch(O.synthetic_batch(cfg, B, 8, seed=B))
+        inputs = {k: gb[k] for k in ("motion_input", "audio_input")}
+        seen = []
+        for model in (big, one):
+            model.grad_arena.zero_()
+            loss = float(model.forward_backward(inputs, gb["target"]))
+            seen.append((loss, {n: g.clone() for n, g in zip(model.variable_names, model.gradients)}, model(inputs).clone()))
+        assert seen[0][0] == pytest.approx(seen[1][0], rel=1e-5) and rel(seen[0][2], seen[1][2]) < 1e-5
+        # The engine's fp32 atomics (bias and split-K sums) add in any order, also between two runs of one handle; a sum that lies
+        # at a border of bf16 rounds to either neighbour, one step of 2^-7 apart, so no value downstream is off by more than that
+        # share of what it sums.  Pieces written over each other would be off by whole terms.
+        for n in seen[0][1]:
+            assert rel(seen[0][1][n], seen[1][1][n]) < 2.0 ** -7, (B, n)
 
 
 def test_checkpoint_round_trip_with_options(tmp_path):
