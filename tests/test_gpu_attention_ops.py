@@ -269,6 +269,11 @@ def test_bias_edges_distances_and_a_hidden_key():
         m = torch.randint(-3, buckets + 3, (2 * dist + 1,), generator=gen, dtype=torch.int32).to(DEV)  # any map, clamped
         t = _rand(gen, buckets, 2, std=2.0, dtype=torch.float32)
         _check(q, k, v, 32 ** -0.5, rel_table=t, rel_map=m)
+    # the widest map beside the widest head: more than 64 KB of LDS
+    q, k, v = (_rand(gen, 1, 1100, 2, 128) for _ in range(3))
+    _check(q, k, v, 128 ** -0.5, rel_table=_rand(gen, 256, 2, dtype=torch.float32),
+           rel_map=torch.randint(0, 256, (2 * 1024 + 1,), generator=gen, dtype=torch.int32).to(DEV))
+    q, k, v = (_rand(gen, 1, n, 2, 32) for _ in range(3))
     t, m = _table(gen, 2)
     t[int(m[24 + 3])] = -math.inf  # hides every key whose distance lies in that bucket
     ref = _reference(q, k, v, 0.2, rel_table=t, rel_map=m)
