@@ -30,18 +30,26 @@ EXACT_KEYS = 512
 DTYPES = {torch.bfloat16: 0, torch.float32: 1}
 
 
+def _need(cond, msg, *args):
+    if not cond:
+        raise ValueError(msg % args)
+
+
+def _int32(x, name):
+    """ctypes would drop the upper bits."""
+    x = int(x)
+    _need(-1 << 31 <= x < 1 << 31, "%s must fit 32 bits, not %d", name, x)
+    return x
+
+
 def relative_buckets(num_buckets, max_distance, bidirectional=True, device=None):
     """int32 [2 * max_distance + 1]: bucket of each distance key - query clipped to +-max_distance.  Half of a side's buckets
     hold one distance each, the rest grow by equal ratios up to max_distance; with `bidirectional` keys after the query have the
     upper half of the buckets, without it they share bucket 0."""
-    got = (C.c_int32 * (2 * max(0, int(max_distance)) + 1))()
-    L.check(L.lib().fact_relative_buckets(int(num_buckets), int(max_distance), 1 if bidirectional else 0, got))
+    num_buckets, max_distance = _int32(num_buckets, "num_buckets"), _int32(max_distance, "max_distance")
+    got = (C.c_int32 * (2 * min(max(0, max_distance), 1024) + 1))()  # (a wider map is refused)
+    L.check(L.lib().fact_relative_buckets(num_buckets, max_distance, 1 if bidirectional else 0, got))
     return torch.tensor(list(got), dtype=torch.int32, device=device)
-
-
-def _need(cond, msg, *args):
-    if not cond:
-        raise ValueError(msg % args)
 
 
 def _heads(t, name, dtype, device=None):
@@ -145,8 +153,9 @@ def _attention_args(q, k, v, scale, window, sinks, rel_table, rel_map, kv_len, q
     nk, Hkv = k.shape[1], k.shape[2]
     _need(Hkv > 0 and H % Hkv == 0, "the %d query heads must be a multiple of the %d key heads", H, Hkv)
     _need(len(window) == 2, "window must be (left, right)")
-    a = L.FactAttention(B=B, H=H, Hkv=Hkv, nq=nq, nk=nk, dh=dh, window_left=int(window[0]), window_right=int(window[1]),
-                        sinks=int(sinks), scale=float(dh ** -0.5 if scale is None else scale))
+    a = L.FactAttention(B=B, H=H, Hkv=Hkv, nq=nq, nk=nk, dh=dh, window_left=_int32(window[0], "window"),
+                        window_right=_int32(window[1], "window"), sinks=_int32(sinks, "sinks"),
+                        scale=float(dh ** -0.5 if scale is None else scale))
     _need((rel_table is None) == (rel_map is None), "rel_table and rel_map belong together")
     if rel_table is not None:
         _need(torch.is_tensor(rel_table) and rel_table.dim() == 2 and rel_table.shape[1] == H,
@@ -183,7 +192,7 @@ def _inputs(a, held):
 
 
 def _options(scale, window, sinks):
-    return (None if scale is None else float(scale), (-1, -1) if window is None else tuple(window), int(sinks))
+    return (None if scale is None else float(scale), (-1, -1) if window is None else tuple([int(w) for w in window]), int(sinks))
 
 
 def attention(q, k, v, scale=None, window=None, sinks=0, rel_table=None, rel_map=None, kv_len=None, q_start=None,
@@ -311,8 +320,9 @@ def _norm_args(q, k, q_gamma, k_gamma, positions, eps, rotary_dim, base, interle
           tuple(k.shape))
     q_gamma = _vector(q_gamma, "q_gamma", (dh,), torch.float32, dev)
     k_gamma = _vector(k_gamma, "k_gamma", (dh,), torch.float32, dev)
-    a = L.FactQkNorm(B=B, n=n, H=H, Hkv=k.shape[2], dh=dh, rotary_dim=dh if rotary_dim is None else rotary_dim,
-                     interleaved=1 if interleaved else 0, dtype=DTYPES[q.dtype], position0=position0, eps=eps, base=base)
+    a = L.FactQkNorm(B=B, n=n, H=H, Hkv=k.shape[2], dh=dh,
+                     rotary_dim=dh if rotary_dim is None else _int32(rotary_dim, "rotary_dim"), interleaved=1 if interleaved else 0, dtype=DTYPES[q.dtype], position0=_int32(position0, "position0"),
+                     eps=eps, base=base)
     if positions is not None:
         _need(torch.is_tensor(positions) and positions.dtype == torch.int32 and positions.device == dev
               and tuple(positions.shape) in ((B, n), (n,)), "positions must be an int32 tensor of shape %s or %s on %s",

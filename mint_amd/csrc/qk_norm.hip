@@ -355,6 +355,7 @@ int qk_norm_check(const FactQkNorm& a, bool backward, const char** why) {
   if (a.dh < 8 || a.dh > 128 || a.dh % 8) return bad(-3, "unsupported head dim (a multiple of 8 up to 128)");
   if (a.rotary_dim < 0 || a.rotary_dim > a.dh || a.rotary_dim % 8) return bad(-1, "rotary_dim must be a multiple of 8 up to dh");
   if (a.dtype != 0 && a.dtype != 1) return bad(-1, "dtype must be 0 (bf16) or 1 (fp32)");
+  if (!a.positions && (long long)a.position0 + a.n - 1 > INT_MAX) return bad(-1, "the last token's position must fit 32 bits");
   if (!(a.eps >= 0.f) || !(a.eps < 3.0e38f)) return bad(-1, "eps must be finite and not negative");
   if (a.rotary_dim && !(a.base > 0.0 && a.base < 1e300)) return bad(-1, "base must be positive and finite");
   struct T { const void* p; const int64_t* st; int heads; bool out; };

@@ -130,7 +130,7 @@ def _norm(**kw):
     (dict(dh=132), -3, "head dim"), (dict(dh=20), -3, "head dim"), (dict(rotary_dim=72), -1, "rotary_dim"),
     (dict(rotary_dim=-8), -1, "rotary_dim"), (dict(rotary_dim=12), -1, "rotary_dim"), (dict(dtype=2), -1, "dtype"),
     (dict(eps=-1.0), -1, "eps"), (dict(eps=math.nan), -1, "eps"), (dict(base=0.0), -1, "base"), (dict(base=math.nan), -1, "base"),
-    (dict(k=None), -1, "null"), (dict(dq=4096 + 4), -1, "aligned"), (dict(q_gamma=4096 + 4), -1, "aligned"),
+    (dict(position0=(1 << 31) - 5), -1, "position"), (dict(k=None), -1, "null"), (dict(dq=4096 + 4), -1, "aligned"), (dict(q_gamma=4096 + 4), -1, "aligned"),
     (dict(q_stride=(8 * 256, 252, 64)), -1, "multiples of 8"), (dict(dk_stride=(8 * 256, 0, 64)), -1, "broadcast")])
 def test_norm_refuses(lib, kw, rc, word):
     n = C.c_size_t(0)
@@ -170,6 +170,12 @@ def test_bucket_map_against_exact_powers(lib, buckets, dist, both):
                                   (2, 1, False)])
 def test_bucket_map_refuses(lib, args):
     with pytest.raises(L.FactError):
+        A.relative_buckets(*args)
+
+
+@pytest.mark.parametrize("args", [(32, 1 << 33, True), ((1 << 32) + 32, 128, True), (32, (1 << 32) + 128, False)])
+def test_bucket_map_refuses_what_ctypes_would_cut(lib, args):
+    with pytest.raises(ValueError, match="32 bits"):
         A.relative_buckets(*args)
 
 

@@ -455,7 +455,10 @@ def test_refusals():
                  lambda: A.qk_norm_rope(q.half(), q.half()), lambda: A.qk_norm_rope(q, q.float()),
                  lambda: A.qk_norm_rope(q, q, q_gamma=torch.ones(63, device=DEV)),
                  lambda: A.qk_norm_rope(q, q, positions=torch.zeros(2, 20, device=DEV)),
-                 lambda: A.qk_norm_rope(q, q[:, :5])):
+                 lambda: A.qk_norm_rope(q, q[:, :5]), lambda: A.attention(q, q, q, window=(1 << 32, 0)),
+                 lambda: A.attention(q, q, q, window=(5, -(1 << 33))), lambda: A.attention(q, q, q, window=(5, 0, 0)),
+                 lambda: A.attention(q, q, q, window=(5, 0), sinks=(1 << 32) + 1), lambda: A.qk_norm_rope(q, q, position0=1 << 32),
+                 lambda: A.qk_norm_rope(q, q, rotary_dim=(1 << 32) + 64)):
         with pytest.raises(ValueError):
             call()
     from mint_amd._lib import FactError
@@ -463,7 +466,9 @@ def test_refusals():
     for call in (lambda: A.attention(odd, odd, odd), lambda: A.attention(q, q, q, scale=0.0), lambda: A.attention(q, q, q, sinks=-1),
                  lambda: A.attention(q, q, q, scale=float("nan")), lambda: A.qk_norm_rope(q, q, rotary_dim=65),
                  lambda: A.qk_norm_rope(q, q, rotary_dim=12), lambda: A.qk_norm_rope(q, q, eps=-1.0),
-                 lambda: A.qk_norm_rope(q, q, base=0.0)):
+                 lambda: A.qk_norm_rope(q, q, base=0.0), lambda: A.qk_norm_rope(q, q, position0=(1 << 31) - 10),
+                 lambda: A.attention(q, q.clone(), q.clone(), out=q, window=(1, 1), sinks=-2),
+                 lambda: (lambda k: A.attention(q, k, q.clone(), out=k))(q.clone())):
         with pytest.raises(FactError):
             call()
 
