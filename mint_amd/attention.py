@@ -320,9 +320,9 @@ def _norm_args(q, k, q_gamma, k_gamma, positions, eps, rotary_dim, base, interle
           tuple(k.shape))
     q_gamma = _vector(q_gamma, "q_gamma", (dh,), torch.float32, dev)
     k_gamma = _vector(k_gamma, "k_gamma", (dh,), torch.float32, dev)
-    a = L.FactQkNorm(B=B, n=n, H=H, Hkv=k.shape[2], dh=dh,
-                     rotary_dim=dh if rotary_dim is None else _int32(rotary_dim, "rotary_dim"), interleaved=1 if interleaved else 0, dtype=DTYPES[q.dtype], position0=_int32(position0, "position0"),
-                     eps=eps, base=base)
+    a = L.FactQkNorm(B=B, n=n, H=H, Hkv=k.shape[2], dh=dh, interleaved=1 if interleaved else 0, dtype=DTYPES[q.dtype],
+                     rotary_dim=dh if rotary_dim is None else _int32(rotary_dim, "rotary_dim"),
+                     position0=_int32(position0, "position0"), eps=eps, base=base)
     if positions is not None:
         _need(torch.is_tensor(positions) and positions.dtype == torch.int32 and positions.device == dev
               and tuple(positions.shape) in ((B, n), (n,)), "positions must be an int32 tensor of shape %s or %s on %s",
