@@ -121,7 +121,7 @@ def _ws_bytes(name, a, backward):
 
 # Calls of one geometry (shapes, strides, types, devices, options) share their checks: the first one leaves its filled-in argument
 # struct and workspace size, the next ones copy it and set the pointers.  Nothing of the tensors themselves is kept.  (A call
-# costs the host 9 instead of 18 us; one new token of 32 sequences takes the GPU 4.)
+# costs the host 9-11 instead of 18 us; one new token of 32 sequences takes the GPU 4.)
 _PLANS = {}
 _MOST_PLANS = 512
 _Plan = collections.namedtuple("_Plan", ["args", "fn", "ws", "extra"])
