@@ -11,6 +11,7 @@ mkdir -p "$OUT" "$OUT/obj"
 HIPCC=${HIPCC:-/opt/rocm/bin/hipcc}
 # packed fp32 instructions off: some forms that -O3 makes of ordinary float code have given wrong results on this hardware
 # now and then (the host pass warns that it does not know the feature)
+UNITS="gemm gemm_big rowops attention rel_attention qk_norm"  # and engine, probe (tools/build_variant.sh takes UNITS and FLAGS from here)
 FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -fvisibility=hidden -fvisibility-inlines-hidden -Wno-unused-result -Xclang -target-feature -Xclang -packed-fp32-ops $FACT_EXTRA_FLAGS"
 # the flag set is part of the object cache key: a default build after a variant build (FACT_EXTRA_FLAGS=-D...) must not
 # link the variant's objects into the shipped library, nor the other way round
@@ -22,7 +23,7 @@ pids=()
 stale() {  # $1 = object, $2 = source
   [ ! -f "$1" ] || [ "$2" -nt "$1" ] || [ -n "$(find . ../../include -name '*.h' -newer "$1" 2>/dev/null)" ]
 }
-for f in gemm gemm_big rowops attention rel_attention qk_norm engine probe; do
+for f in $UNITS engine probe; do
   if stale "$OUT/obj/$f.o" "$f.hip"; then
     $HIPCC $FLAGS -c "$f.hip" -o "$OUT/obj/$f.o" &
     pids+=($!)
@@ -35,7 +36,10 @@ for f in engine probe; do
   fi
 done
 for p in "${pids[@]}"; do wait "$p"; done
-COMMON="$OUT/obj/gemm.o $OUT/obj/gemm_big.o $OUT/obj/rowops.o $OUT/obj/attention.o $OUT/obj/rel_attention.o $OUT/obj/qk_norm.o"
-$HIPCC --offload-arch=gfx950 -shared -fPIC -Wl,--version-script=exports.map -o "$OUT/libfact_hip.so" $COMMON "$OUT/obj/engine.o" "$OUT/obj/probe.o"
-$HIPCC --offload-arch=gfx950 -shared -fPIC -Wl,--version-script=exports.map -o "$OUT/libfact_hip_dbg.so" $COMMON "$OUT/obj/engine_dbg.o" "$OUT/obj/probe_dbg.o"
+COMMON=""
+for f in $UNITS; do COMMON="$COMMON $OUT/obj/$f.o"; done
+# (-z defs: a unit that is missing here is an error of the link, not of whoever loads the library)
+LINK="--offload-arch=gfx950 -shared -fPIC -Wl,-z,defs -Wl,--version-script=exports.map"
+$HIPCC $LINK -o "$OUT/libfact_hip.so" $COMMON "$OUT/obj/engine.o" "$OUT/obj/probe.o"
+$HIPCC $LINK -o "$OUT/libfact_hip_dbg.so" $COMMON "$OUT/obj/engine_dbg.o" "$OUT/obj/probe_dbg.o"
 echo "built $OUT/libfact_hip.so $OUT/libfact_hip_dbg.so"
