@@ -282,7 +282,8 @@ int fact_relative_buckets(int num_buckets, int max_distance, int bidirectional, 
  *   y = x * rsqrt(mean(x^2) + eps) * gamma;  pairs of the first rotary_dim values turned by pos * base^(-2 i / rotary_dim)
  * Pair i is (i, i + rotary_dim / 2), or (2 i, 2 i + 1) with interleaved.  dtype 0 = bf16, 1 = fp32 (all tensors but the
  * fp32 gains and the int32 positions).  dh a multiple of 8 up to 128, rotary_dim a multiple of 8 up to dh (0: no rotation).
- * Outputs may be the inputs themselves (same pointer and strides). */
+ * q_out may be q and k_out k, dq may be dq_out or q and dk dk_out or k (same pointer and strides); no output may be another
+ * tensor of the call. */
 typedef struct FactQkNorm {
   const void *q, *k;            /* [B][n][H][dh], [B][n][Hkv][dh]: the projections (both directions) */
   void *q_out, *k_out;          /* forward */

@@ -374,6 +374,26 @@ int qk_norm_check(const FactQkNorm& a, bool backward, const char** why) {
     }
   }
   if (((uintptr_t)a.q_gamma | (uintptr_t)a.k_gamma) & 15) return bad(-1, "tensors must be 16-byte aligned");
+  // Queries and keys are different workgroups of one launch, and a workgroup reads a value right before it writes the result in
+  // its place: an output may stand where its own side's input does, value by value, and nowhere else.
+  for (int i = 0; i < (backward ? 6 : 4); ++i)
+    for (int k = 0; k < i; ++k) {
+      if (t[i].p != t[k].p || !(t[i].out || t[k].out)) continue;
+      const int n[3] = {a.B, a.n, t[i].heads};
+      bool place = (i & 1) == (k & 1);  // (both lists alternate queries and keys)
+      for (int j = 0; j < 3; ++j) place = place && (n[j] == 1 || t[i].st[j] == t[k].st[j]);
+      if (!place) return bad(-1, "an output must not be another tensor (but its own input, with the same strides)");
+    }
+  if (backward) {
+    const void* gains[] = {a.dq_gamma, a.dk_gamma};
+    for (int i = 0; i < 2; ++i) {
+      if (!gains[i]) continue;
+      for (const void* x : {(const void*)a.q_gamma, (const void*)a.k_gamma, (const void*)a.positions, gains[1 - i]})
+        if (gains[i] == x) return bad(-1, "an output must not be another tensor");
+      for (const T& x : bwd)
+        if (gains[i] == x.p) return bad(-1, "an output must not be another tensor");
+    }
+  }
   return 0;
 }
 
