@@ -240,7 +240,8 @@ int fact_create_ex(const FactConfig* cfg, const FactAttnCfg* attn, int max_batch
  *   out_i = softmax over the visible keys of s_i, times v; a row that sees no key (or only keys whose bias is -inf) gives 0
  * H query heads, head h reads key / value head h / (H / Hkv).  dh 32, 64, 80, 96 or 128.  What stands at keys and values that
  * no query row of the sequence sees (at j >= len_b, behind a window, in a cache's free places) reaches no result, be it NaN.
- * `out` may be q itself (same strides); other outputs may be no input.  Scores, softmax statistics and all sums are fp32; the probabilities enter the second product as bf16.
+ * `out` may be q itself (same pointer and strides); other outputs may be no input.  Scores, softmax statistics and all sums are
+ * fp32; the probabilities enter the second product as bf16.
  * Every sum (over heads that share keys, over the splits of a long key range, over the positions behind a bucket) has a fixed
  * order: results do not change from run to run. */
 typedef struct FactAttention {

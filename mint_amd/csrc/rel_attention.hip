@@ -1412,9 +1412,15 @@ int rel_attention_check(const FactAttention& a, bool backward, const char** why)
       if (t[i].out && t[i].st[k] == 0 && n[k] > 1) return bad(-1, "an output must not be broadcast");
     }
   }
+  // (`out` may be q: a workgroup reads its own rows before it writes them, if they are the same)
   for (int i = 0; i < (backward ? 8 : 4); ++i)
-    for (int k = 0; k < i; ++k)
-      if (t[i].p == t[k].p && (t[i].out || t[k].out) && !(i == 3 && k == 0)) return bad(-1, "an output must not be another tensor");
+    for (int k = 0; k < i; ++k) {
+      if (t[i].p != t[k].p || !(t[i].out || t[k].out)) continue;
+      const int n[3] = {a.B, a.nq, a.H};
+      bool place = i == 3 && k == 0;
+      for (int j = 0; j < 3; ++j) place = place && (n[j] == 1 || t[i].st[j] == t[k].st[j]);
+      if (!place) return bad(-1, "an output must not be another tensor (but `out` may be q, with the same strides)");
+    }
   if ((uintptr_t)a.out_lo & 15) return bad(-1, "tensors must be 16-byte aligned");
   if (backward && !a.lse) return bad(-1, "the backward needs the forward's lse");
   if (backward && a.rel_table && !a.drel) return bad(-1, "the backward with rel_table needs drel");

@@ -5,7 +5,7 @@ import ctypes as C
 import pytest
 
 from mint_amd import _lib as L
-from tests.test_attention_args import _norm, lib  # noqa: F401
+from tests.test_attention_args import _attention, _norm, lib  # noqa: F401
 
 NORM_TENSORS = ("q", "k", "q_out", "k_out", "dq_out", "dk_out", "dq", "dk")
 NORM_FORWARD = {("q_out", "q"), ("k_out", "k")}
@@ -59,3 +59,20 @@ def test_norm_calls_refuse_too(lib):  # noqa: F811
     assert lib.fact_qk_norm(C.byref(a), None, 0, None) == -1
     a = _norm(dk=7 * 4096)
     assert lib.fact_qk_norm_backward(C.byref(a), 1 << 26, 1 << 20, None) == -1
+
+
+def _attention_says(lib, backward, **kw):
+    n = C.c_size_t(0)
+    rc = lib.fact_attention_workspace(C.byref(_attention(**kw)), backward, C.byref(n))
+    return rc, lib.fact_last_error().decode() if rc else ""
+
+
+def test_attention_in_place_of_the_queries_needs_their_strides(lib):  # noqa: F811
+    assert _attention_says(lib, 0, out=4096)[0] == 0
+    for strides in ((64, 256, 2048), (8 * 256, 64, 512), (8 * 512, 512, 64)):
+        rc, why = _attention_says(lib, 0, out=4096, out_stride=strides)
+        assert rc == -1 and "another tensor" in why, strides
+    assert _attention_says(lib, 0, out=4096, out_stride=(8, 256, 64), B=1)[0] == 0  # one sequence: its stride is never used
+    assert _attention_says(lib, 0, out=4096, nq=1, out_stride=(8 * 256, 8, 64))[0] == 0
+    a = _attention(out=4096, out_stride=(64, 256, 2048))
+    assert lib.fact_attention(C.byref(a), None, 0, None) == -1
