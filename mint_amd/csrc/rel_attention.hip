@@ -1421,6 +1421,15 @@ int rel_attention_check(const FactAttention& a, bool backward, const char** why)
       for (int j = 0; j < 3; ++j) place = place && (n[j] == 1 || t[i].st[j] == t[k].st[j]);
       if (!place) return bad(-1, "an output must not be another tensor (but `out` may be q, with the same strides)");
     }
+  const void* more[] = {a.out_lo, a.lse, a.drel, a.rel_table, a.rel_map, a.kv_len, a.q_start};
+  for (int i = 0; i < 7; ++i) {
+    if (!more[i]) continue;
+    const bool out = backward ? i == 2 : i < 2;
+    for (int k = 0; k < (backward ? 8 : 4); ++k)
+      if (more[i] == t[k].p && (out || t[k].out)) return bad(-1, "an output must not be another tensor");
+    for (int k = 0; k < 7; ++k)
+      if (out && k != i && more[i] == more[k]) return bad(-1, "an output must not be another tensor");
+  }
   if ((uintptr_t)a.out_lo & 15) return bad(-1, "tensors must be 16-byte aligned");
   if (backward && !a.lse) return bad(-1, "the backward needs the forward's lse");
   if (backward && a.rel_table && !a.drel) return bad(-1, "the backward with rel_table needs drel");

@@ -5,7 +5,7 @@ import ctypes as C
 import pytest
 
 from mint_amd import _lib as L
-from tests.test_attention_args import _attention, _norm, lib  # noqa: F401
+from tests.test_attention_args import BIAS, _attention, _norm, lib  # noqa: F401
 
 NORM_TENSORS = ("q", "k", "q_out", "k_out", "dq_out", "dk_out", "dq", "dk")
 NORM_FORWARD = {("q_out", "q"), ("k_out", "k")}
@@ -76,3 +76,23 @@ def test_attention_in_place_of_the_queries_needs_their_strides(lib):  # noqa: F8
     assert _attention_says(lib, 0, out=4096, nq=1, out_stride=(8 * 256, 8, 64))[0] == 0
     a = _attention(out=4096, out_stride=(64, 256, 2048))
     assert lib.fact_attention(C.byref(a), None, 0, None) == -1
+
+
+@pytest.mark.parametrize("backward", [0, 1])
+def test_attention_outputs_beside_the_heads(lib, backward):  # noqa: F811
+    """The fp32 outputs and the tables: drel over rel_table would be read as the bias by the kernel that follows."""
+    kw = dict(BIAS, kv_len=1 << 23, q_start=1 << 24, out_lo=1 << 25, lse=1 << 26)
+    assert _attention_says(lib, backward, **kw)[0] == 0
+    small = ["drel"] if backward else ["out_lo", "lse"]
+    others = ["q", "k", "v", "out", "rel_table", "rel_map", "kv_len", "q_start", "out_lo", "lse"]
+    others += ["dout", "dq", "dk", "dv"] if backward else []
+    place = _attention(**kw)
+    for out in small:
+        for other in others:
+            if other != out:
+                rc, why = _attention_says(lib, backward, **dict(kw, **{out: getattr(place, other)}))
+                assert rc == -1 and "another tensor" in why, (out, other)
+    for out in ("dq", "dk", "dv") if backward else ("out",):
+        for other in ("rel_table", "rel_map", "kv_len", "q_start"):
+            rc, why = _attention_says(lib, backward, **dict(kw, **{out: getattr(place, other)}))
+            assert rc == -1 and "another tensor" in why, (out, other)
