@@ -7,7 +7,9 @@
 Tensors are [batch, token, head, dh] CUDA tensors of any strides whose last dimension is contiguous (views of one packed
 projection are read in place; what the kernels cannot address is copied first).  Calls run on the current stream of the
 tensors' device, never synchronise, and take their scratch memory from torch's allocator per call, so they can be captured into
-graphs and run on several streams at once.  There is no autograd: as in the engine, the backward is a call of its own.
+graphs and run on several streams at once.  There is no autograd: as in the engine, the backward is a call of its own, and a
+tensor that requires grad is refused while grad mode is on (its gradient would be lost without a word): detach it, or call under
+torch.no_grad().
 Models use the same kernels through the transformer options of their config (mint_amd/protos.py).
 """
 import collections
@@ -42,6 +44,12 @@ def _int32(x, name):
     return x
 
 
+def _detached(t, name):
+    _need(not (t.requires_grad and torch.is_grad_enabled()),
+          "%s requires grad, and these calls record no graph: detach it or call under torch.no_grad(), and take the gradients from "
+          "the backward call", name)
+
+
 def relative_buckets(num_buckets, max_distance, bidirectional=True, device=None):
     """int32 [2 * max_distance + 1]: bucket of each distance key - query clipped to +-max_distance.  Half of a side's buckets
     hold one distance each, the rest grow by equal ratios up to max_distance; with `bidirectional` keys after the query have the
@@ -55,6 +63,7 @@ def relative_buckets(num_buckets, max_distance, bidirectional=True, device=None)
 def _heads(t, name, dtype, device=None):
     """A [batch, token, head, dh] tensor that the kernels can read in place, or a contiguous copy of it."""
     _need(torch.is_tensor(t) and t.dim() == 4, "%s must be a [batch, token, head, dh] tensor", name)
+    _detached(t, name)
     _need(t.is_cuda, "%s must be a CUDA tensor: there is no CPU path", name)
     _need(device is None or t.device == device, "%s is on %s, expected %s", name, t.device, device)
     if dtype is not None:
@@ -73,6 +82,7 @@ def _dest(t, name, shape, dtype, device):
         return torch.empty(shape, dtype=dtype, device=device)
     _need(torch.is_tensor(t) and t.shape == torch.Size(shape) and t.dtype == dtype and t.device == device,
           "%s must be a %s tensor of shape %s on %s", name, dtype, tuple(shape), device)
+    _detached(t, name)
     _need(_addressable(t), "%s must have a contiguous last dimension, 16-byte alignment and strides that are multiples of 8", name)
     _need(all(t.stride(i) for i in range(3) if t.shape[i] > 1), "%s must not be a broadcast tensor", name)
     return t
@@ -83,6 +93,7 @@ def _vector(t, name, shape, dtype, device):
         return None
     _need(torch.is_tensor(t) and t.dtype == dtype and t.device == device and t.shape == torch.Size(shape),
           "%s must be a %s tensor of shape %s on %s", name, dtype, tuple(shape), device)
+    _detached(t, name)
     return t if t.is_contiguous() and not t.data_ptr() & 15 else t.clone(memory_format=torch.contiguous_format)
 
 
@@ -135,8 +146,12 @@ def _keep(key, args, fn, ws, extra=None):
 
 
 def _key(op, tensors, options):
-    """None where an argument is no tensor: the checks say so."""
+    """None where an argument is no tensor or has to be refused: the checks say so."""
     try:
+        if torch.is_grad_enabled():
+            for t in tensors:
+                if t is not None and t.requires_grad:
+                    return None
         return (op,) + tuple([None if t is None else (t.shape, t.stride(), t.dtype, t.device) for t in tensors]) + options
     except AttributeError:
         return None
