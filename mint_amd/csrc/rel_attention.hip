@@ -380,24 +380,29 @@ __global__ __launch_bounds__(256, 2) void rel_fwd_kernel(const RelP p) {
     // The reference point m of a row's exponents is raised only when a score passes it by THR powers of two: any m that keeps
     // exp2 in range gives the same softmax, and the common path needs no lane but its own.
     const float mu = m == -INFINITY ? 0.f : m;  // -inf: the row has seen no key yet
+    f32x4 x[2];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      s[0][r] = fmaf(s[0][r], p.sc, -mu);
-      s[1][r] = fmaf(s[1][r], p.sc, -mu);
+      x[0][r] = fmaf(s[0][r], p.sc, -mu);
+      x[1][r] = fmaf(s[1][r], p.sc, -mu);
     }
-    const float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
-                           fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+    const float mx = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])),
+                           fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
     if (__any((mx > THR) | ((m == -INFINITY) & (mx > -INFINITY)))) {
       const bool first = m == -INFINITY;
       const float top = allmax4(mx);                   // relative to m, or to 0
       const float d = first ? (top == -INFINITY ? 0.f : top) : fmaxf(top, 0.f);
-      const float alpha = __builtin_amdgcn_exp2f(-d);  // (first: nothing has been summed)
-      m = first ? top : m + d;
-      l = first ? 0.f : l * alpha;
+      const float mn = first ? top : m + d;
+      const float alpha = __builtin_amdgcn_exp2f(m - mn);
+      m = mn;
+      l = first ? 0.f : l * alpha;  // (first: nothing has been summed)
+      // exponents from the scores again: a reference point far below them, such as that of keys with a bias of -1e9, has left
+      // them none of their last bits
+      const float mv = mn == -INFINITY ? 0.f : mn;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        s[0][r] -= d;
-        s[1][r] -= d;
+        x[0][r] = fmaf(s[0][r], p.sc, -mv);
+        x[1][r] = fmaf(s[1][r], p.sc, -mv);
       }
 #pragma unroll
       for (int dt = 0; dt < ND; ++dt)
@@ -408,8 +413,8 @@ __global__ __launch_bounds__(256, 2) void rel_fwd_kernel(const RelP p) {
     float ls = 0.f;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      e0[r] = __builtin_amdgcn_exp2f(s[0][r]);
-      e1[r] = __builtin_amdgcn_exp2f(s[1][r]);
+      e0[r] = __builtin_amdgcn_exp2f(x[0][r]);
+      e1[r] = __builtin_amdgcn_exp2f(x[1][r]);
       ls += e0[r] + e1[r];
     }
     l += ls;
