@@ -238,6 +238,8 @@ int fact_create_ex(const FactConfig* cfg, const FactAttnCfg* attn, int max_batch
  *                                           window_left  < 0 or j >= p - window_left or j < sinks
  *   s_ij = scale * q_i . k_j + (rel_table ? rel_table[m(j - p)][h] : 0),  m(d) = rel_map[clamp(d, -D, D) + D]
  *   out_i = softmax over the visible keys of s_i, times v; a row that sees no key (or only keys whose bias is -inf) gives 0
+ * Finite values of rel_table count up to +-2^14, so 1e9 or the type's largest and lowest value force and hide keys as well; a row
+ * that sees hidden keys only has the softmax of its scores over them, as if there were no bias, but for -inf.
  * H query heads, head h reads key / value head h / (H / Hkv).  dh 32, 64, 80, 96 or 128.  What stands at keys and values that
  * no query row of the sequence sees (at j >= len_b, behind a window, in a cache's free places) reaches no result, be it NaN.
  * `out` may be q itself (same pointer and strides); other outputs may be no input.  Scores, softmax statistics and all sums are

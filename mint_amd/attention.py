@@ -216,7 +216,8 @@ def attention(q, k, v, scale=None, window=None, sinks=0, rel_table=None, rel_map
 
     Query row i of sequence b stands at position q_start[b] + i (0 + i without q_start) and sees the keys j with j < kv_len[b],
     j <= position + window[1] and (j >= position - window[0] or j < sinks); a negative window side is open.  rel_table
-    [buckets, H] fp32 adds rel_table[rel_map[clip(j - position)]][h] to scale * q . k.  A row that sees no key gives zeros.
+    [buckets, H] fp32 adds rel_table[rel_map[clip(j - position)]][h] to scale * q . k; -inf hides a key, finite values count up to
+    +-2^14.  A row that sees no key gives zeros.
     What stands at keys and values that no row of their sequence sees (from kv_len on, behind the window, in a cache's free places)
     reaches no result.  `out` may be q, and must not overlap k or v.  Returns out [B, nq, H, dh], with `training`
     (out, AttentionSaved)."""

@@ -287,13 +287,22 @@ DEVINL void staged() {
   __syncthreads();
 }
 
+// Finite values of the table count up to +-2^14: exp(-2^14) is 0 beside any key that is not hidden as well, and where a row sees
+// nothing but such keys its scores keep 2^-10 and less than a step of bf16 of their probabilities.  Further out (1e9 and the type's
+// lowest value are what programs hide keys with) value / scale overflows, the rounding of a score is larger than the score, and of
+// log-sum-exp = reference point + log2(sum) the second part is lost.  -inf hides a key, NaN stays one.
+constexpr float MOST_BIAS = 16384.f;
+DEVINL float bias_of(const RelP& p, int i, int h) {  // of head h at place i of the map, divided by scale
+  const int bk = min(max(p.a.rel_map[i], 0), p.a.rel_buckets - 1);
+  const float x = p.a.rel_table[(size_t)bk * p.a.H + h], y = fabsf(x);
+  return ((y > MOST_BIAS) & (y < INFINITY) ? copysignf(MOST_BIAS, x) : x) * p.rscale;
+}
 // bias of head h for distances -(D + PAD) .. D + PAD, divided by scale
 DEVINL void load_bias(float* eb, const RelP& p, int h, int tid, int nthr) {
   const int D = p.a.rel_max_distance;
   for (int i = tid; i < 2 * (D + PAD) + 1; i += nthr) {
     const int d = min(max(i - (D + PAD), -D), D);
-    const int bk = min(max(p.a.rel_map[d + D], 0), p.a.rel_buckets - 1);
-    eb[i] = p.a.rel_table[(size_t)bk * p.a.H + h] * p.rscale;
+    eb[i] = bias_of(p, d + D, h);
   }
 }
 
@@ -1037,9 +1046,7 @@ __global__ __launch_bounds__(256, 2) void rel_rows_kernel(const RelP p) {
   Lane<DH> at;
   at.init(lane);
   const int D = a.rel_max_distance, n = 2 * D + 1, hr = row / a.nq;
-  auto bias = [&](int head, int i) {  // distance i - D
-    return a.rel_table[(size_t)min(max(a.rel_map[i], 0), a.rel_buckets - 1) * a.H + head] * p.rscale;
-  };
+  auto bias = [&](int head, int i) { return bias_of(p, i, head); };  // distance i - D
 
   struct Tile {  // one 32-key tile in flight: K as fragments, V as rows
     Frag<DH> K[2];
