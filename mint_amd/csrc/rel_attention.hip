@@ -880,8 +880,6 @@ __global__ __launch_bounds__(256, dkdv_slots(DH)) void rel_dkdv_kernel(const Rel
     const bf16_t* Os = Qs + G::IMG;
     const float* sl = reinterpret_cast<const float*>(Qs + 2 * G::IMG);
     const int q0 = (t0 + qt) * 32, p0 = start + q0;
-    if (DH > 96) asm("" : "+v"(at.tr));  // offsets made from them each tile: kept, they do not fit the registers of 3 waves
-    if (REL && DH > 96) asm("" : "+v"(at.rows));
     const bool skip = !active || v.none<16>(j0, p0);
     if (DH >= 80) asm("" : "+v"(at.tr));  // offsets made from them each tile: kept, they do not fit the registers
     if (DH >= 80 && (REL || DH < 96)) asm("" : "+v"(at.rows));
