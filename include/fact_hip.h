@@ -251,8 +251,8 @@ typedef struct FactAttention {
   void* out;               /* [B][nq][H][dh] */
   float* out_lo;           /* may be NULL: what the rounding of `out` left, fp32 [B][nq][H][dh] without gaps.  A forward that is
                             * given it carries the probabilities to 24 bits through the product with v, and the backward's row
-                            * sums dO . O take out + out_lo: the fp32 gradient of the table needs it, the gradients of short
-                            * sequences (up to some 512 keys) gain from it */
+                            * sums dO . O take out + out_lo: the fp32 gradient of the table needs it, the gradients of rows
+                            * that see some tens of keys gain from it (at 512 nothing is left of the gain) */
   float* lse;              /* [B][H][nq] base-2 log-sum-exp of the scaled scores (+inf: row without keys); forward: may be NULL */
   const void* dout;        /* backward: gradient of out */
   void *dq, *dk, *dv;      /* backward: written */

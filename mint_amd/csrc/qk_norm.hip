@@ -3,9 +3,10 @@
 //
 // Forward   r = rsqrt(mean x^2 + eps), y = x r gamma, z = R(pos) y
 // Backward  dy = R(pos)^T dz, dgamma = sum dy x r, dx = r (gamma dy - x r mean(gamma dy x r))
-// Both read each value once and write each result once, so the rate of the copy they amount to bounds them: fp32, B 8, n 1440,
-// 24 heads of 128 takes 54 us forward (5.2 TB/s) and 91 + 5 backward (4.6 TB/s); bf16, B 16, n 360, 20 heads of 80, which caches
-// hold, 12 and 17.5 + 4; one token of 32 sequences 4.  A head of dh
+// Both read each value once and write each result once.  In fp32 the rate of the copy they amount to bounds them: B 8, n 1440,
+// 24 heads of 128 takes 54 us forward (5.2 TB/s) and 91 + 5 backward (4.6 TB/s).  In bf16, B 16, n 360, 20 heads of 80, which caches
+// hold, 12 and 17 + 4, where the copy would take 7 and 11: 10 of a group's 16 lanes and 10 of a piece's 12 heads are in use, half of
+// the lanes, by 8-byte loads.  One token of 32 sequences takes 4.  (Launches under the profiler.)  A head of dh
 // values is held by dh / 8 lanes of a group of GL = 4, 8 or 16 (its row sums stay inside a 16-lane row); a lane holds 4 pairs
 // of one rotation slot, so the partner of every value is in the same lane.  A wave takes heads of one token, of the queries or
 // of the keys: the angles, reduced in double (a far position times a frequency loses whole turns in 32 bits), are computed once
@@ -103,6 +104,8 @@ DEVINL void angles(const NormP& p, int pos, int s, int lane, f32x4& co, f32x4& s
   for (int k = 0; k < 6; ++k) turn *= (lane >> k) & 1 ? p.ratio[k] : 1.0;
   double x = pos * turn;
   x -= rint(x);
+  // (The rest, at most half a turn, in 32 bits: an angle is off by 2^-24 of up to pi, 2^-22.3.  fp32 results are 6.2e-8 off in
+  // norm with it, and 5.8e-8 with cosines and sines of 64 bits.)
   float u, w;
   sincospif((float)(2.0 * x), &u, &w);
 #pragma unroll

@@ -1,5 +1,6 @@
 // Attention with a sliding window, sinks and a learned relative position bias by buckets, forward and backward
 // (definition: include/fact_hip.h, FactAttention).
+// Times below are of launches under the profiler, each alone between two others; calls one after another take about a tenth less.
 //
 // Fragment conventions (common.h): scores are computed transposed, S^T = K Q^T, on 16x16x32 bf16 MFMAs, so that one query
 // lives in one lane column: lane (g = lane >> 4, c = lane & 15) holds keys 4 g .. 4 g + 3 of query c.  Two stacked 16-key
@@ -234,8 +235,9 @@ DEVINL u32x4 load16(const bf16_t* base, unsigned off) {
 // Loads that write LDS themselves, 16 bytes a lane and 64 consecutive places of a tile an instruction: no registers hold what is
 // in flight.  Each wave waits for its own before the barrier (__syncthreads alone does not).  The two buffers of a kernel are two
 // objects, each named by half of the unrolled loop: of one array with a computed half the compiler would wait for the loads in
-// flight before each read.  At B 8, H 12, n 1440, dh 128 with a bias dK/dV takes 350 us with them and 427 staged through registers;
-// a third buffer, with two tiles in flight, costs the workgroups it leaves no LDS for (354 instead of 263, forward 172 and 162).
+// flight before each read.  At B 8, H 12, n 1440, dh 128 with a bias dK/dV, which took 32 keys a wave then, went from 427 us staged
+// through registers to 350 with them; a third buffer, with two tiles in flight, cost the workgroups it left no LDS for (354 instead
+// of 263, forward 172 instead of 162, without a bias and in that form as well).
 typedef __attribute__((address_space(3))) void lds_void;
 typedef __attribute__((address_space(1))) const void glb_void;
 template <int DH>
@@ -309,7 +311,10 @@ DEVINL void load_bias(float* eb, const RelP& p, int h, int tid, int nthr) {
 // ---------------------------------------------------------------------------------------------------------------------
 // forward: workgroup = 64 queries of one head, 4 waves x 16; 32-key tiles double-buffered in LDS.  One pass over the keys:
 //   m' = max(m, s);  l' = l 2^(m - m') + sum 2^(s - m');  O' = O 2^(m - m') + P V;  out = O / l
-// Bound by vector instructions (60 % of a SIMD's issue with a bias; LDS 20 %, matrix pipe below 30 %).  With 32 queries a wave each
+// In training with a bias vector instructions bound it (60 % of a SIMD's issue, half of them the 24-bit split below; LDS 20 to 27 %,
+// matrix pipe below 30 %): B 8, H 12, n 1440, dh 128, all keys 234 us.  Without one no pipe is full (vector 41 to 50 %, LDS 21 to
+// 28 %): what bounds it is a tile's dependent chain - scores, exponents, packing, product, one after another in a wave - and the
+// barrier every 32 keys: n 8192, H 10, dh 80, window 1023 causal 57 us.  With 32 queries a wave each
 // K and V fragment feeds two products, but half as many waves fit, and a block's edge tiles are twice as many: B 4, H 12, n 1440,
 // dh 128, window 257 takes 40 us instead of 29, B 8, H 12, n 1440, dh 128, all keys 172 instead of 159.
 // ---------------------------------------------------------------------------------------------------------------------
@@ -477,8 +482,9 @@ __global__ __launch_bounds__(256, 2) void rel_fwd_kernel(const RelP p) {
 //   * The four rows of lanes are 4 distances apart: rows 2 and 3 join rows 0 and 1 moved by 8 lanes, row 1 joins row 0 moved by 4;
 //     what leaves on that side belongs to the sub-tile at d + 16.
 // Key tiles are visited in ascending order, so a distance is complete after its two neighbours, and row 0 stores 16 of them at a
-// time, each once per 16 queries.  At B 8, H 12, n 1440, dh 128 dQ takes 735 us with an LDS add per value, 300 with one per
-// folded row (its four rows meet in the same words), 177 without any sums and 214 with this (32 queries a wave).
+// time, each once per 16 queries.  At B 8, H 12, n 1440, dh 128 dQ, which took 32 queries a wave when this was chosen, needed 735 us
+// with an LDS add per value, 300 with one per folded row (its four rows meet in the same words), 177 without any sums and 214 with
+// this.
 template <int CTRL, int BANKS = 0xf>
 DEVINL float moved(float y) {  // y moved inside rows of 16 lanes; zero from outside and in lanes of other banks of 4
   return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, y), CTRL, 0xf, BANKS, true));
@@ -556,7 +562,9 @@ struct Diagonals {
 // ---------------------------------------------------------------------------------------------------------------------
 // backward dQ and the bias gradient: workgroup = 64 queries of one head, 16 a wave
 //   P = exp2(S c - L);  dP = V dO^T;  dS = P (dP - D), D = rowsum(dO . O);  dQ^T += K^T dS;  dbias[j - p] += dS
-// Bound by instruction issue and the tile's dependent chain (vector 45 %, LDS 25 %, matrix pipe 25 %).  32 queries a wave: 49 us
+// Bound by the tile's dependent chain and its barrier: no pipe is above 45 % (vector 45 % at dh 80 with a bias, 39 at dh 64, 27 at
+// dh 128 without one and 2.4 waves a SIMD; LDS 17 to 33 %, matrix pipe 25 %).  B 8, H 12, n 1440, dh 128, all keys with a bias: 266 us,
+// B 4, window 257 without one: 41.  32 queries a wave: 49 us
 // instead of 38 (B 4, H 12, n 1440, dh 128, window 257), 231 instead of 237 where nothing but full tiles is left (B 8, all keys).
 // ---------------------------------------------------------------------------------------------------------------------
 template <int DH, bool REL>
@@ -814,7 +822,8 @@ DEVINL KBlock kblock_of(const RelP& p, int id) {
 // A wave has 16 keys and its four sums fit the registers of 4 (dh 128: 3) workgroups a CU.  With 32 keys a wave every Q and dO
 // fragment feeds two products, but two workgroups a CU are left: dh 64, B 2, H 12 on 4 key heads, n 2047, window 256 took 45.8 us
 // against 29.8; B 4, H 12, n 1440, window 257: 57 against 38; B 8, H 12, n 1440, all keys: 186 against 176 (dh 80: 222 and 214,
-// dh 32: 115 and 132, the one that lost).  What is left is latency: vector issue 40 %, LDS 27 %, matrix pipe 18 %.
+// dh 32: 115 and 132, the one that lost).  What is left is latency, as in dQ: vector issue 26 to 40 %, LDS 21 to 40 %, matrix pipe
+// 18 %.  B 8, H 12, n 1440, dh 128, all keys with a bias: 305 us; B 4, window 257 without one: 56 and the join 5.
 constexpr int BLOCK_KEYS = 64;
 constexpr int dkdv_slots(int dh) { return dh <= 96 ? 4 : 3; }  // workgroups of a CU
 template <int DH, bool REL>
