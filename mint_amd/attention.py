@@ -21,14 +21,16 @@ from mint_amd import _lib as L
 
 AttentionSaved = collections.namedtuple("AttentionSaved", ["lse", "out_lo"])
 AttentionSaved.__doc__ = """What attention(training=True) leaves for the backward: the base-2 log-sum-exp of every row, fp32
-[batch, heads, queries], and - with a relative bias, or up to EXACT_KEYS keys - the fp32 rounding residual of the output,
-[batch, queries, heads, dh]: the backward's row sums dO . O need it where they are added up (the fp32 gradient of the table) or
-rows average the rounding of few probabilities."""
+[batch, heads, queries], and - with a relative bias, up to EXACT_KEYS keys, or where a window and its sinks leave up to EXACT_WINDOW
+to a row - the fp32 rounding residual of the output, [batch, queries, heads, dh]: the backward's row sums dO . O need it where they
+are added up (the fp32 gradient of the table) or rows average the rounding of few probabilities."""
 
-# Without the residual dq and dk of 57 causal keys are 2.7e-3 off (norm), with it 2.35e-3, what the rounding of dS and of the result
-# costs.  The longer the rows, the less there is to gain - 2.38e-3 and 2.36e-3 at 512 keys - and the more it costs: two products more
-# in the forward (B 16, H 10, dh 80, 512 keys: 42 instead of 27 us).
-EXACT_KEYS = 512
+# The residual is worth its price where rows average the rounding of few probabilities: without it dq and dk of 2 keys a row are
+# 3.8e-3 off (norm), of 9 keys 2.65e-3, of 57 causal ones 2.7e-3, of 65 2.5e-3; with it all are 2.35e-3, what the rounding of dS and of
+# the result costs.  At 512 keys nothing is left of the gain (2.38e-3 and 2.36e-3).  It costs two products more in the forward: B 16,
+# H 10, dh 80, 512 keys 42 instead of 27 us, n 1440, H 12, dh 128, window +-8 27 + 60 us instead of 20 + 56.
+EXACT_KEYS = 512   # short sequences
+EXACT_WINDOW = 64  # and rows that see this many keys of a long one
 
 DTYPES = {torch.bfloat16: 0, torch.float32: 1}
 
@@ -253,7 +255,8 @@ def attention(q, k, v, scale=None, window=None, sinks=0, rel_table=None, rel_map
     saved = None
     if training:
         lse = torch.empty((a.B, a.H, a.nq), dtype=torch.float32, device=dev)
-        exact = rel_table is not None or a.nk <= EXACT_KEYS
+        narrow = min(a.window_left, a.window_right) >= 0 and a.window_left + 1 + a.window_right + a.sinks <= EXACT_WINDOW
+        exact = rel_table is not None or a.nk <= EXACT_KEYS or narrow
         lo = torch.empty(shape, dtype=torch.float32, device=dev) if exact else None
         saved = AttentionSaved(lse, lo)
         a.lse, a.out_lo = lse.data_ptr(), _p(lo)

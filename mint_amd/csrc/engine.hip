@@ -611,8 +611,9 @@ void layout_stack_acts(FactHandle* h, Bump& b, Stack& st, int B) {
     }
     for (int w = 0; w < 2; ++w)
       a.nrow[w] = (st.at.qk_norm && h->training) ? b.take<bf16_t>(BH * st.NP * st.dhp) : a.row[w];
-    // (short sequences gain from it without a bias too: FactAttention.out_lo)
-    if (st.ext() && h->training && (st.at.rel_buckets > 0 || st.n <= 512)) a.out_lo = b.take<float>(M * st.d);
+    // (rows of short sequences and of narrow windows gain from it without a bias too: FactAttention.out_lo)
+    const bool narrow = st.at.window > 0 && 2ll * st.at.window + 1 + st.at.sinks <= 64;
+    if (st.ext() && h->training && (st.at.rel_buckets > 0 || st.n <= 512 || narrow)) a.out_lo = b.take<float>(M * st.d);
     a.lse2 = b.take<float>(BH * st.NP);
   }
   float* pp[2] = {nullptr, nullptr};
